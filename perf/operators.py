@@ -289,7 +289,7 @@ def _plain_verify(st):
     total = res.sum(1)
     res = torch.where(total[:, None] == 0, p, res)
     total = torch.where(total == 0, zf, total)
-    t = _scale_draw((u[first] * 2.0**53).long(), total)
+    t = _scale_draw((u[off[1:] - 1] * 2.0**53).long(), total)  # the last row's number draws
     tok = (torch.cumsum(res, 1) <= t[:, None]).sum(1)
     tok = torch.where(greedy[first], best[first], tok)
     here = first[seq_of]
