@@ -262,6 +262,104 @@ PB_API int pb_stop_check(const int64_t* tokens, int64_t n_rows, const int32_t* r
                          const int32_t* stop_ids, int32_t eos_id, int32_t max_model_len, int8_t* out_reason,
                          void* stream);
 
+/*
+ * Verification of drafted tokens (speculative decoding): no counterpart in the reference, which
+ * decodes one token a step. A sequence with d drafts owns d + 1 consecutive logits rows, the target's
+ * distributions at each draft's position and after the last; rows of sequence s are
+ * row_offsets[s] .. row_offsets[s + 1) - 1, row_offsets[0] = 0, at least one row a sequence.
+ *
+ *   logits       device [n_rows, vocab] as pb_sample's.
+ *   params       device pb_row_params[n_seqs]: the sequence's sampling parameters (`uniform` and
+ *                `rng` are not read).
+ *   drafts       device int64[n_rows]: drafts[r] is the draft that row r judges (not read at a
+ *                sequence's last row).
+ *   uniforms     device double[n_rows], in [0, 1): the row's random number. It decides the row's
+ *                draft; that of a sequence's last row draws the token after the accepted drafts,
+ *                wherever the sequence stops.
+ *   draft_probs  optional device [n_probs, vocab] (probs_dtype, rows probs_stride elements apart): the
+ *                draft model's distribution at every draft, in row order without the sequences' last
+ *                rows (row r of sequence s has draft_probs row r - s). Null: a draft is certain (its
+ *                distribution is one token), as drafts looked up in the prompt are.
+ *   kinds        which kinds of sequences the batch holds (PB_VERIFY_*, 0: any): a launch whose kind
+ *                is absent is left out. A sequence of a kind not named reports PB_ROW_INTERNAL.
+ *   out_tokens   device int64[n_rows]: from the sequence's first row on, its accepted drafts and the
+ *                token drawn after them, then -1. A sequence whose status is not PB_ROW_OK has no
+ *                drawn token (-1 there).
+ *   out_accepted device int32[n_seqs]: accepted drafts.
+ *   out_status   optional device int32[n_seqs]: PB_ROW_* of the row where the sequence stopped.
+ *
+ * Semantics, per row, with P_i = q_i on the kept set of pb_sample's rule, Z = sum P (kept_q), x the
+ * draft, u = floor(uniform * 2^53) / 2^53 and D_i the draft distribution (D_x = 1 without one):
+ *   accept x iff (u * D_x) * Z < P_x, in fp64, every conversion and product rounded to nearest
+ *   (greedy rows: iff x is the row's first maximum; a draft outside [0, vocab) is never accepted);
+ *   at the first row that does not accept, draw from max(0, P_i - floor(D_i * Z)) (fp64 product; 0
+ *   for D_i <= 0 or NaN), or without a distribution from P without x; with every draft accepted
+ *   draw from P at the last row; where those weights are all 0, from P.
+ *   draw: the first index, ascending, whose inclusive prefix of the weights exceeds
+ *   floor(u * 2^53 * sum / 2^53), u of the sequence's last row (the sampler draws in the order of falling probability instead).
+ * workspace: pb_verify_ws_bytes(n_rows, vocab, dtype) bytes of device memory, 256-byte aligned, of any
+ * content, not used by another call while this one runs.
+ */
+#define PB_VERIFY_SMALL 1 /* greedy, or 0 < top_k <= 128 */
+#define PB_VERIFY_WHOLE 2 /* neither top-k nor top-p */
+#define PB_VERIFY_OTHER 4 /* any other parameters */
+#define PB_VERIFY_ANY 7
+PB_API int64_t pb_verify_ws_bytes(int64_t n_rows, int64_t vocab, int dtype);
+PB_API int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                     const pb_row_params* params, int64_t n_seqs, const int32_t* row_offsets, const int64_t* drafts,
+                     const double* uniforms, const void* draft_probs, int probs_dtype, int64_t n_probs,
+                     int64_t probs_stride, int kinds, int64_t* out_tokens, int32_t* out_accepted, int32_t* out_status,
+                     void* workspace, int64_t ws_bytes, void* stream);
+
+/*
+ * The k largest log-probabilities of every row (1 <= k <= PB_TOP_MAX and k <= vocab), their indices
+ * and the row's log-sum-exp, in one launch: what a server returns beside a token, and what a teacher
+ * records for pb_distill_forward. No counterpart in the reference.
+ *   y_j = x_j / temperature (2^-20 .. 2^20), lse = log sum exp(y), logprob = y - lse
+ *   order: value descending (NaN first), index ascending on ties
+ * A row with a NaN or +inf logit, or only -inf, has NaN log-probabilities (its indices still follow
+ * the order). row_stride may be anything from 0 (every row the same) up.
+ *   out_logprob  device float[n_rows * k];  out_index  device int32[n_rows * k];  out_lse  device float[n_rows]
+ */
+#define PB_TOP_MAX 256
+PB_API int pb_top_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride, int32_t k,
+                           float temperature, float* out_logprob, int32_t* out_index, float* out_lse, void* stream);
+
+/*
+ * Distillation of student logits rows from a teacher's top entries: the loss of every row, and its
+ * gradient. No counterpart in the reference.
+ *   entries      teacher[r * teacher_stride + i] (float) and indices[r * index_stride + i] (int32 or
+ *                int64 by index_bytes), i < n_entries <= PB_DISTILL_MAX_ENTRIES. Index -1: padding.
+ *   temperature  tau, 2^-20 .. 2^20; y = logits / tau, s = softmax(y) over the row.
+ *   tail == 0    t = softmax of the entries' values; loss = sum t (log t - log s).
+ *   tail != 0    t = exp(value), T = max(0, 1 - sum t), S = sum of s outside the entries; the loss gains
+ *                T (log T - log S) (left out where S < 2^-1000: logits masked with -inf or the type's
+ *                lowest value).
+ *   row_weight   optional device float[n_rows]; the loss and the gradient are times it.
+ * A row without entries (tail == 0: without an entry above -inf) or of weight 0 has loss 0 and
+ * gradient 0, whatever its logits. An index outside [-1, vocab) makes the row's loss NaN (and its
+ * gradient, unless its incoming gradient is 0: then the gradient is 0, as for every row). Entries that
+ * name the same element add up. vocab <= PB_DISTILL_MAX_VOCAB; row_stride may be 0 (rows shared).
+ *   out_loss     device float[n_rows]
+ *   stats        device, pb_distill_stats_bytes(n_rows), 16-byte aligned: written by the forward, read
+ *                by the backward with the same rows, entries, temperature and weights
+ *   grad_loss    device float, the incoming gradient of row r at grad_loss[r * grad_stride] (stride 0:
+ *                one for all rows)
+ *   out_grad     device [n_rows, vocab] of the logits' type, contiguous
+ */
+#define PB_DISTILL_MAX_ENTRIES 1024
+#define PB_DISTILL_MAX_VOCAB (1 << 20)
+PB_API int64_t pb_distill_stats_bytes(int64_t n_rows);
+PB_API int pb_distill_forward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                              const float* teacher, int64_t teacher_stride, const void* indices, int64_t index_stride,
+                              int index_bytes, int32_t n_entries, float temperature, int tail, const float* row_weight,
+                              float* out_loss, void* out_stats, void* stream);
+PB_API int pb_distill_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                               const float* teacher, int64_t teacher_stride, const void* indices, int64_t index_stride,
+                               int index_bytes, int32_t n_entries, float temperature, const float* row_weight,
+                               const void* stats, const float* grad_loss, int64_t grad_stride, void* out_grad,
+                               void* stream);
+
 /* Order-preserving 32-bit key of a float (NaN above +inf, -0 == +0); host helper for tests. */
 PB_API uint32_t pb_key_of(float x);
 

@@ -71,6 +71,8 @@ def lib() -> ctypes.CDLL:
         L.pbo_key_value.restype = ctypes.c_float
         L.pbo_philox4x32_10.argtypes = [vp, vp, vp]
         L.pbo_philox4x32_10.restype = None
+        L.pbo_weights.argtypes = [vp, i64, ctypes.c_float, vp]
+        L.pbo_weights.restype = None
         L.pbo_row_u53.argtypes = [vp, vp]
         L.pbo_row_u53.restype = i32
         _lib = L

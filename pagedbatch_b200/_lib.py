@@ -24,6 +24,9 @@ ROW_FALLBACK = 32
 CAND_FALLBACK, CAND_GREEDY, CAND_MAX_CAP = 0x100, 0x200, 2048
 PATH_GREEDY, PATH_SMALL, PATH_LARGE, PATH_STREAM = 1, 2, 4, 8
 FINISH_NONE, FINISH_STOP, FINISH_LENGTH = 0, 1, 2
+VERIFY_SMALL, VERIFY_WHOLE, VERIFY_OTHER, VERIFY_ANY = 1, 2, 4, 7
+TOP_MAX = 256
+DISTILL_MAX_ENTRIES, DISTILL_MAX_VOCAB = 1024, 1 << 20
 MAX_VOCAB = 1 << 24
 
 # struct pb_row_params / pb_row_info (include/pagedbatch_b200.h)
@@ -69,6 +72,12 @@ EXPORTS = (
     "pb_exp",
     "pb_philox_u53",
     "pb_stop_check",
+    "pb_verify",
+    "pb_verify_ws_bytes",
+    "pb_top_logprobs",
+    "pb_distill_forward",
+    "pb_distill_backward",
+    "pb_distill_stats_bytes",
     "pb_philox4x32_10",
     "pb_strerror",
     "pb_version",
@@ -127,6 +136,19 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     L.pb_exp.restype = ctypes.c_float
     L.pb_stop_check.argtypes = [vp, i64, vp, vp, vp, i32, i32, vp, vp]
     L.pb_stop_check.restype = i32
+    f32 = ctypes.c_float
+    L.pb_verify_ws_bytes.argtypes = [i64, i64, i32]
+    L.pb_verify_ws_bytes.restype = i64
+    L.pb_verify.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, i32, i64, i64, i32, vp, vp, vp, vp, i64, vp]
+    L.pb_verify.restype = i32
+    L.pb_top_logprobs.argtypes = [vp, i32, i64, i64, i64, i32, f32, vp, vp, vp, vp]
+    L.pb_top_logprobs.restype = i32
+    L.pb_distill_stats_bytes.argtypes = [i64]
+    L.pb_distill_stats_bytes.restype = i64
+    L.pb_distill_forward.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, i64, i32, i32, f32, i32, vp, vp, vp, vp]
+    L.pb_distill_forward.restype = i32
+    L.pb_distill_backward.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, i64, i32, i32, f32, vp, vp, vp, i64, vp, vp]
+    L.pb_distill_backward.restype = i32
     L.pb_philox_u53.argtypes = [ctypes.c_uint64, ctypes.c_uint32]
     L.pb_philox_u53.restype = ctypes.c_uint64
     L.pb_philox4x32_10.argtypes = [vp, vp, vp]

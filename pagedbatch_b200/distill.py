@@ -1,0 +1,118 @@
+"""Distillation of a draft model from a teacher's top entries: the loss of each row of student logits
+and its gradient, in one pass over the logits each way. The reference does not train
+(pagedbatch has no optimiser) and has no counterpart.
+
+The teacher's record of a row is what ``top_logprobs`` returns for it: K log-probabilities and token
+ids. Formulas and edge cases are stated at ``pb_distill_forward`` in ``include/pagedbatch_b200.h``.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+from .logprobs import check_temperature
+
+__all__ = ["distill_loss"]
+
+
+def _entries(idx: torch.Tensor, lp: torch.Tensor):
+    return lp.data_ptr(), lp.stride(0), idx.data_ptr(), idx.stride(0), idx.element_size(), idx.shape[1]
+
+
+def _forward(z, lp, idx, weight, temperature, tail):
+    n, V = z.shape
+    L = _lib.load()
+    loss = torch.empty(n, dtype=torch.float32, device=z.device)
+    with torch.cuda.device(z.device):
+        stats = torch.empty(L.pb_distill_stats_bytes(n), dtype=torch.uint8, device=z.device)
+        rc = L.pb_distill_forward(
+            z.data_ptr(), ops._DTYPE_CODE[z.dtype], n, V, z.stride(0), *_entries(idx, lp), temperature, int(tail),
+            weight.data_ptr() if weight is not None else None, loss.data_ptr(), stats.data_ptr(),
+            torch.cuda.current_stream(z.device).cuda_stream)
+    _lib.check(rc, "pb_distill_forward")
+    return loss, stats
+
+
+def _backward(z, lp, idx, weight, stats, grad_loss, temperature):
+    n, V = z.shape
+    L = _lib.load()
+    dz = torch.empty((n, V), dtype=z.dtype, device=z.device)
+    with torch.cuda.device(z.device):
+        rc = L.pb_distill_backward(
+            z.data_ptr(), ops._DTYPE_CODE[z.dtype], n, V, z.stride(0), *_entries(idx, lp), temperature,
+            weight.data_ptr() if weight is not None else None, stats.data_ptr(), grad_loss.data_ptr(),
+            grad_loss.stride(0), dz.data_ptr(), torch.cuda.current_stream(z.device).cuda_stream)
+    _lib.check(rc, "pb_distill_backward")
+    return dz
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, lp, idx, weight, temperature, tail):
+        loss, stats = _forward(z, lp, idx, weight, temperature, tail)
+        ctx.save_for_backward(z, lp, idx, weight, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        z, lp, idx, weight, stats = ctx.saved_tensors
+        # a gradient of one value for all rows (from a sum or mean) is read through its stride of 0
+        return _backward(z, lp, idx, weight, stats, grad_loss, ctx.temperature), None, None, None, None, None
+
+
+def distill_loss(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_indices: torch.Tensor, *,
+                 temperature: float = 1.0, tail: bool = False, row_weight: torch.Tensor | None = None,
+                 reduction: str = "none") -> torch.Tensor:
+    """KL divergence of the student's distribution from the teacher's, per row of ``student_logits
+    [n, V]`` (CUDA, float32 / bfloat16 / float16, last dim contiguous, V at most 2^20): float32 ``[n]``,
+    or their sum with ``reduction="sum"``. Differentiable in ``student_logits`` (once).
+
+    * ``teacher_logprobs [n, K]`` (K at most 1024) and ``teacher_indices [n, K]`` (int32 or int64): the
+      teacher's entries, index -1 for padding. The teacher's distribution is the softmax of the entries'
+      values (any constant per row may be added to them), or with ``tail=True`` their exponentials, the
+      rest of the mass being compared with the student's mass outside the entries.
+    * ``temperature`` divides the student's logits (the teacher's entries are at it already; multiply
+      the loss by its square for the usual scaling).
+    * ``row_weight float32[n]``: a factor of each row's loss. Rows of weight 0, and rows whose entries
+      are all padding, have loss and gradient 0 whatever their logits hold.
+
+    An index outside [-1, V) makes its row's loss NaN."""
+    z, lp, idx = student_logits, teacher_logprobs, teacher_indices
+    if not z.is_cuda:
+        raise ValueError("pagedbatch_b200.distill_loss needs CUDA logits; move the tensor with .cuda() first")
+    if z.dim() != 2 or (z.stride(1) != 1 and z.shape[1] > 1):
+        raise ValueError("student_logits must be a [rows, vocab] tensor with a contiguous last dimension")
+    if z.dtype not in ops._DTYPE_CODE:
+        raise ValueError(f"unsupported student_logits dtype {z.dtype}")
+    n, V = z.shape
+    if not 1 <= V <= _lib.DISTILL_MAX_VOCAB:
+        raise ValueError(f"the vocabulary must hold 1 to {_lib.DISTILL_MAX_VOCAB} tokens, got {V}")
+    if lp.dim() != 2 or lp.shape[0] != n or not 1 <= lp.shape[1] <= _lib.DISTILL_MAX_ENTRIES:
+        raise ValueError(f"teacher_logprobs must be [{n}, K] with K in [1, {_lib.DISTILL_MAX_ENTRIES}]")
+    if lp.dtype not in ops._DTYPE_CODE:
+        raise ValueError(f"unsupported teacher_logprobs dtype {lp.dtype}")
+    if idx.shape != lp.shape or idx.dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_indices must be int32 or int64, of teacher_logprobs' shape")
+    if lp.requires_grad or (row_weight is not None and row_weight.requires_grad):
+        raise ValueError("the teacher's entries and the row weights take no gradient: detach them")
+    if row_weight is not None and (row_weight.dtype != torch.float32 or row_weight.shape != (n,)):
+        raise ValueError(f"row_weight must be a float32 tensor of {n} values")
+    for name, t in (("teacher_logprobs", lp), ("teacher_indices", idx), ("row_weight", row_weight)):
+        if t is not None and t.device != z.device:
+            raise ValueError(f"{name} must be on the logits' device {z.device}")
+    if reduction not in ("none", "sum"):
+        raise ValueError(f"reduction must be 'none' or 'sum', got {reduction!r}")
+    t = check_temperature(temperature)
+    lp = lp.float()
+    if lp.stride(1) != 1:
+        lp = lp.contiguous()
+    if idx.stride(1) != 1:
+        idx = idx.contiguous()
+    if row_weight is not None:
+        row_weight = row_weight.contiguous()
+    loss = _Distill.apply(z, lp, idx, row_weight, t, bool(tail))
+    return loss.sum() if reduction == "sum" else loss

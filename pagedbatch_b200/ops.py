@@ -67,9 +67,23 @@ def group_rows(rec: np.ndarray) -> tuple[bool, int]:
     return ok, kmax
 
 
+def row_kinds(rec: np.ndarray) -> tuple[int, int]:
+    """Which kinds of rows the records hold (PB_VERIFY_* bits), taking every top_k as below the
+    vocabulary, and the largest top_k that has to be for that to be so."""
+    t, p, k = rec["temperature"], rec["top_p"], rec["top_k"]
+    valid = (t >= 0.0) & (p > 0.0) & (p <= 1.0) & (k >= 0)
+    greedy = valid & (t == 0.0)
+    small = greedy | (valid & (k > 0) & (k <= GROUP_KMAX))
+    whole = valid & ~small & (k == 0) & (p.astype(np.float32) >= 1.0)
+    bits = (_lib.VERIFY_SMALL * bool(small.any()) | _lib.VERIFY_WHOLE * bool(whole.any())
+            | _lib.VERIFY_OTHER * bool((~small & ~whole).any()))
+    return bits, int(k[~greedy].max()) if np.any(~greedy) else 0
+
+
 def mark_rows(params: torch.Tensor, rec: np.ndarray) -> torch.Tensor:
     """Record on the device params tensor which launch suits its rows (read by the path choice)."""
     params._pb_group_rows = group_rows(rec)
+    params._pb_kinds = row_kinds(rec)
     return params
 
 

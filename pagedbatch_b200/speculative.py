@@ -1,0 +1,178 @@
+"""Verification of drafted tokens: several tokens a step from one pass of the target model.
+
+A draft model (or a lookup in the prompt) proposes a few tokens for each sequence, the target model
+computes its logits at every drafted position in one forward pass, and ``verify`` accepts a prefix of
+the drafts and draws one more token, so that the tokens are distributed exactly as the target's own
+samples (``sample_tokens`` with the same ``SamplingParams``) are. The reference decodes one token a
+step (pagedbatch/engine.py:130-171) and has no counterpart.
+
+Layout: the sequences' rows follow one another; a sequence with ``d`` drafts owns ``d + 1`` rows, row
+``j`` being the target's distribution at its ``j``-th draft and the last one that after all of them.
+The rule, its arithmetic and the order of the draws are stated at ``pb_verify`` in
+``include/pagedbatch_b200.h``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from collections.abc import Sequence
+
+import numpy as np
+import torch
+
+from . import _lib, ops
+from .sampling import _INVALID_DISTRIBUTION, pack_rows
+
+__all__ = ["verify", "verify_tokens"]
+
+
+def _kinds(params: torch.Tensor, vocab: int) -> int:
+    bits, kmax = getattr(params, "_pb_kinds", (0, 0))
+    return bits if kmax < vocab else 0  # a top_k of the vocabulary or more is no filter: any kind
+
+
+def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs):
+    if not logits.is_cuda:
+        raise ValueError("pagedbatch_b200.verify needs CUDA logits; move the tensor with .cuda() first")
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be a [rows, vocab] tensor with a contiguous last dimension")
+    if logits.dtype not in ops._DTYPE_CODE:
+        raise ValueError(f"unsupported logits dtype {logits.dtype}")
+    if params.dtype != torch.uint8 or params.numel() % _lib.ROW_PARAMS.itemsize or not params.is_contiguous():
+        raise ValueError("params must be packed pb_row_params records (uint8), one per sequence")
+    dev = logits.device
+    R, V = logits.shape
+    S = params.numel() // _lib.ROW_PARAMS.itemsize
+    for name, t, dtype, n in (("drafts", drafts, torch.int64, R), ("row_offsets", row_offsets, torch.int32, S + 1),
+                              ("uniforms", uniforms, torch.float64, R)):
+        if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values")
+    for name, t in (("params", params), ("drafts", drafts), ("row_offsets", row_offsets), ("uniforms", uniforms),
+                    ("draft_probs", draft_probs)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} must be on the logits' device {dev}")
+    if S > R:
+        raise ValueError(f"{S} sequences for {R} rows: every sequence has at least one row")
+    if draft_probs is not None:
+        if draft_probs.dim() != 2 or draft_probs.shape != (R - S, V) or (draft_probs.stride(1) != 1 and V > 1):
+            raise ValueError(f"draft_probs must be [{R - S}, {V}] with a contiguous last dimension: a row per draft")
+        if draft_probs.dtype not in ops._DTYPE_CODE:
+            raise ValueError(f"unsupported draft_probs dtype {draft_probs.dtype}")
+    tokens = torch.empty(R, dtype=torch.int64, device=dev)
+    accepted = torch.empty(S, dtype=torch.int32, device=dev)
+    status = torch.empty(S, dtype=torch.int32, device=dev)
+    if S == 0:
+        if R:
+            raise ValueError(f"{R} rows for no sequence")
+        return tokens, accepted, status
+    L = _lib.load()
+    code = ops._DTYPE_CODE[logits.dtype]
+    with torch.cuda.device(dev):
+        # a buffer of this call's own: the allocator hands it on in stream order, and a captured
+        # graph keeps its copy
+        ws = torch.empty(L.pb_verify_ws_bytes(R, V, code), dtype=torch.uint8, device=dev)
+        rc = L.pb_verify(
+            logits.data_ptr(), code, R, V, logits.stride(0) if R > 1 else V, params.data_ptr(), S,
+            row_offsets.data_ptr(), drafts.data_ptr(), uniforms.data_ptr(),
+            draft_probs.data_ptr() if draft_probs is not None and R > S else None,
+            ops._DTYPE_CODE[draft_probs.dtype] if draft_probs is not None else 0, R - S,
+            draft_probs.stride(0) if draft_probs is not None and R - S > 1 else V, _kinds(params, V),
+            tokens.data_ptr(), accepted.data_ptr(), status.data_ptr(), ws.data_ptr(), ws.numel(),
+            torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "pb_verify")
+    return tokens, accepted, status
+
+
+@torch.library.custom_op("pagedbatch_b200::verify", mutates_args=())
+def verify_op(logits: torch.Tensor, params: torch.Tensor, drafts: torch.Tensor, row_offsets: torch.Tensor,
+              uniforms: torch.Tensor, draft_probs: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Tokens and accepted counts."""
+    tokens, accepted, _ = _launch(logits, params, drafts, row_offsets, uniforms, draft_probs)
+    return tokens, accepted
+
+
+@verify_op.register_fake
+def _(logits, params, drafts, row_offsets, uniforms, draft_probs=None):
+    s = params.numel() // _lib.ROW_PARAMS.itemsize
+    return logits.new_empty((logits.shape[0],), dtype=torch.int64), logits.new_empty((s,), dtype=torch.int32)
+
+
+def verify(logits: torch.Tensor, params: torch.Tensor, drafts: torch.Tensor, row_offsets: torch.Tensor,
+           uniforms: torch.Tensor, draft_probs: torch.Tensor | None = None, with_status: bool = False):
+    """Verify the drafts of ``S`` sequences against their ``R`` target rows, on the device and without
+    a host read: ``(tokens int64[R], accepted int32[S])``.
+
+    * ``logits [R, V]``: CUDA, float32 / bfloat16 / float16, last dim contiguous;
+    * ``params``: one packed ``pb_row_params`` record per sequence (``ops.params_tensor``), which may be
+      kept from step to step (their ``uniform`` is not used);
+    * ``drafts int64[R]``: the draft each row judges (ignored at a sequence's last row);
+    * ``row_offsets int32[S + 1]``: sequence ``s`` owns rows ``row_offsets[s]`` to ``row_offsets[s + 1] - 1``;
+      it starts at 0, ends at R and gives every sequence at least one row (not checked on the host);
+    * ``uniforms float64[R]``: one random number in [0, 1) per row. It decides the row's draft; that of a
+      sequence's last row draws the token after the accepted drafts;
+    * ``draft_probs [R - S, V]``: the draft model's distribution at each draft, in row order (float32 /
+      bfloat16 / float16), as ``ops.sample(..., with_probs=True)`` returns it. ``None``: the drafts are
+      certain (looked up, or a greedy draft model).
+
+    ``tokens`` holds, from each sequence's first row on, its accepted drafts and the token drawn after
+    them, then -1. ``with_status`` adds ``int32[S]`` status codes (``PB_ROW_*``; where it is not 0 the
+    drawn token is -1). Runs on the current stream of the logits' device and can be captured."""
+    out = _launch(logits, params, drafts, row_offsets, uniforms, draft_probs)
+    return out if with_status else out[:2]
+
+
+def verify_tokens(logits: torch.Tensor, drafts: Sequence[Sequence[int]], params: Sequence,
+                  generators: Sequence[torch.Generator], draft_probs: torch.Tensor | None = None) -> list[list[int]]:
+    """The tokens of one verified step, per sequence: its accepted drafts and the one drawn after them.
+
+    ``drafts[s]`` are sequence ``s``'s drafted token ids, ``params[s]`` its ``SamplingParams``;
+    ``logits [R, V]`` holds ``len(drafts[s]) + 1`` rows for each sequence, one after another. A sequence that is
+    not greedy takes ``len(drafts[s]) + 1`` float64 draws from its generator. CPU logits are copied to
+    the current CUDA device first, as in ``sample_tokens``."""
+    S = len(drafts)
+    if len(params) != S or len(generators) != S:
+        raise ValueError(f"{len(params)} params and {len(generators)} generators for {S} sequences")
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
+    V = logits.shape[1]
+    lens = np.array([len(d) for d in drafts], dtype=np.int64)
+    offsets = np.zeros(S + 1, dtype=np.int32)
+    np.cumsum(lens + 1, out=offsets[1:])
+    R = int(offsets[-1])
+    if logits.shape[0] != R:
+        raise ValueError(f"{logits.shape[0]} logits rows for {R} (one per draft and one more per sequence)")
+    flat = np.zeros(R, dtype=np.int64)
+    for s, d in enumerate(drafts):
+        flat[offsets[s] : offsets[s] + len(d)] = d
+    if R and (flat.min() < 0 or flat.max() >= V):
+        raise ValueError(f"drafts must be token ids in [0, {V})")
+    rec = pack_rows(params, np.zeros(S))
+    if S == 0:
+        return []
+    uniforms = np.zeros(R)
+    for s, (p, g) in enumerate(zip(params, generators, strict=True)):
+        if p.temperature != 0:
+            n = int(lens[s]) + 1
+            uniforms[offsets[s] : offsets[s] + n] = torch.rand(n, dtype=torch.float64, generator=g).numpy()
+    if not logits.is_cuda:
+        if not torch.cuda.is_available():
+            raise RuntimeError("pagedbatch_b200 verifies on a CUDA device and none is available")
+        logits = logits.to(torch.cuda.current_device(), non_blocking=logits.is_pinned())
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    # parameters, random numbers, drafts and offsets in one pinned buffer and one copy
+    parts = [rec.view(np.uint8).reshape(-1), uniforms.view(np.uint8), flat.view(np.uint8), offsets.view(np.uint8)]
+    ends = np.cumsum([p.size for p in parts])
+    host = torch.empty(int(ends[-1]), dtype=torch.uint8, pin_memory=True)
+    np.concatenate(parts, out=host.numpy())
+    dev = host.to(logits.device, non_blocking=True)
+    tokens, accepted, status = _launch(
+        logits, ops.mark_rows(dev[: ends[0]], rec), dev[ends[1] : ends[2]].view(torch.int64),
+        dev[ends[2] : ends[3]].view(torch.int32), dev[ends[0] : ends[1]].view(torch.float64), draft_probs)
+    got, n_ok, st = tokens.tolist(), accepted.tolist(), status.tolist()
+    for s, code in enumerate(st):
+        if code == _lib.ROW_NONFINITE:
+            raise RuntimeError(_INVALID_DISTRIBUTION)
+        if code != _lib.ROW_OK:
+            raise RuntimeError(f"verification failed on sequence {s} (status {code})")
+    return [got[offsets[s] : offsets[s] + n_ok[s] + 1] for s in range(S)]
