@@ -313,17 +313,21 @@ PB_API int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t voca
 
 /*
  * The k largest log-probabilities of every row (1 <= k <= PB_TOP_MAX and k <= vocab), their indices
- * and the row's log-sum-exp, in one launch: what a server returns beside a token, and what a teacher
+ * and the row's log-sum-exp: what a server returns beside a token, and what a teacher
  * records for pb_distill_forward. No counterpart in the reference.
  *   y_j = x_j / temperature (2^-20 .. 2^20), lse = log sum exp(y), logprob = y - lse
  *   order: value descending (NaN first), index ascending on ties
  * A row with a NaN or +inf logit, or only -inf, has NaN log-probabilities (its indices still follow
  * the order). row_stride may be anything from 0 (every row the same) up.
  *   out_logprob  device float[n_rows * k];  out_index  device int32[n_rows * k];  out_lse  device float[n_rows]
+ * workspace: pb_top_ws_bytes(n_rows, vocab, dtype) bytes of device memory, 256-byte aligned, of any
+ * content, not used by another call while this one runs.
  */
 #define PB_TOP_MAX 256
+PB_API int64_t pb_top_ws_bytes(int64_t n_rows, int64_t vocab, int dtype);
 PB_API int pb_top_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride, int32_t k,
-                           float temperature, float* out_logprob, int32_t* out_index, float* out_lse, void* stream);
+                           float temperature, float* out_logprob, int32_t* out_index, float* out_lse, void* workspace,
+                           int64_t ws_bytes, void* stream);
 
 /*
  * Distillation of student logits rows from a teacher's top entries: the loss of every row, and its
@@ -346,19 +350,24 @@ PB_API int pb_top_logprobs(const void* logits, int dtype, int64_t n_rows, int64_
  *   grad_loss    device float, the incoming gradient of row r at grad_loss[r * grad_stride] (stride 0:
  *                one for all rows)
  *   out_grad     device [n_rows, vocab] of the logits' type, contiguous
+ *   workspace    device, pb_distill_ws_bytes(n_rows, vocab, dtype), 16-byte aligned, of any content, not
+ *                used by another call while this one runs
+ * pb_distill_sum: the sum of the rows' losses (64-bit accumulation, fixed order), float[1].
  */
 #define PB_DISTILL_MAX_ENTRIES 1024
 #define PB_DISTILL_MAX_VOCAB (1 << 20)
 PB_API int64_t pb_distill_stats_bytes(int64_t n_rows);
+PB_API int64_t pb_distill_ws_bytes(int64_t n_rows, int64_t vocab, int dtype);
 PB_API int pb_distill_forward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
                               const float* teacher, int64_t teacher_stride, const void* indices, int64_t index_stride,
                               int index_bytes, int32_t n_entries, float temperature, int tail, const float* row_weight,
-                              float* out_loss, void* out_stats, void* stream);
+                              float* out_loss, void* out_stats, void* workspace, int64_t ws_bytes, void* stream);
 PB_API int pb_distill_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
                                const float* teacher, int64_t teacher_stride, const void* indices, int64_t index_stride,
                                int index_bytes, int32_t n_entries, float temperature, const float* row_weight,
                                const void* stats, const float* grad_loss, int64_t grad_stride, void* out_grad,
                                void* stream);
+PB_API int pb_distill_sum(const float* loss, int64_t n_rows, float* out_sum, void* stream);
 
 /* Order-preserving 32-bit key of a float (NaN above +inf, -0 == +0); host helper for tests. */
 PB_API uint32_t pb_key_of(float x);

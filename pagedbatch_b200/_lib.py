@@ -75,9 +75,12 @@ EXPORTS = (
     "pb_verify",
     "pb_verify_ws_bytes",
     "pb_top_logprobs",
+    "pb_top_ws_bytes",
     "pb_distill_forward",
     "pb_distill_backward",
     "pb_distill_stats_bytes",
+    "pb_distill_ws_bytes",
+    "pb_distill_sum",
     "pb_philox4x32_10",
     "pb_strerror",
     "pb_version",
@@ -141,14 +144,20 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     L.pb_verify_ws_bytes.restype = i64
     L.pb_verify.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, i32, i64, i64, i32, vp, vp, vp, vp, i64, vp]
     L.pb_verify.restype = i32
-    L.pb_top_logprobs.argtypes = [vp, i32, i64, i64, i64, i32, f32, vp, vp, vp, vp]
+    L.pb_top_logprobs.argtypes = [vp, i32, i64, i64, i64, i32, f32, vp, vp, vp, vp, i64, vp]
     L.pb_top_logprobs.restype = i32
     L.pb_distill_stats_bytes.argtypes = [i64]
     L.pb_distill_stats_bytes.restype = i64
-    L.pb_distill_forward.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, i64, i32, i32, f32, i32, vp, vp, vp, vp]
+    L.pb_distill_forward.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, i64, i32, i32, f32, i32, vp, vp, vp, vp, i64, vp]
     L.pb_distill_forward.restype = i32
     L.pb_distill_backward.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, i64, i32, i32, f32, vp, vp, vp, i64, vp, vp]
     L.pb_distill_backward.restype = i32
+    L.pb_distill_ws_bytes.argtypes = [i64, i64, i32]
+    L.pb_distill_ws_bytes.restype = i64
+    L.pb_top_ws_bytes.argtypes = [i64, i64, i32]
+    L.pb_top_ws_bytes.restype = i64
+    L.pb_distill_sum.argtypes = [vp, i64, vp, vp]
+    L.pb_distill_sum.restype = i32
     L.pb_philox_u53.argtypes = [ctypes.c_uint64, ctypes.c_uint32]
     L.pb_philox_u53.restype = ctypes.c_uint64
     L.pb_philox4x32_10.argtypes = [vp, vp, vp]

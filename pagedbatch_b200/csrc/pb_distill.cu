@@ -11,24 +11,20 @@
 //              = (1 / tau) (A s_j - T s_j / S)                    for the others
 // A row without an entry of weight, and a row whose row weight is 0, has loss 0 and gradient 0.
 //
-// Forward: one cluster of C CTAs per row, each reading its slice of the row once, with a running
-// maximum and sum of exponentials per thread. For the tail bucket the entries are kept out of that
-// sum exactly (a bit per element of the slice in shared memory), so S has no cancellation however
-// sure the student is. Backward: one pass, z in and dz out, on the statistics of the forward.
-// Both are bound by HBM: V * es bytes a row forward, twice that backward.
+// Forward, two launches: part_kernel reads every row once, a CTA per segment of it, with a running
+// maximum and sum of exponentials; finish_kernel, one warp per row, joins the segments and takes the
+// loss from the row's entries. For the tail bucket the entries are kept out of the sums exactly (a bit
+// per element of the segment in shared memory), so S has no cancellation however sure the student is.
+// Backward: one launch, z in and dz out, on the statistics of the forward. Both passes are bound by
+// HBM: V * es bytes a row forward, twice that backward.
 #include "pb_rows.cuh"
 
 using namespace pb;
 
 namespace {
 
-constexpr int DT = 512;         // threads per CTA
-constexpr int DNW = DT / 32;
-constexpr int DU = 4;           // vectors each thread has in flight
-constexpr int DKMAX = PB_DISTILL_MAX_ENTRIES;     // entries per row
-constexpr int DEPT = DKMAX / DT;  // entries per thread
+constexpr int DKMAX = PB_DISTILL_MAX_ENTRIES;    // entries per row
 constexpr int64_t DVMAX = PB_DISTILL_MAX_VOCAB;  // logits per row (one bit each in shared memory)
-
 enum : int32_t { D_ROW = 0, D_EMPTY = 1, D_DUP = 2 };  // D_DUP: two entries name one element
 
 // log2 of the student's mass outside the entries below which there is none: logits there of -inf, or
@@ -45,6 +41,12 @@ struct alignas(16) RowStats {
   int32_t flags;       // D_*
 };
 
+// What a segment adds to its row.
+struct Part {
+  ExpSum rest, mem;  // sums outside the entries, over the segment's distinct entries
+  int32_t dup, pad;  // two entries name one of its elements
+};
+
 struct DistillArgs {
   const void* z;
   int64_t z_stride;  // elements
@@ -57,223 +59,19 @@ struct DistillArgs {
   const float* weight;  // per row, or null
   float* loss;          // forward: [n]
   RowStats* stats;      // [n]
+  Part* parts;          // [n][segs]
   const float* grad;    // backward: incoming gradient, row r at grad[r * grad_stride]
   int64_t grad_stride;
   void* dz;             // backward: [n][V]
   int64_t n;
   int32_t V, K;
   float c, inv_tau;     // log2(e) / tau, 1 / tau
-  int32_t chunks;       // backward: CTAs per row
+  SegPlan seg;
 };
 
 __device__ __forceinline__ int64_t entry_index(const DistillArgs& a, int64_t row, int i) {
   const int64_t at = row * a.idx_stride + i;
   return a.idx64 ? __ldg(static_cast<const long long*>(a.idx) + at) : (int64_t)__ldg(static_cast<const int*>(a.idx) + at);
-}
-
-struct FwdShared {
-  ExpSum red[DNW];
-  float fred[DNW];
-  ExpSum pub_rest, pub_mem;  // this CTA's sums: outside the entries, over its distinct entries
-  float pub_dot;             // this CTA's part of sum t (log t - log s)
-};
-
-template <typename T, bool TAIL>
-__global__ void __launch_bounds__(DT, 2) distill_forward_kernel(DistillArgs a) {
-  constexpr int EPV = Elem<T>::EPV;
-  extern __shared__ __align__(16) uint32_t mask[];  // a bit per element of the slice: an entry's
-  __shared__ FwdShared sh;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t row = blockIdx.x / C;
-  const int tid = threadIdx.x;
-  const RowView<T> rv(static_cast<const T*>(a.z) + row * a.z_stride, a.V);
-  const int32_t v0 = (int32_t)((int64_t)rv.nvec * rank / C), v1 = (int32_t)((int64_t)rv.nvec * (rank + 1) / C);
-  const int32_t words = ((v1 - v0) * EPV + 31) / 32;
-
-  for (int32_t w = tid; w < words; w += DT) mask[w] = 0;
-
-  // this thread's entries
-  int32_t ix[DEPT];
-  float lp[DEPT];
-  bool bad = false, any = false;
-  float mx = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < DEPT; ++j) {
-    const int i = tid + j * DT;
-    ix[j] = -1;
-    lp[j] = -INFINITY;
-    if (i < a.K) {
-      const int64_t e = entry_index(a, row, i);
-      if (e < -1 || e >= a.V) bad = true;
-      else if (e >= 0) {
-        ix[j] = (int32_t)e;
-        lp[j] = __ldg(a.lp + row * a.lp_stride + i);
-        any = true;
-        mx = fmaxf(mx, lp[j]);
-      }
-    }
-  }
-  // the entries' probabilities: t_i = exp(lp_i - norm)
-  float norm = 0.0f;
-  if (!TAIL) {
-    mx = block_max<DNW>(mx, sh.fred);
-    norm = (mx == -INFINITY) ? 0.0f : mx;
-  }
-  float t[DEPT], part = 0.0f;
-#pragma unroll
-  for (int j = 0; j < DEPT; ++j) {
-    t[j] = (ix[j] >= 0) ? expf(lp[j] - norm) : 0.0f;
-    part += t[j];
-  }
-  float sum_t = block_sum<DNW>(part, sh.fred);
-  const bool row_bad = __syncthreads_or(bad) != 0;
-  const bool row_any = __syncthreads_or(any) != 0;
-  // no entry, or (renormalised) none of any weight: a padded row
-  const float wt = a.weight ? __ldg(a.weight + row) : 1.0f;
-  const bool empty = !row_bad && (wt == 0.0f || !row_any || (!TAIL && sum_t == 0.0f));
-  if (empty) {  // the whole cluster: every CTA sees the same entries
-    if (rank == 0 && tid == 0) {
-      a.loss[row] = 0.0f;
-      a.stats[row] = RowStats{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, D_EMPTY};
-    }
-    return;
-  }
-  if (!TAIL) {
-    norm += logf(sum_t);
-    const float inv = 1.0f / sum_t;
-#pragma unroll
-    for (int j = 0; j < DEPT; ++j) t[j] *= inv;
-  }
-
-  // mark the slice's entries; the first to mark an element owns it (its term of the student's sum
-  // counts once, however many entries name it)
-  float z[DEPT];
-  bool own[DEPT], mine[DEPT], dup = false;
-#pragma unroll
-  for (int j = 0; j < DEPT; ++j) {
-    mine[j] = own[j] = false;
-    z[j] = 0.0f;
-    if (ix[j] >= 0) {
-      const int32_t v = (ix[j] + rv.off) / EPV;
-      if (v >= v0 && v < v1) {
-        mine[j] = true;
-        const uint32_t b = (uint32_t)(ix[j] + rv.off - v0 * EPV);
-        own[j] = !((atomicOr(&mask[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1u);
-        dup |= !own[j];
-        z[j] = Elem<T>::ld(rv.row + ix[j]);
-      }
-    }
-  }
-  // (this barrier also ends the marking)
-  const bool row_dup = __syncthreads_or(dup) != 0;
-
-  // the slice: a running maximum and sum of 2^(z c)
-  ExpSum acc = expsum_empty();
-  for (int32_t vb = v0; vb < v1; vb += DT * DU) {
-    uint4 q[DU];
-#pragma unroll
-    for (int u = 0; u < DU; ++u) {
-      const int32_t v = vb + u * DT + tid;
-      if (v < v1) q[u] = load_vec(rv, v);
-    }
-#pragma unroll
-    for (int u = 0; u < DU; ++u) {
-      const int32_t v = vb + u * DT + tid;
-      if (v < v1) {
-        float x[EPV];
-        Elem<T>::unpack(q[u], x);
-        if constexpr (TAIL) {
-          const int32_t b = (v - v0) * EPV;
-          uint32_t bits = (mask[b >> 5] >> (b & 31)) & ((1u << EPV) - 1u);
-          if (bits) {
-#pragma unroll
-            for (int e = 0; e < EPV; ++e)
-              if ((bits >> e) & 1u) x[e] = -INFINITY;
-          }
-        }
-        expsum_add<T>(acc, x, a.c);
-      }
-    }
-  }
-  ExpSum rest = block_expsum<DNW>(acc, a.c, sh.red);
-  ExpSum mem = expsum_empty();
-  if constexpr (TAIL) {
-#pragma unroll
-    for (int j = 0; j < DEPT; ++j)
-      if (own[j]) {
-        // (a NaN or +inf logit makes the sum NaN, as in the stream)
-        const float m = fmaxf(LOWEST, z[j]);
-        mem = expsum_join(mem, ExpSum{m, ex2((z[j] - m) * a.c)}, a.c);
-      }
-    mem = block_expsum<DNW>(mem, a.c, sh.red);
-  }
-  if (tid == 0) {
-    sh.pub_rest = rest;
-    sh.pub_mem = mem;
-  }
-  cluster_barrier(C);
-  if (C > 1) {
-    rest = cluster.map_shared_rank(&sh, 0)->pub_rest;
-    mem = cluster.map_shared_rank(&sh, 0)->pub_mem;
-    for (int r = 1; r < C; ++r) {
-      rest = expsum_join(rest, cluster.map_shared_rank(&sh, r)->pub_rest, a.c);
-      if (TAIL) mem = expsum_join(mem, cluster.map_shared_rank(&sh, r)->pub_mem, a.c);
-    }
-  }
-  const ExpSum all = TAIL ? expsum_join(rest, mem, a.c) : rest;
-  const float all_l = log2f(all.s);
-
-  // sum t (log t - log s) over the slice's entries
-  constexpr float LN2 = 0.6931471805599453f;
-  float dot = 0.0f;
-#pragma unroll
-  for (int j = 0; j < DEPT; ++j) {
-    if (mine[j] && t[j] != 0.0f) {  // (NaN counts)
-      dot += t[j] * ((lp[j] - norm) - ((z[j] - all.m) * a.inv_tau - all_l * LN2));
-    }
-  }
-  dot = block_sum<DNW>(dot, sh.fred);
-  bool any_dup = row_dup;
-  if (C > 1) {
-    if (tid == 0) {
-      sh.pub_dot = dot;
-      sh.fred[0] = row_dup ? 1.0f : 0.0f;
-    }
-    cluster_barrier(C);
-    if (rank == 0 && tid == 0) {
-      for (int r = 1; r < C; ++r) {
-        dot += cluster.map_shared_rank(&sh, r)->pub_dot;
-        any_dup |= cluster.map_shared_rank(&sh, r)->fred[0] != 0.0f;
-      }
-    }
-  }
-  if (rank == 0 && tid == 0) {
-    float loss = dot;
-    RowStats st;
-    st.ref_m = st.all_m = all.m;
-    st.ref_l = st.all_l = all_l;
-    st.coef = st.mass = 1.0f;
-    st.norm = norm;
-    st.flags = any_dup ? D_DUP : D_ROW;
-    if (TAIL) {
-      const float rest_l = log2f(rest.s);
-      const float log2_share = (rest.m - all.m) * a.c + (rest_l - all_l);  // log2 S
-      float tm = 1.0f - sum_t;
-      tm = (tm < 0.0f || log2_share < NO_SHARE) ? 0.0f : tm;  // (NaN stays)
-      st.coef = st.mass = sum_t + tm;
-      if (tm != 0.0f) {
-        loss += tm * (logf(tm) - log2_share * LN2);
-        st.ref_m = rest.m;
-        st.ref_l = rest_l;
-        st.coef = st.mass * exp2f(log2_share) - tm;
-      }
-    }
-    if (row_bad || all.s == 0.0f) loss = st.all_l = st.ref_l = NAN;  // an index out of range; no student mass at all
-    a.loss[row] = loss * wt;
-    a.stats[row] = st;
-  }
-  if (C > 1) cluster.sync();  // shared memory stays until rank 0 has read it
 }
 
 template <typename T>
@@ -306,66 +104,55 @@ __device__ __forceinline__ uint4 pack_vec(const float* x) {
   }
 }
 
-// CTA (row, chunk): the gradient of the row's vectors [v0, v1), then the entries among them.
+// A row's gradient: where it goes, and its scale g.
 template <typename T>
-__global__ void __launch_bounds__(DT, 2) distill_backward_kernel(DistillArgs a) {
-  constexpr int EPV = Elem<T>::EPV;
-  const int64_t row = blockIdx.x / a.chunks;
-  const int chunk = (int)(blockIdx.x - row * a.chunks);
-  const int tid = threadIdx.x;
-  const RowView<T> rv(static_cast<const T*>(a.z) + row * a.z_stride, a.V);
-  T* out = static_cast<T*>(a.dz) + row * (int64_t)a.V;
-  const bool together = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(rv.row)) & 15) == 0;
-  const int32_t v0 = (int32_t)((int64_t)rv.nvec * chunk / a.chunks),
-                v1 = (int32_t)((int64_t)rv.nvec * (chunk + 1) / a.chunks);
-  const RowStats st = a.stats[row];
-  float g = __ldg(a.grad + row * a.grad_stride) * a.inv_tau;
-  if (a.weight) g *= __ldg(a.weight + row);
-  const bool zero = (st.flags & D_EMPTY) || g == 0.0f;
-  const float gc = g * st.coef;
-
-  auto put = [&](int32_t v, const float* x) {
+struct GradRow {
+  static constexpr int EPV = Elem<T>::EPV;
+  const DistillArgs& a;
+  const RowView<T>& rv;
+  const RowStats& st;
+  int64_t row;
+  T* out;
+  bool together;  // the row and its gradient lie alike on 16-byte boundaries
+  float g;
+  __device__ GradRow(const DistillArgs& a_, const RowView<T>& rv_, const RowStats& st_, int64_t row_, float g_)
+      : a(a_), rv(rv_), st(st_), row(row_), g(g_) {
+    out = static_cast<T*>(a.dz) + row * (int64_t)a.V;
+    together = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(rv.row)) & 15) == 0;
+  }
+  __device__ __forceinline__ void put(int32_t v, const float* x) const {
     const int32_t e0 = rv.first(v);
     if (together && rv.whole(v)) {
-      *reinterpret_cast<uint4*>(out + e0) = pack_vec<T>(x);
+      __stcs(reinterpret_cast<uint4*>(out + e0), pack_vec<T>(x));
     } else {
 #pragma unroll
       for (int q = 0; q < EPV; ++q)
         if (e0 + q >= 0 && e0 + q < a.V) out[e0 + q] = narrow<T>(x[q]);
     }
-  };
-  if (zero) {
+  }
+  __device__ __forceinline__ void put_zero(int32_t v) const {
     float x[EPV];
 #pragma unroll
     for (int q = 0; q < EPV; ++q) x[q] = 0.0f;
-    for (int32_t v = v0 + tid; v < v1; v += DT) put(v, x);
-    return;
+    put(v, x);
   }
-  for (int32_t vb = v0; vb < v1; vb += DT * DU) {
-    uint4 in[DU];
+  // the elements of vector v as if none were an entry
+  __device__ __forceinline__ void put_rest(int32_t v, uint4 in, const Exponent& ex) const {
+    const float gc = g * st.coef;
+    float x[EPV];
+    uint64_t e[EPV / 2];
+    ex.template of<T>(in, e);
+    const uint64_t g2 = pack2(gc, gc);
 #pragma unroll
-    for (int u = 0; u < DU; ++u) {
-      const int32_t v = vb + u * DT + tid;
-      if (v < v1) in[u] = load_vec(rv, v);
+    for (int i = 0; i < EPV / 2; ++i) {
+      float lo, hi;
+      unpack2(e[i], lo, hi);
+      unpack2(mul2(pack2(ex2(lo), ex2(hi)), g2), x[2 * i], x[2 * i + 1]);
     }
-#pragma unroll
-    for (int u = 0; u < DU; ++u) {
-      const int32_t v = vb + u * DT + tid;
-      if (v < v1) {
-        float x[EPV];
-        Elem<T>::unpack(in[u], x);
-#pragma unroll
-        for (int q = 0; q < EPV; ++q) x[q] = ex2(fmaf(x[q] - st.ref_m, a.c, -st.ref_l)) * gc;
-        put(v, x);
-      }
-    }
+    put(v, x);
   }
-  __syncthreads();  // the entries' elements are written again, after the stream's
-  for (int i = tid; i < a.K; i += DT) {
-    const int64_t e = entry_index(a, row, i);
-    if (e < 0 || e >= a.V) continue;
-    const int32_t v = ((int32_t)e + rv.off) / EPV;
-    if (v < v0 || v >= v1) continue;
+  // entry i, which names element e
+  __device__ __forceinline__ void put_entry(int i, int64_t e) const {
     float t = 0.0f;
     if (st.flags & D_DUP) {  // every entry that names e writes the same sum, taken in entry order
       for (int j = 0; j < a.K; ++j)
@@ -376,35 +163,236 @@ __global__ void __launch_bounds__(DT, 2) distill_backward_kernel(DistillArgs a) 
     const float s = ex2(fmaf(Elem<T>::ld(rv.row + e) - st.all_m, a.c, -st.all_l));
     out[e] = narrow<T>((st.mass * s - t) * g);
   }
+};
+
+// CTA (row, segment): the sums of the segment's exponentials.
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(SEG_T, 4) part_kernel(DistillArgs a) {
+  constexpr int EPV = Elem<T>::EPV;
+  __shared__ uint32_t mask[SEG_T * SEG_V * EPV / 32];  // a bit per element of the segment: an entry's
+  __shared__ uint32_t marked[SEG_T];                   // by thread: a bit per vector that holds an entry
+  __shared__ Part warps[SEG_NW];
+  __shared__ int32_t any_dup;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const RowView<T> rv(static_cast<const T*>(a.z) + row * a.z_stride, a.V);
+  const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+  uint4 q[SEG_V];
+  load_segment(rv, v0, v1, q);
+  grid_release();
+
+  // mark the segment's entries, while its vectors are on their way
+  int64_t e = tid < a.K ? entry_index(a, row, tid) : -1;
+#pragma unroll
+  for (int w = tid; w < SEG_T * SEG_V * EPV / 32; w += SEG_T) mask[w] = 0;
+  marked[tid] = 0;
+  if (tid == 0) any_dup = 0;
+  __syncthreads();
+  ExpSum mem = expsum_empty();
+  const int32_t e0 = max(0, rv.first(v0)), e1 = min(a.V, rv.first(v1));
+  for (int i = tid; i < a.K; i += SEG_T) {
+    if (i != tid) e = entry_index(a, row, i);
+    if (e < e0 || e >= e1) continue;
+    const uint32_t b = (uint32_t)((int32_t)e - rv.first(v0)), v = b / EPV;
+    if ((atomicOr(&mask[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1u) {
+      any_dup = 1;
+    } else if (TAIL) {
+      // the first to mark an element adds its term, which counts once, however many entries name it
+      // (a NaN or +inf logit makes the sum NaN, as in the stream)
+      atomicOr(&marked[v % SEG_T], 1u << (v / SEG_T));
+      const float z = Elem<T>::ld(rv.row + e), m = fmaxf(LOWEST, z);
+      mem = expsum_join(mem, ExpSum{m, ex2((z - m) * a.c)}, a.c);
+    }
+  }
+  __syncthreads();
+
+  if constexpr (TAIL) {
+    uint32_t mk = marked[tid];
+    if (mk) {  // an entry's element counts as -inf here
+#pragma unroll
+      for (int i = 0; i < SEG_V; ++i) {
+        if (!((mk >> i) & 1u)) continue;
+        const uint32_t b = (uint32_t)(tid + i * SEG_T) * EPV;
+        const uint32_t bits = mask[b >> 5] >> (b & 31);
+        uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+        for (int x = 0; x < EPV; ++x) {
+          const uint32_t part = (EPV == 4) ? 0xFFFFFFFFu : 0xFFFFu << (16 * (x & 1));
+          uint32_t& word = w[(EPV == 4) ? x : x >> 1];
+          if ((bits >> x) & 1u) word = (word & ~part) | (Elem<T>::NEG_INF_WORD & part);
+        }
+        q[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  RunningSum acc;
+#pragma unroll
+  for (int i = 0; i < SEG_V; i += 4) acc.template add<T, 4>(q + i, a.c);
+  const ExpSum rest = warp_expsum(acc.total(), a.c);
+  if (TAIL) mem = warp_expsum(mem, a.c);
+  if (lane == 0) warps[warp] = Part{rest, mem, 0, 0};
+  __syncthreads();
+  if (warp != 0) return;
+  Part p = lane < SEG_NW ? warps[lane] : Part{expsum_empty(), expsum_empty(), 0, 0};
+  p.rest = warp_expsum(p.rest, a.c);
+  if (TAIL) p.mem = warp_expsum(p.mem, a.c);
+  p.dup = any_dup;
+  if (lane == 0) a.parts[row * a.seg.segs + blockIdx.y] = p;
 }
 
-// CTAs per row: enough to give every SM two, with slices of at least 8 KB.
-int cluster_for(int64_t n, int64_t bytes) {
-  const int64_t want = 2 * (int64_t)device_sms();
-  int C = 1;
-  while (C < 8 && n * C < want && bytes / (2 * C) >= 8192) C <<= 1;
-  return C;
+// One warp per row: joins the row's segments, takes the loss from its entries, and leaves what the
+// backward pass needs.
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(256) finish_kernel(DistillArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= a.n) return;
+  const float wt = a.weight ? __ldg(a.weight + row) : 1.0f;
+  const T* zr = static_cast<const T*>(a.z) + row * a.z_stride;
+
+  // the entries: sum of exp(value - top) (the tail's are probabilities as they are: top is 0)
+  bool any = false, bad = false;
+  float top = -INFINITY, sum = 0.0f;
+  for (int i = lane; i < a.K; i += 32) {
+    const int64_t e = entry_index(a, row, i);
+    const float lp = __ldg(a.lp + row * a.lp_stride + i);
+    bad |= e < -1 || e >= a.V;
+    if (e >= 0) {
+      any = true;
+      top = max_nan(top, lp);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  if (TAIL || top == -INFINITY) top = 0.0f;
+  for (int i = lane; i < a.K; i += 32)
+    if (entry_index(a, row, i) >= 0) sum += expf(__ldg(a.lp + row * a.lp_stride + i) - top);
+  sum = warp_sum(sum);
+  any = __any_sync(0xFFFFFFFFu, any);
+  bad = __any_sync(0xFFFFFFFFu, bad);
+  const float norm = TAIL ? 0.0f : top + logf(sum);  // t_i = exp(value_i - norm)
+
+  grid_wait();  // the segments' sums
+  // no entry, or (renormalised) none of any weight: a padded row
+  if (!bad && (wt == 0.0f || !any || (!TAIL && sum == 0.0f))) {
+    if (lane == 0) {
+      a.loss[row] = 0.0f;
+      a.stats[row] = RowStats{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, D_EMPTY};
+    }
+    return;
+  }
+  ExpSum rest = expsum_empty(), mem = rest;
+  int32_t dup = 0;
+  for (int s = lane; s < a.seg.segs; s += 32) {
+    const Part p = a.parts[row * a.seg.segs + s];
+    rest = expsum_join(rest, p.rest, a.c);
+    if (TAIL) mem = expsum_join(mem, p.mem, a.c);
+    dup |= p.dup;
+  }
+  rest = warp_expsum(rest, a.c);
+  if (TAIL) mem = warp_expsum(mem, a.c);
+  dup = __any_sync(0xFFFFFFFFu, dup);
+  constexpr float LN2 = 0.6931471805599453f;
+  const ExpSum full = TAIL ? expsum_join(rest, mem, a.c) : rest;
+  RowStats st;
+  st.ref_m = st.all_m = full.m;
+  st.ref_l = st.all_l = log2f(full.s);
+  st.coef = st.mass = 1.0f;
+  st.norm = norm;
+  st.flags = dup ? D_DUP : D_ROW;
+  float dot = 0.0f;
+  for (int i = lane; i < a.K; i += 32) {
+    const int64_t e = entry_index(a, row, i);
+    if (e < 0 || e >= a.V) continue;
+    const float lp = __ldg(a.lp + row * a.lp_stride + i), t = expf(lp - norm);
+    if (t != 0.0f)  // (NaN counts)
+      dot += t * ((lp - norm) - ((Elem<T>::ld(zr + e) - full.m) * a.inv_tau - st.all_l * LN2));
+  }
+  float loss = warp_sum(dot);
+  if (TAIL) {
+    const float rest_l = log2f(rest.s);
+    const float log2_share = (rest.m - full.m) * a.c + (rest_l - st.all_l);  // log2 S
+    float tm = 1.0f - sum;
+    tm = (tm < 0.0f || log2_share < NO_SHARE) ? 0.0f : tm;  // (NaN stays)
+    st.coef = st.mass = sum + tm;
+    if (tm != 0.0f) {
+      loss += tm * (logf(tm) - log2_share * LN2);
+      st.ref_m = rest.m;
+      st.ref_l = rest_l;
+      st.coef = st.mass * exp2f(log2_share) - tm;
+    }
+  }
+  if (bad || full.s == 0.0f) loss = st.all_l = st.ref_l = NAN;  // an index out of range; no student mass at all
+  if (lane == 0) {
+    a.loss[row] = loss * wt;
+    a.stats[row] = st;
+  }
 }
 
-size_t mask_bytes(int64_t V, int es, int C) {
-  const int64_t epv = 16 / es, nvec = (V + 2 * epv - 2) / epv;  // the most vectors a row of any alignment has
-  return (size_t)(((nvec + C - 1) / C * epv + 31) / 32 * 4);
+// CTA (row, segment): the gradient of the segment, then of the entries in it.
+template <typename T>
+__global__ void __launch_bounds__(SEG_T, 4) backward_kernel(DistillArgs a) {
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const RowView<T> rv(static_cast<const T*>(a.z) + row * a.z_stride, a.V);
+  const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+  uint4 q[SEG_V];
+  load_segment(rv, v0, v1, q);
+  const RowStats st = a.stats[row];
+  float g = __ldg(a.grad + row * a.grad_stride) * a.inv_tau;
+  if (a.weight) g *= __ldg(a.weight + row);
+  const GradRow<T> grad(a, rv, st, row, g);
+  if ((st.flags & D_EMPTY) || g == 0.0f) {
+    for (int32_t v = v0 + tid; v < v1; v += SEG_T) grad.put_zero(v);
+    return;
+  }
+  const Exponent ex(st.ref_m, a.c, st.ref_l);
+#pragma unroll
+  for (int i = 0; i < SEG_V; ++i)
+    if (v0 + i * SEG_T + tid < v1) grad.put_rest(v0 + i * SEG_T + tid, q[i], ex);
+  __syncthreads();  // the entries' elements are written again, after the stream's
+  const int32_t e0 = max(0, rv.first(v0)), e1 = min(a.V, rv.first(v1));
+  for (int i = tid; i < a.K; i += SEG_T) {
+    const int64_t e = entry_index(a, row, i);
+    if (e >= e0 && e < e1) grad.put_entry(i, e);
+  }
+}
+
+// Sum of the rows' losses, in 64 bits and a fixed order, by one CTA.
+__global__ void __launch_bounds__(1024) distill_sum_kernel(const float* loss, int64_t n, float* out) {
+  __shared__ double part[32];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)loss[i];
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = warp_sum(part[threadIdx.x]);
+    if (threadIdx.x == 0) *out = (float)s;
+  }
+}
+
+template <typename T, bool TAIL>
+int forward_as(const DistillArgs& a, cudaStream_t st) {
+  part_kernel<T, TAIL><<<dim3((unsigned)a.n, (unsigned)a.seg.segs), SEG_T, 0, st>>>(a);
+  if (cudaGetLastError() != cudaSuccess) return PB_E_LAUNCH;
+  return launch_after(finish_kernel<T, TAIL>, a, dim3((unsigned)((a.n + 7) / 8)), 256, st);
 }
 
 template <typename T>
-int forward(const DistillArgs& a, cudaStream_t st) {
-  const int C = cluster_for(a.n, (int64_t)a.V * sizeof(T));
-  const size_t smem = mask_bytes(a.V, sizeof(T), C);
-  return a.tail ? launch_cluster(distill_forward_kernel<T, true>, a, a.n * C, DT, C, smem, st)
-                : launch_cluster(distill_forward_kernel<T, false>, a, a.n * C, DT, C, smem, st);
+int forward(DistillArgs a, cudaStream_t st) {
+  a.seg = seg_plan(a.V, sizeof(T));
+  return a.tail ? forward_as<T, true>(a, st) : forward_as<T, false>(a, st);
 }
 
 template <typename T>
 int backward(DistillArgs a, cudaStream_t st) {
-  // chunks of a row: CTAs of at least 4 vectors a thread, unless the rows alone cannot fill the SMs
-  a.chunks = cluster_for(a.n, (int64_t)a.V * sizeof(T));
-  return launch_cluster(distill_backward_kernel<T>, a, a.n * a.chunks, DT, 1, 0, st);
+  a.seg = seg_plan(a.V, sizeof(T));
+  backward_kernel<T><<<dim3((unsigned)a.n, (unsigned)a.seg.segs), SEG_T, 0, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? PB_OK : PB_E_LAUNCH;
 }
+
+constexpr int64_t stats_bytes(int64_t n) { return n * (int64_t)sizeof(RowStats); }
 
 int check(const DistillArgs& a, int es, int64_t vocab, float temperature) {
   if (a.n < 0 || vocab <= 0 || a.K < 1 || a.K > DKMAX) return PB_E_INVALID;
@@ -426,12 +414,18 @@ int check(const DistillArgs& a, int es, int64_t vocab, float temperature) {
 
 extern "C" {
 
-int64_t pb_distill_stats_bytes(int64_t n_rows) { return n_rows < 0 ? PB_E_INVALID : n_rows * (int64_t)sizeof(RowStats); }
+int64_t pb_distill_stats_bytes(int64_t n_rows) { return n_rows < 0 ? PB_E_INVALID : stats_bytes(n_rows); }
+
+int64_t pb_distill_ws_bytes(int64_t n_rows, int64_t vocab, int dtype) {
+  const int es = elem_size(dtype);
+  if (n_rows < 0 || vocab <= 0 || vocab > DVMAX || !es) return PB_E_INVALID;
+  return n_rows * seg_plan(vocab, es).segs * (int64_t)sizeof(Part);
+}
 
 int pb_distill_forward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
                        const float* teacher, int64_t teacher_stride, const void* indices, int64_t index_stride,
                        int index_bytes, int32_t n_entries, float temperature, int tail, const float* row_weight,
-                       float* out_loss, void* out_stats, void* stream) {
+                       float* out_loss, void* out_stats, void* workspace, int64_t ws_bytes, void* stream) {
   const int es = elem_size(dtype);
   if (index_bytes != 4 && index_bytes != 8) return PB_E_INVALID;
   DistillArgs a = {};
@@ -451,7 +445,9 @@ int pb_distill_forward(const void* logits, int dtype, int64_t n_rows, int64_t vo
   a.K = n_entries;
   const int rc = check(a, es, vocab, temperature);
   if (rc != PB_OK || n_rows == 0) return rc;
-  if (!out_loss) return PB_E_INVALID;
+  if (!out_loss || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)) return PB_E_INVALID;
+  if (ws_bytes < pb_distill_ws_bytes(n_rows, vocab, dtype)) return PB_E_INVALID;
+  a.parts = static_cast<Part*>(workspace);
   a.c = (float)(1.4426950408889634 / (double)temperature);
   a.inv_tau = 1.0f / temperature;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -492,6 +488,12 @@ int pb_distill_backward(const void* logits, int dtype, int64_t n_rows, int64_t v
   if (dtype == PB_DTYPE_F32) return backward<float>(a, st);
   if (dtype == PB_DTYPE_BF16) return backward<__nv_bfloat16>(a, st);
   return backward<__half>(a, st);
+}
+
+int pb_distill_sum(const float* loss, int64_t n_rows, float* out_sum, void* stream) {
+  if (n_rows < 0 || !out_sum || (n_rows && !loss)) return PB_E_INVALID;
+  distill_sum_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(loss, n_rows, out_sum);
+  return cudaGetLastError() == cudaSuccess ? PB_OK : PB_E_LAUNCH;
 }
 
 }  // extern "C"

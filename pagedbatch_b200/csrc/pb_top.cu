@@ -5,27 +5,29 @@
 //   the k largest x in the order (value descending, index ascending), NaN above every value
 //   (the sampler's order). A row holding NaN or +inf, or only -inf, has NaN log-probabilities.
 //
-// One cluster of C CTAs per row reads the row once. Every thread keeps a running maximum and sum of
-// exponentials, and the key of the largest value of each run of TU vectors it loads together (its
-// groups) in shared memory. A lower bound of the k-th largest value follows from the lanes' largest
-// group keys: with W warps in the cluster, each warp's ceil(k / W)-th largest lane maximum is reached
-// by that many values of the warp, so the smallest of these over the warps is reached by at least k
-// values of the row. Only the groups whose key reaches the bound are read again (from L2); their
-// values at or above it are the candidates, a little more than k, sorted in one CTA.
-// HBM-bound: V * es bytes a row. A row with more candidates than the list holds (rows of very many
-// equal values) is selected by bisection over (value, index) in its first CTA.
+// Two launches. part_kernel reads every row once, a CTA per segment of it: per thread a running
+// maximum and sum of exponentials, and the key of the largest value of its vectors (its group).
+// select_kernel, a CTA per row: a lower bound of the k-th largest value follows from the lanes'
+// largest group keys, since each of its 8 warps holds ceil(k / 8) values at or above its
+// ceil(k / 8)-th largest lane maximum, so the row holds k at or above the smallest of these. Only the
+// groups whose key reaches the bound are read again (from L2); their values at or above it are the
+// candidates, a little more than k, put in order by counting for each the candidates before it, or
+// where they are many by a bitonic network. A row with more candidates than the list holds (very many
+// equal values) is selected by bisection over (value, index).
+// HBM-bound: V * es bytes a row, and 1/32 of that written as keys.
 #include "pb_rows.cuh"
 
 using namespace pb;
 
 namespace {
 
-constexpr int TT = 512;            // threads per CTA
-constexpr int TNW = TT / 32;
-constexpr int TU = 4;              // vectors a thread loads together: one group
-constexpr int TKMAX = PB_TOP_MAX;   // largest k
+constexpr int TT = SEG_T;          // threads per CTA
+constexpr int TNW = SEG_NW;
+constexpr int TKMAX = PB_TOP_MAX;  // largest k
 constexpr int TCAP = 2048;         // candidates of a row
-constexpr int TGROUPS = 16;        // groups a thread keeps; longer slices keep the largest of several
+constexpr int TRANK = 512;         // candidates ordered by counting
+constexpr int TLIST = 1024;        // groups of a row that are read again
+static_assert((TKMAX + TNW - 1) / TNW <= 32, "every warp has enough lanes");
 
 struct TopArgs {
   const void* x;
@@ -36,17 +38,19 @@ struct TopArgs {
   float* logprob;        // [n][k]
   int32_t* index;        // [n][k]
   float* lse;            // [n]
+  SegPlan seg;
+  ExpSum* parts;         // workspace: [n][segs]
+  uint32_t* keys;        // workspace: [n][segs][TT]
 };
 
 struct TopShared {
-  ExpSum red[TNW];
-  uint32_t bound[TNW], top[TNW];
-  ExpSum pub_sum;
-  uint32_t pub_bound;    // smallest of the CTA's warps' bounds
-  uint32_t pub_max;      // largest key
-  uint32_t n;            // rank 0: candidates of the row
-  uint32_t cnt[2];       // bisection counts
-  uint64_t list[TCAP];   // rank 0: candidates
+  ExpSum sum[TNW];
+  uint32_t bound[TNW];
+  uint32_t groups;                  // groups listed
+  uint32_t n;                       // candidates
+  uint32_t cnt[2];                  // bisection counts
+  uint32_t group[TLIST];
+  alignas(16) uint64_t list[TCAP];  // candidates
 };
 
 // c-th largest (1 <= c <= 32) of the warp's 32 values: c rounds of a warp maximum, one copy of the
@@ -123,107 +127,131 @@ __device__ __noinline__ void select_slow(const RowView<T>& rv, int k, TopShared&
 }
 
 template <typename T>
-__global__ void __launch_bounds__(TT, 2) top_kernel(TopArgs a) {
+__global__ void __launch_bounds__(TT, 4) part_kernel(TopArgs a) {
+  __shared__ ExpSum scratch[TNW];
+  const int64_t row = blockIdx.x;
+  const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
+  const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+  uint4 q[SEG_V];
+  load_segment(rv, v0, v1, q);
+  grid_release();
+  RunningSum acc;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < SEG_V; i += 4) mx = max_nan(mx, acc.template add<T, 4>(q + i, a.c));
+  const int64_t part = row * a.seg.segs + blockIdx.y;
+  a.keys[part * TT + threadIdx.x] = key_of(mx);
+  const ExpSum sum = block_expsum<TNW>(acc.total(), a.c, scratch);
+  if (threadIdx.x == 0) a.parts[part] = sum;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
   constexpr int EPV = Elem<T>::EPV;
-  extern __shared__ __align__(16) uint32_t keys[];  // [groups][TT]: keys of the thread's groups
   __shared__ TopShared sh;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t row = blockIdx.x / C;
+  const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
-  const int32_t v0 = (int32_t)((int64_t)rv.nvec * rank / C), v1 = (int32_t)((int64_t)rv.nvec * (rank + 1) / C);
-  const int32_t iters = (v1 - v0 + TT * TU - 1) / (TT * TU);
-  const int32_t per = (iters + TGROUPS - 1) / TGROUPS;  // loads that share one kept key
-
-  if (tid == 0) sh.n = 0;
-  ExpSum acc = expsum_empty();
-  uint32_t lmax = 0, gkey = 0;  // 0: below every key (a thread without vectors)
-  for (int32_t it = 0; it < iters; ++it) {
-    const int32_t vb = v0 + it * TT * TU + tid;
-    uint4 q[TU];
+  const int32_t segs = a.seg.segs;
+  if (tid == 0) sh.groups = sh.n = 0;
+  grid_wait();  // the segments' keys and sums
+  const uint32_t* keys = a.keys + row * segs * TT + tid;
+  constexpr int HELD = 16;  // keys a thread keeps; longer rows' are read twice
+  uint32_t key[HELD], lmax = 0;
 #pragma unroll
-    for (int u = 0; u < TU; ++u)
-      if (vb + u * TT < v1) q[u] = load_vec(rv, vb + u * TT);
-#pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      if (vb + u * TT < v1) {
-        float x[EPV];
-        Elem<T>::unpack(q[u], x);
-        gkey = max(gkey, key_of(vec_max_nan<T>(q[u])));
-        expsum_add<T>(acc, x, a.c);
-      }
-    }
-    if ((it + 1) % per == 0 || it + 1 == iters) {
-      keys[(it / per) * TT + tid] = gkey;
-      lmax = max(lmax, gkey);
-      gkey = 0;
-    }
+  for (int s = 0; s < HELD; ++s) key[s] = s < segs ? __ldcg(keys + s * TT) : 0u;
+  ExpSum sum = expsum_empty();
+  for (int32_t s = tid; s < segs; s += TT) {
+    const float2 p = __ldcg(reinterpret_cast<const float2*>(a.parts + row * segs + s));
+    sum = expsum_join(sum, ExpSum{p.x, p.y}, a.c);
   }
-
-  // the bound of the k-th largest value, from the lanes' largest keys
-  const int nth = (a.k + C * TNW - 1) / (C * TNW);
-  const uint32_t wb = warp_nth_largest(lmax, nth);
-  const uint32_t wm = __reduce_max_sync(0xFFFFFFFFu, lmax);
+#pragma unroll
+  for (int s = 0; s < HELD; ++s) lmax = max(lmax, key[s]);
+  for (int32_t s = HELD; s < segs; ++s) lmax = max(lmax, __ldcg(keys + (int64_t)s * TT));
+  const uint32_t wb = warp_nth_largest(lmax, (a.k + TNW - 1) / TNW);
+  sum = warp_expsum(sum, a.c);
   if (lane == 0) {
     sh.bound[warp] = wb;
-    sh.top[warp] = wm;
+    sh.sum[warp] = sum;
   }
-  const ExpSum cta = block_expsum<TNW>(acc, a.c, sh.red);
-  if (tid == 0) {
-    uint32_t b = sh.bound[0], m = sh.top[0];
-    for (int w = 1; w < TNW; ++w) {
-      b = min(b, sh.bound[w]);
-      m = max(m, sh.top[w]);
-    }
-    sh.pub_sum = cta;
-    sh.pub_bound = b;
-    sh.pub_max = m;
-  }
-  cluster_barrier(C);
-  TopShared* first = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
-  ExpSum all = first->pub_sum;
-  uint32_t bound = first->pub_bound, mx = first->pub_max;
-  for (int r = 1; r < C; ++r) {
-    const TopShared* o = cluster.map_shared_rank(&sh, r);
-    all = expsum_join(all, o->pub_sum, a.c);
-    bound = min(bound, o->pub_bound);
-    mx = max(mx, o->pub_max);
+  __syncthreads();
+  uint32_t bound = sh.bound[0];
+  sum = sh.sum[0];
+#pragma unroll
+  for (int w = 1; w < TNW; ++w) {
+    bound = min(bound, sh.bound[w]);
+    sum = expsum_join(sum, sh.sum[w], a.c);
   }
 
-  // candidates: values at or above the bound, from the groups whose key reaches it
-  for (int32_t g = 0; g * per < iters; ++g) {
-    if (keys[g * TT + tid] < bound) continue;
-    for (int32_t it = g * per; it < min(iters, (g + 1) * per); ++it) {
-      const int32_t vb = v0 + it * TT * TU + tid;
+  // the groups that reach the bound, then the values in them that do
+  auto list_group = [&](int32_t s, bool hit) {
+    const uint32_t b = __ballot_sync(0xFFFFFFFFu, hit);
+    if (!b) return;
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(&sh.groups, (uint32_t)__popc(b));
+    at = __shfl_sync(0xFFFFFFFFu, at, 0) + (uint32_t)__popc(b & lanemask_lt());
+    if (hit && at < (uint32_t)TLIST) sh.group[at] = (uint32_t)(s * TT + tid);
+  };
 #pragma unroll
-      for (int u = 0; u < TU; ++u) {
-        const int32_t v = vb + u * TT;
-        if (v >= v1) break;
-        float x[EPV];
-        Elem<T>::unpack(load_vec(rv, v), x);
+  for (int s = 0; s < HELD; ++s)
+    if (s < segs) list_group(s, key[s] >= bound);
+  for (int32_t s = HELD; s < segs; ++s) list_group(s, __ldcg(keys + (int64_t)s * TT) >= bound);
+  __syncthreads();
+  const uint32_t groups = sh.groups;
+  if (groups <= (uint32_t)TLIST) {
+    for (uint32_t i = tid; i < groups * SEG_V; i += TT) {
+      const uint32_t g = sh.group[i / SEG_V];
+      const int32_t v0 = (int32_t)(g / TT) * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+      const int32_t v = v0 + (int32_t)(g % TT) + (int32_t)(i % SEG_V) * TT;
+      if (v >= v1) continue;
+      const uint4 q = load_vec(rv, v);
+      if (key_of(vec_max_nan<T>(q)) < bound) continue;
+      float x[EPV];
+      Elem<T>::unpack(q, x);
 #pragma unroll
-        for (int q = 0; q < EPV; ++q) {
-          const uint32_t key = key_of(x[q]);
-          const int32_t e = rv.first(v) + q;
-          if (key >= bound && e >= 0 && e < a.V) {
-            const uint32_t at = atomicAdd(&first->n, 1u);
-            if (at < (uint32_t)TCAP) first->list[at] = compose(key, (uint32_t)e);
-          }
+      for (int j = 0; j < EPV; ++j) {
+        const uint32_t kx = key_of(x[j]);
+        const int32_t e = rv.first(v) + j;
+        if (kx >= bound && e >= 0 && e < a.V) {
+          const uint32_t at = atomicAdd(&sh.n, 1u);
+          if (at < (uint32_t)TCAP) sh.list[at] = compose(kx, (uint32_t)e);
         }
       }
     }
   }
-  cluster_barrier(C);
-  if (rank != 0) return;
+  __syncthreads();
+  constexpr float LN2 = 0.6931471805599453f;
+  // NaN or +inf in the row (the sum is NaN then), or nothing above -inf: no distribution
+  const float l = (sum.s == 0.0f) ? NAN : log2f(sum.s);
+  if (tid == 0) a.lse[row] = sum.m / a.temperature + l * LN2;
+  auto put = [&](uint32_t at, uint64_t e) {
+    a.logprob[row * a.k + at] = (value_of(comp_key(e)) - sum.m) / a.temperature - l * LN2;
+    a.index[row * a.k + at] = (int32_t)comp_idx(e);
+  };
   uint32_t n = sh.n;
-  if (n > (uint32_t)TCAP) {
+  if (n > (uint32_t)TCAP || groups > (uint32_t)TLIST) {
     __syncthreads();
     select_slow<T>(rv, a.k, sh);
     n = (uint32_t)a.k;
   }
-  // sort: a bitonic network over the next power of two, padded with zeros (below every entry)
-  uint32_t size = 64;
+  if (n <= (uint32_t)TRANK) {
+    // the place of each candidate: the number of those above it (no two are equal)
+    if (tid == 0 && (n & 1)) sh.list[n] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += TT) {
+      const uint64_t e = sh.list[i];
+      uint32_t above = 0;
+#pragma unroll 4
+      for (uint32_t j = 0; j < n; j += 2) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.list[j]);
+        above += (o.x > e ? 1u : 0u) + (o.y > e ? 1u : 0u);
+      }
+      if (above < (uint32_t)a.k) put(above, e);
+    }
+    return;
+  }
+  // a bitonic network over the next power of two, padded with zeros (below every entry)
+  uint32_t size = 2 * TRANK;
   while (size < n) size <<= 1;
   for (uint32_t i = n + tid; i < size; i += TT) sh.list[i] = 0;
   __syncthreads();
@@ -239,40 +267,41 @@ __global__ void __launch_bounds__(TT, 2) top_kernel(TopArgs a) {
       }
       __syncthreads();
     }
-  constexpr float LN2 = 0.6931471805599453f;
-  // NaN or +inf in the row (the sum is NaN then), or nothing above -inf: no distribution
-  const float l = (all.s == 0.0f) ? NAN : log2f(all.s);
-  if (tid == 0) a.lse[row] = all.m / a.temperature + l * LN2;
-  for (int i = tid; i < a.k; i += TT) {
-    const uint64_t e = sh.list[i];
-    a.logprob[row * a.k + i] = (value_of(comp_key(e)) - all.m) / a.temperature - l * LN2;
-    a.index[row * a.k + i] = (int32_t)comp_idx(e);
-  }
+  for (int i = tid; i < a.k; i += TT) put(i, sh.list[i]);
 }
 
-int top_cluster(int64_t n, int64_t bytes) {
-  const int64_t want = 2 * (int64_t)device_sms();
-  int C = 1;
-  while (C < 8 && n * C < want && bytes / (2 * C) >= 8192) C <<= 1;
-  return C;
+struct TopPlan {
+  SegPlan seg;
+  int64_t keys, bytes;  // offset of the keys in the workspace, and its size
+};
+TopPlan top_plan(int64_t n, int64_t V, int es) {
+  TopPlan p;
+  p.seg = seg_plan(V, es);
+  p.keys = (n * p.seg.segs * (int64_t)sizeof(ExpSum) + 255) & ~(int64_t)255;
+  p.bytes = p.keys + n * p.seg.segs * TT * 4;
+  return p;
 }
 
 template <typename T>
 int top_run(const TopArgs& a, cudaStream_t st) {
-  const int C = top_cluster(a.n, (int64_t)a.V * sizeof(T));
-  constexpr int EPV = 16 / (int)sizeof(T);
-  const int64_t nvec = ((int64_t)a.V + 2 * EPV - 2) / EPV, slice = (nvec + C - 1) / C;
-  const int64_t iters = (slice + TT * TU - 1) / (TT * TU);
-  const size_t smem = (size_t)std::min<int64_t>(iters, TGROUPS) * TT * 4;
-  return launch_cluster(top_kernel<T>, a, a.n * C, TT, C, smem, st);
+  part_kernel<T><<<dim3((unsigned)a.n, (unsigned)a.seg.segs), TT, 0, st>>>(a);
+  if (cudaGetLastError() != cudaSuccess) return PB_E_LAUNCH;
+  return launch_after(select_kernel<T>, a, dim3((unsigned)a.n), TT, st);
 }
 
 }  // namespace
 
 extern "C" {
 
+int64_t pb_top_ws_bytes(int64_t n_rows, int64_t vocab, int dtype) {
+  const int es = elem_size(dtype);
+  if (n_rows < 0 || vocab <= 0 || !es) return PB_E_INVALID;
+  return top_plan(n_rows, vocab, es).bytes;
+}
+
 int pb_top_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride, int32_t k,
-                    float temperature, float* out_logprob, int32_t* out_index, float* out_lse, void* stream) {
+                    float temperature, float* out_logprob, int32_t* out_index, float* out_lse, void* workspace,
+                    int64_t ws_bytes, void* stream) {
   const int es = elem_size(dtype);
   if (n_rows < 0 || vocab <= 0 || row_stride < 0 || !es) return PB_E_INVALID;
   if (vocab >= PB_MAX_VOCAB) return PB_E_TOO_LARGE;
@@ -282,6 +311,8 @@ int pb_top_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab
   if (!logits || !out_logprob || !out_index || !out_lse) return PB_E_INVALID;
   if (n_rows > (int64_t)(0x7FFFFFFF / 8)) return PB_E_INVALID;
   if (reinterpret_cast<uintptr_t>(logits) % es) return PB_E_INVALID;
+  const TopPlan plan = top_plan(n_rows, vocab, es);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || ws_bytes < plan.bytes) return PB_E_INVALID;
   TopArgs a;
   a.x = logits;
   a.row_stride = row_stride;
@@ -293,6 +324,9 @@ int pb_top_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab
   a.logprob = out_logprob;
   a.index = out_index;
   a.lse = out_lse;
+  a.seg = plan.seg;
+  a.parts = static_cast<ExpSum*>(workspace);
+  a.keys = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + plan.keys);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == PB_DTYPE_F32) return top_run<float>(a, st);
   if (dtype == PB_DTYPE_BF16) return top_run<__nv_bfloat16>(a, st);

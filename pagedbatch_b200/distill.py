@@ -16,42 +16,59 @@ from .logprobs import check_temperature
 
 __all__ = ["distill_loss"]
 
-
-def _entries(idx: torch.Tensor, lp: torch.Tensor):
-    return lp.data_ptr(), lp.stride(0), idx.data_ptr(), idx.stride(0), idx.element_size(), idx.shape[1]
+STATS = 32  # bytes of a row's statistics (pb_distill_stats_bytes)
 
 
-def _forward(z, lp, idx, weight, temperature, tail):
-    n, V = z.shape
-    L = _lib.load()
-    loss = torch.empty(n, dtype=torch.float32, device=z.device)
-    with torch.cuda.device(z.device):
-        stats = torch.empty(L.pb_distill_stats_bytes(n), dtype=torch.uint8, device=z.device)
-        rc = L.pb_distill_forward(
-            z.data_ptr(), ops._DTYPE_CODE[z.dtype], n, V, z.stride(0), *_entries(idx, lp), temperature, int(tail),
-            weight.data_ptr() if weight is not None else None, loss.data_ptr(), stats.data_ptr(),
-            torch.cuda.current_stream(z.device).cuda_stream)
-    _lib.check(rc, "pb_distill_forward")
-    return loss, stats
+class _Rows:
+    """The arguments of one call: student rows, teacher entries, row weights."""
 
+    __slots__ = ("z", "lp", "idx", "weight", "temperature", "args")
 
-def _backward(z, lp, idx, weight, stats, grad_loss, temperature):
-    n, V = z.shape
-    L = _lib.load()
-    dz = torch.empty((n, V), dtype=z.dtype, device=z.device)
-    with torch.cuda.device(z.device):
-        rc = L.pb_distill_backward(
-            z.data_ptr(), ops._DTYPE_CODE[z.dtype], n, V, z.stride(0), *_entries(idx, lp), temperature,
-            weight.data_ptr() if weight is not None else None, stats.data_ptr(), grad_loss.data_ptr(),
-            grad_loss.stride(0), dz.data_ptr(), torch.cuda.current_stream(z.device).cuda_stream)
-    _lib.check(rc, "pb_distill_backward")
-    return dz
+    def __init__(self, z, lp, idx, weight, temperature):
+        self.z, self.lp, self.idx, self.weight, self.temperature = z, lp, idx, weight, temperature
+        self.args = (z.data_ptr(), ops._DTYPE_CODE[z.dtype], z.shape[0], z.shape[1], z.stride(0), lp.data_ptr(),
+                     lp.stride(0), idx.data_ptr(), idx.stride(0), idx.element_size(), idx.shape[1], temperature)
+
+    def weight_ptr(self):
+        return None if self.weight is None else self.weight.data_ptr()
+
+    def forward(self, tail, total=False):
+        """The rows' losses (or their sum) and statistics."""
+        z = self.z
+        n, V = z.shape
+        L = _lib.load()
+        n_ws = L.pb_distill_ws_bytes(n, V, self.args[1])
+        # one buffer: statistics, losses, and the launch's own workspace
+        keep = n * (STATS + 4)
+        buf = torch.empty(-(-keep // 16) * 16 + n_ws, dtype=torch.uint8, device=z.device)
+        loss = buf[n * STATS : keep].view(torch.float32)
+        with ops.on_device(z.device):
+            stream = torch.cuda.current_stream(z.device).cuda_stream
+            base = buf.data_ptr()
+            rc = L.pb_distill_forward(*self.args, int(tail), self.weight_ptr(), base + n * STATS, base,
+                                      base + buf.numel() - n_ws, n_ws, stream)
+            _lib.check(rc, "pb_distill_forward")
+            if total:
+                loss = torch.empty((), dtype=torch.float32, device=z.device)
+                _lib.check(L.pb_distill_sum(base + n * STATS, n, loss.data_ptr(), stream), "pb_distill_sum")
+        return loss, buf
+
+    def backward(self, stats, grad_loss):
+        z = self.z
+        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        with ops.on_device(z.device):
+            rc = _lib.load().pb_distill_backward(
+                *self.args, self.weight_ptr(), stats.data_ptr(), grad_loss.data_ptr(),
+                grad_loss.stride(0) if grad_loss.dim() else 0, dz.data_ptr(),
+                torch.cuda.current_stream(z.device).cuda_stream)
+        _lib.check(rc, "pb_distill_backward")
+        return dz
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, lp, idx, weight, temperature, tail):
-        loss, stats = _forward(z, lp, idx, weight, temperature, tail)
+    def forward(ctx, z, lp, idx, weight, temperature, tail, total):
+        loss, stats = _Rows(z, lp, idx, weight, temperature).forward(tail, total)
         ctx.save_for_backward(z, lp, idx, weight, stats)
         ctx.temperature = temperature
         return loss
@@ -61,7 +78,8 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, grad_loss):
         z, lp, idx, weight, stats = ctx.saved_tensors
         # a gradient of one value for all rows (from a sum or mean) is read through its stride of 0
-        return _backward(z, lp, idx, weight, stats, grad_loss, ctx.temperature), None, None, None, None, None
+        dz = _Rows(z, lp, idx, weight, ctx.temperature).backward(stats, grad_loss)
+        return dz, None, None, None, None, None, None
 
 
 def distill_loss(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_indices: torch.Tensor, *,
@@ -114,5 +132,7 @@ def distill_loss(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, t
         idx = idx.contiguous()
     if row_weight is not None:
         row_weight = row_weight.contiguous()
-    loss = _Distill.apply(z, lp, idx, row_weight, t, bool(tail))
-    return loss.sum() if reduction == "sum" else loss
+    total = reduction == "sum"
+    if not (z.requires_grad and torch.is_grad_enabled()):
+        return _Rows(z, lp, idx, row_weight, t).forward(tail, total)[0]
+    return _Distill.apply(z, lp, idx, row_weight, t, bool(tail), total)

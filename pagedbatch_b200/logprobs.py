@@ -47,9 +47,11 @@ def _launch(logits: torch.Tensor, k: int, temperature: float):
     idx = torch.empty((n, k), dtype=torch.int32, device=dev)
     lse = torch.empty(n, dtype=torch.float32, device=dev)
     L = _lib.load()
-    with torch.cuda.device(dev):
-        rc = L.pb_top_logprobs(logits.data_ptr(), ops._DTYPE_CODE[logits.dtype], n, V, logits.stride(0), k, t,
-                               lp.data_ptr(), idx.data_ptr(), lse.data_ptr(),
+    with ops.on_device(dev):
+        code = ops._DTYPE_CODE[logits.dtype]
+        ws = torch.empty(L.pb_top_ws_bytes(n, V, code), dtype=torch.uint8, device=dev)
+        rc = L.pb_top_logprobs(logits.data_ptr(), code, n, V, logits.stride(0), k, t, lp.data_ptr(), idx.data_ptr(),
+                               lse.data_ptr(), ws.data_ptr(), ws.numel(),
                                torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(rc, "pb_top_logprobs")
     return lp, idx, lse
@@ -70,6 +72,6 @@ def _(logits, k, temperature):
 
 def top_logprobs(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogprobs:
     """The ``k`` (at most 256) largest log-probabilities of ``softmax(logits / temperature)`` of every
-    row of ``logits [n, V]`` (CUDA, float32 / bfloat16 / float16), in one launch on the current stream.
+    row of ``logits [n, V]`` (CUDA, float32 / bfloat16 / float16), on the current stream.
     Rows with NaN or +inf logits, or only -inf, have NaN log-probabilities. No gradient flows back."""
     return TopLogprobs(*_launch(logits.detach(), int(k), temperature))

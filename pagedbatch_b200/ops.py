@@ -47,6 +47,24 @@ def pack_params(temperature, top_p, top_k, uniform, seeds=None, steps=None) -> n
     return rec
 
 
+class on_device:
+    """``torch.cuda.device(dev)``, at no cost where ``dev`` is the current device already."""
+
+    __slots__ = ("index", "prev")
+
+    def __init__(self, dev: torch.device):
+        self.index = dev.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.index is not None and self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.index is not None and self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
 GROUP_KMAX = 128  # largest top_k the two-pass launch of pb_sample_ws settles
 
 

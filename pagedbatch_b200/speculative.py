@@ -67,7 +67,7 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs):
         return tokens, accepted, status
     L = _lib.load()
     code = ops._DTYPE_CODE[logits.dtype]
-    with torch.cuda.device(dev):
+    with ops.on_device(dev):
         # a buffer of this call's own: the allocator hands it on in stream order, and a captured
         # graph keeps its copy
         ws = torch.empty(L.pb_verify_ws_bytes(R, V, code), dtype=torch.uint8, device=dev)

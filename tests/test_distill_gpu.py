@@ -112,6 +112,17 @@ def test_formula(cuda, tail, dtype, n, V, K):
 
 
 @pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 131003), (torch.float32, 131063), (torch.float32, 300007),
+                                     (torch.bfloat16, 600011), (torch.float16, 1 << 20)])
+def test_long_rows(cuda, tail, dtype, V):
+    """Rows at and beyond what a cluster holds in shared memory."""
+    z = torch.randn(2, V, generator=torch.Generator().manual_seed(V)).to(dtype)
+    lp, idx = entries(z, 40, 1)
+    check(z, lp, idx, tail=tail)
+    check(z, lp, idx, tail=tail, reduction="sum")
+
+
+@pytest.mark.parametrize("tail", [False, True])
 def test_many_rows(cuda, tail):
     z = workloads.head_boosted(700, 1000, seed=1, dtype=torch.bfloat16)
     lp, idx = entries(z, 16, 2)
@@ -206,6 +217,11 @@ def test_rows_that_do_not_count(cuda, tail):
     big = idx.long()
     big[4, 0] = 1 << 40
     assert pb.distill_loss(dev, lp.cuda(), big.cuda(), tail=tail)[4].isnan()
+    for i in (0, 300):  # a NaN of the teacher's, alone in its warp or not
+        wide_lp, wide = torch.full((1, 400), torch.nan), torch.full((1, 400), -1)
+        wide_lp[0, :2], wide[0, :2], wide[0, i] = -1.0, torch.tensor([3, 4]), 7
+        wide_lp[0, i] = torch.nan
+        assert pb.distill_loss(z[4:].cuda(), wide_lp.cuda(), wide.cuda(), tail=tail).isnan().all()
     z[:] = 1.0
     z[0], z[1] = torch.nan, -torch.inf
     nothing = pb.distill_loss(z[1:2].cuda(), lp[1:2].cuda(), idx[1:2].cuda(), tail=tail)

@@ -110,18 +110,18 @@ def test_c_abi_refusals(lib):
     assert lib.pb_verify_ws_bytes(-1, 8, 0) == -1 and lib.pb_verify_ws_bytes(1, 8, 7) == -1
 
     def top(**kw):
-        a = dict(logits=base, dtype=0, n_rows=2, vocab=8, stride=8, k=2, t=1.0, lp=base, idx=base, lse=base, stream=None) | kw
+        a = dict(logits=base, dtype=0, n_rows=2, vocab=8, stride=8, k=2, t=1.0, lp=base, idx=base, lse=base, ws=base, ws_bytes=1 << 20, stream=None) | kw
         return lib.pb_top_logprobs(*a.values())
 
     for kw in (dict(dtype=9), dict(n_rows=-1), dict(vocab=0), dict(stride=-1), dict(k=0), dict(k=9), dict(vocab=999, k=257),
                dict(t=0.0), dict(t=float("nan")), dict(t=float("inf")), dict(logits=None), dict(lp=None), dict(idx=None),
-               dict(lse=None), dict(logits=base + 1)):
+               dict(lse=None), dict(logits=base + 1), dict(ws=None), dict(ws=base + 16), dict(ws_bytes=64)):
         assert top(**kw) == -1, kw
     assert top(vocab=1 << 24) == -2 and top(n_rows=0, logits=None) == 0
 
     def forward(**kw):
         a = dict(z=base, dtype=0, n=2, vocab=8, stride=8, lp=base, ls=2, idx=base, xs=2, xb=4, k=2, t=1.0, tail=0, w=None,
-                 loss=base, stats=base, stream=None) | kw
+                 loss=base, stats=base, ws=base, ws_bytes=1 << 20, stream=None) | kw
         return lib.pb_distill_forward(*a.values())
 
     def backward(**kw):
@@ -132,12 +132,15 @@ def test_c_abi_refusals(lib):
     common = (dict(dtype=9), dict(n=-1), dict(vocab=0), dict(stride=-1), dict(ls=-1), dict(xs=-1), dict(xb=2), dict(k=0),
               dict(k=1025), dict(t=0.0), dict(t=float("nan")), dict(z=None), dict(lp=None), dict(idx=None), dict(stats=None),
               dict(stats=base + 4), dict(z=base + 1), dict(lp=base + 2), dict(idx=base + 4, xb=8))
-    for kw in (*common, dict(loss=None)):
+    for kw in (*common, dict(loss=None), dict(ws=None), dict(ws=base + 8), dict(ws_bytes=0)):
         assert forward(**kw) == -1, kw
     for kw in (*common, dict(grad=None), dict(dz=None), dict(gs=-1), dict(dz=base + 2)):
         assert backward(**kw) == -1, kw
     assert forward(vocab=(1 << 20) + 1) == -2 and backward(vocab=(1 << 20) + 1) == -2
     assert forward(n=0, z=None) == 0 and backward(n=0, z=None) == 0
+    assert lib.pb_distill_ws_bytes(1, 8, 9) == -1 and lib.pb_distill_ws_bytes(1, (1 << 20) + 1, 0) == -1
+    assert lib.pb_top_ws_bytes(1, 8, 9) == -1 and lib.pb_top_ws_bytes(-1, 8, 0) == -1
+    assert lib.pb_distill_sum(None, 1, base, None) == -1 and lib.pb_distill_sum(base, 1, None, None) == -1
     assert lib.pb_distill_stats_bytes(-1) == -1 and lib.pb_distill_stats_bytes(3) == 96
 
 
