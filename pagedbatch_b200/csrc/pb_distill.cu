@@ -24,7 +24,7 @@ using namespace pb;
 namespace {
 
 constexpr int DKMAX = PB_DISTILL_MAX_ENTRIES;    // entries per row
-constexpr int64_t DVMAX = PB_DISTILL_MAX_VOCAB;  // logits per row (one bit each in shared memory)
+constexpr int64_t DVMAX = PB_DISTILL_MAX_VOCAB;  // logits per row
 enum : int32_t { D_ROW = 0, D_EMPTY = 1, D_DUP = 2 };  // D_DUP: two entries name one element
 
 // log2 of the student's mass outside the entries below which there is none: logits there of -inf, or
@@ -167,7 +167,7 @@ struct GradRow {
 
 // CTA (row, segment): the sums of the segment's exponentials.
 template <typename T, bool TAIL>
-__global__ void __launch_bounds__(SEG_T, 4) part_kernel(DistillArgs a) {
+__global__ void __launch_bounds__(SEG_T, SEG_CTAS) part_kernel(DistillArgs a) {
   constexpr int EPV = Elem<T>::EPV;
   __shared__ uint32_t mask[SEG_T * SEG_V * EPV / 32];  // a bit per element of the segment: an entry's
   __shared__ uint32_t marked[SEG_T];                   // by thread: a bit per vector that holds an entry
@@ -225,10 +225,7 @@ __global__ void __launch_bounds__(SEG_T, 4) part_kernel(DistillArgs a) {
       }
     }
   }
-  RunningSum acc;
-#pragma unroll
-  for (int i = 0; i < SEG_V; i += 4) acc.template add<T, 4>(q + i, a.c);
-  const ExpSum rest = warp_expsum(acc.total(), a.c);
+  const ExpSum rest = warp_expsum(sum_segment<T>(q, v1 - v0, a.c).total(), a.c);
   if (TAIL) mem = warp_expsum(mem, a.c);
   if (lane == 0) warps[warp] = Part{rest, mem, 0, 0};
   __syncthreads();
@@ -250,22 +247,38 @@ __global__ void __launch_bounds__(256) finish_kernel(DistillArgs a) {
   const float wt = a.weight ? __ldg(a.weight + row) : 1.0f;
   const T* zr = static_cast<const T*>(a.z) + row * a.z_stride;
 
-  // the entries: sum of exp(value - top) (the tail's are probabilities as they are: top is 0)
+  // the entries: sum of exp(value - top) (the tail's are probabilities as they are: top is 0). The
+  // first FIRST are kept in registers, with their logits, and loaded together.
+  constexpr int FIRST = 128, PER = FIRST / 32;
+  int32_t ix[PER];
+  float val[PER], z[PER];
   bool any = false, bad = false;
   float top = -INFINITY, sum = 0.0f;
-  for (int i = lane; i < a.K; i += 32) {
-    const int64_t e = entry_index(a, row, i);
-    const float lp = __ldg(a.lp + row * a.lp_stride + i);
+  auto look = [&](int64_t e, float lp) {
     bad |= e < -1 || e >= a.V;
     if (e >= 0) {
       any = true;
       top = max_nan(top, lp);
     }
+  };
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = lane + 32 * j;
+    const int64_t e = i < a.K ? entry_index(a, row, i) : -1;
+    val[j] = i < a.K ? __ldg(a.lp + row * a.lp_stride + i) : 0.0f;
+    look(e, val[j]);
+    ix[j] = e >= 0 && e < a.V ? (int32_t)e : -1;
   }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) z[j] = ix[j] >= 0 ? Elem<T>::ld(zr + ix[j]) : 0.0f;
+  for (int i = FIRST + lane; i < a.K; i += 32) look(entry_index(a, row, i), __ldg(a.lp + row * a.lp_stride + i));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   if (TAIL || top == -INFINITY) top = 0.0f;
-  for (int i = lane; i < a.K; i += 32)
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (ix[j] >= 0) sum += expf(val[j] - top);
+  for (int i = FIRST + lane; i < a.K; i += 32)
     if (entry_index(a, row, i) >= 0) sum += expf(__ldg(a.lp + row * a.lp_stride + i) - top);
   sum = warp_sum(sum);
   any = __any_sync(0xFFFFFFFFu, any);
@@ -301,12 +314,17 @@ __global__ void __launch_bounds__(256) finish_kernel(DistillArgs a) {
   st.norm = norm;
   st.flags = dup ? D_DUP : D_ROW;
   float dot = 0.0f;
-  for (int i = lane; i < a.K; i += 32) {
-    const int64_t e = entry_index(a, row, i);
-    if (e < 0 || e >= a.V) continue;
-    const float lp = __ldg(a.lp + row * a.lp_stride + i), t = expf(lp - norm);
+  auto term = [&](float lp, float zi) {
+    const float t = expf(lp - norm);
     if (t != 0.0f)  // (NaN counts)
-      dot += t * ((lp - norm) - ((Elem<T>::ld(zr + e) - full.m) * a.inv_tau - st.all_l * LN2));
+      dot += t * ((lp - norm) - ((zi - full.m) * a.inv_tau - st.all_l * LN2));
+  };
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (ix[j] >= 0) term(val[j], z[j]);
+  for (int i = FIRST + lane; i < a.K; i += 32) {
+    const int64_t e = entry_index(a, row, i);
+    if (e >= 0 && e < a.V) term(__ldg(a.lp + row * a.lp_stride + i), Elem<T>::ld(zr + e));
   }
   float loss = warp_sum(dot);
   if (TAIL) {
@@ -381,13 +399,13 @@ int forward_as(const DistillArgs& a, cudaStream_t st) {
 
 template <typename T>
 int forward(DistillArgs a, cudaStream_t st) {
-  a.seg = seg_plan(a.V, sizeof(T));
+  a.seg = seg_plan(a.V, sizeof(T), a.z, a.z_stride);
   return a.tail ? forward_as<T, true>(a, st) : forward_as<T, false>(a, st);
 }
 
 template <typename T>
 int backward(DistillArgs a, cudaStream_t st) {
-  a.seg = seg_plan(a.V, sizeof(T));
+  a.seg = seg_plan(a.V, sizeof(T), a.z, a.z_stride);
   backward_kernel<T><<<dim3((unsigned)a.n, (unsigned)a.seg.segs), SEG_T, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? PB_OK : PB_E_LAUNCH;
 }
@@ -419,7 +437,7 @@ int64_t pb_distill_stats_bytes(int64_t n_rows) { return n_rows < 0 ? PB_E_INVALI
 int64_t pb_distill_ws_bytes(int64_t n_rows, int64_t vocab, int dtype) {
   const int es = elem_size(dtype);
   if (n_rows < 0 || vocab <= 0 || vocab > DVMAX || !es) return PB_E_INVALID;
-  return n_rows * seg_plan(vocab, es).segs * (int64_t)sizeof(Part);
+  return n_rows * seg_plan(vocab, es, nullptr, 1).segs * (int64_t)sizeof(Part)  /* rows of any alignment */;
 }
 
 int pb_distill_forward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,

@@ -216,17 +216,15 @@ __device__ __forceinline__ ExpSum warp_expsum(ExpSum v, float c) {
   return ExpSum{m, warp_sum(v.s * ex2((v.m - m) * c))};
 }
 
-// The join over the block (NWARP warps); every thread gets it. `scratch` holds NWARP entries; one
-// barrier, so the caller separates two uses of the same scratch.
+// The join over the block (NWARP warps), in warp 0's lanes only. `scratch` holds NWARP entries; one
+// barrier.
 template <int NWARP>
 __device__ __forceinline__ ExpSum block_expsum(ExpSum v, float c, ExpSum* scratch) {
   v = warp_expsum(v, c);
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
-  ExpSum r = scratch[0];
-#pragma unroll
-  for (int w = 1; w < NWARP; ++w) r = expsum_join(r, scratch[w], c);
-  return r;
+  if (threadIdx.x < 32) v = warp_expsum(threadIdx.x < NWARP ? scratch[threadIdx.x] : expsum_empty(), c);
+  return v;
 }
 
 // ---- segments ---------------------------------------------------------------------------------
@@ -240,12 +238,15 @@ __device__ __forceinline__ ExpSum block_expsum(ExpSum v, float c, ExpSum* scratc
 constexpr int SEG_T = 256;
 constexpr int SEG_NW = SEG_T / 32;
 constexpr int SEG_V = 8;
+constexpr int SEG_CTAS = 5;  // CTAs per SM of the launches that read segments
 
 struct SegPlan {
   int32_t segs, per;  // segments per row, vectors per segment (equal shares of the longest row)
 };
-inline SegPlan seg_plan(int64_t V, int es) {
-  const int64_t epv = 16 / es, nvec = (V + 2 * epv - 2) / epv;  // the most vectors a row of any alignment has
+inline SegPlan seg_plan(int64_t V, int es, const void* rows, int64_t row_stride) {
+  // a row's vectors: exactly, where every row starts on a 16-byte boundary, else the most it can have
+  const bool even = reinterpret_cast<uintptr_t>(rows) % 16 == 0 && row_stride * es % 16 == 0;
+  const int64_t epv = 16 / es, nvec = even ? (V + epv - 1) / epv : (V + 2 * epv - 2) / epv;
   SegPlan p;
   p.segs = (int32_t)((nvec + SEG_T * SEG_V - 1) / (SEG_T * SEG_V));
   p.per = (int32_t)((nvec + p.segs - 1) / p.segs);
@@ -280,6 +281,40 @@ __device__ __forceinline__ void load_segment(const RowView<T>& r, int32_t v0, in
       q[i].w = here ? p.w : q[i].w;
     }
   }
+}
+
+// Sum of the segment's exponentials, and its largest element (NaN if one is).
+template <typename T>
+__device__ __forceinline__ RunningSum sum_segment(const uint4* q, int32_t n, float c, float* largest = nullptr) {
+  RunningSum acc;
+  float mx = acc.template add<T, 4>(q, c);
+  if (n > 6 * SEG_T) mx = max_nan(mx, acc.template add<T, 4>(q + 4, c));  // (no thread has a vector past n)
+  else if (n > 4 * SEG_T) mx = max_nan(mx, acc.template add<T, 2>(q + 4, c));
+  if (largest) *largest = mx;
+  return acc;
+}
+
+// The largest element of each 128-byte group (8 vectors side by side, held by 8 lanes) of the segment:
+// thread t ends with the largest of group t, vectors group_of(t) to group_of(t) + 7 of the segment. The
+// eight lanes' eight words are reduced by halves: four words change hands, then two, then one.
+__device__ __forceinline__ int32_t group_of(int32_t t) { return (t & 7) * SEG_T + (t & ~7); }
+template <typename T>
+__device__ __forceinline__ float group_largest(const uint4* q) {
+  static_assert(SEG_V == 8, "eight words for eight lanes");
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = Elem<T>::max2(Elem<T>::max2(q[i].x, q[i].y), Elem<T>::max2(q[i].z, q[i].w));
+  const uint32_t lane = threadIdx.x & 7;
+#pragma unroll
+  for (int half = 4; half > 0; half >>= 1) {
+    const bool up = (lane & half) != 0;  // this lane keeps the upper half of the words
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const uint32_t give = up ? w[i] : w[i + half], keep = up ? w[i + half] : w[i];
+      w[i] = Elem<T>::max2(keep, __shfl_xor_sync(0xFFFFFFFFu, give, half));
+    }
+  }
+  return Elem<T>::word_max(w[0]);
 }
 
 // Start the launch that follows on the stream as soon as this grid's CTAs have all begun (it waits

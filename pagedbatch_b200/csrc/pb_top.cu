@@ -6,13 +6,15 @@
 //   (the sampler's order). A row holding NaN or +inf, or only -inf, has NaN log-probabilities.
 //
 // Two launches. part_kernel reads every row once, a CTA per segment of it: per thread a running
-// maximum and sum of exponentials, and the key of the largest value of its vectors (its group).
+// maximum and sum of exponentials, and for the CTA the key of the largest value of every 128 bytes (a
+// group).
 // select_kernel, a CTA per row: a lower bound of the k-th largest value follows from the lanes'
 // largest group keys, since each of its 8 warps holds ceil(k / 8) values at or above its
-// ceil(k / 8)-th largest lane maximum, so the row holds k at or above the smallest of these. Only the
-// groups whose key reaches the bound are read again (from L2); their values at or above it are the
-// candidates, a little more than k, put in order by counting for each the candidates before it, or
-// where they are many by a bitonic network. A row with more candidates than the list holds (very many
+// ceil(k / 8)-th largest lane maximum, so the row holds k at or above the smallest of these. A
+// histogram of the group keys above that bound (256 equal steps up to the largest key) raises it to
+// the step that k of them reach. Only the groups whose key reaches the raised bound are read again
+// (from L2); their values at or above it are the candidates, a little more than k, put in order by
+// counting for each the candidates before it, or where they are many by a bitonic network. A row with more candidates than the list holds (very many
 // equal values) is selected by bisection over (value, index).
 // HBM-bound: V * es bytes a row, and 1/32 of that written as keys.
 #include "pb_rows.cuh"
@@ -45,7 +47,10 @@ struct TopArgs {
 
 struct TopShared {
   ExpSum sum[TNW];
-  uint32_t bound[TNW];
+  uint32_t bound[TNW], top[TNW];
+  uint32_t hist[TT];                // group keys by step above the bound
+  uint32_t steps[TNW];
+  uint32_t raised;                  // the bound raised by the histogram
   uint32_t groups;                  // groups listed
   uint32_t n;                       // candidates
   uint32_t cnt[2];                  // bisection counts
@@ -127,7 +132,7 @@ __device__ __noinline__ void select_slow(const RowView<T>& rv, int k, TopShared&
 }
 
 template <typename T>
-__global__ void __launch_bounds__(TT, 4) part_kernel(TopArgs a) {
+__global__ void __launch_bounds__(TT, SEG_CTAS) part_kernel(TopArgs a) {
   __shared__ ExpSum scratch[TNW];
   const int64_t row = blockIdx.x;
   const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
@@ -135,13 +140,9 @@ __global__ void __launch_bounds__(TT, 4) part_kernel(TopArgs a) {
   uint4 q[SEG_V];
   load_segment(rv, v0, v1, q);
   grid_release();
-  RunningSum acc;
-  float mx = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < SEG_V; i += 4) mx = max_nan(mx, acc.template add<T, 4>(q + i, a.c));
   const int64_t part = row * a.seg.segs + blockIdx.y;
-  a.keys[part * TT + threadIdx.x] = key_of(mx);
-  const ExpSum sum = block_expsum<TNW>(acc.total(), a.c, scratch);
+  a.keys[part * TT + threadIdx.x] = key_of(group_largest<T>(q));
+  const ExpSum sum = block_expsum<TNW>(sum_segment<T>(q, v1 - v0, a.c).total(), a.c, scratch);
   if (threadIdx.x == 0) a.parts[part] = sum;
 }
 
@@ -154,6 +155,7 @@ __global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
   const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
   const int32_t segs = a.seg.segs;
   if (tid == 0) sh.groups = sh.n = 0;
+  sh.hist[tid] = 0;
   grid_wait();  // the segments' keys and sums
   const uint32_t* keys = a.keys + row * segs * TT + tid;
   constexpr int HELD = 16;  // keys a thread keeps; longer rows' are read twice
@@ -169,19 +171,48 @@ __global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
   for (int s = 0; s < HELD; ++s) lmax = max(lmax, key[s]);
   for (int32_t s = HELD; s < segs; ++s) lmax = max(lmax, __ldcg(keys + (int64_t)s * TT));
   const uint32_t wb = warp_nth_largest(lmax, (a.k + TNW - 1) / TNW);
+  const uint32_t wt = __reduce_max_sync(0xFFFFFFFFu, lmax);
   sum = warp_expsum(sum, a.c);
   if (lane == 0) {
     sh.bound[warp] = wb;
+    sh.top[warp] = wt;
     sh.sum[warp] = sum;
   }
   __syncthreads();
-  uint32_t bound = sh.bound[0];
-  sum = sh.sum[0];
+  uint32_t bound = sh.bound[0], top = sh.top[0];
 #pragma unroll
   for (int w = 1; w < TNW; ++w) {
     bound = min(bound, sh.bound[w]);
-    sum = expsum_join(sum, sh.sum[w], a.c);
+    top = max(top, sh.top[w]);
   }
+  // raise the bound: group keys at or above it, by step; then the steps from the top until k are held
+  // (each group's key is a value of the row, so k values reach the last of these steps)
+  const int shift = max(0, 24 - __clz(top - bound));  // the span above the bound in at most TT steps
+  auto count_key = [&](uint32_t k) {
+    if (k >= bound) atomicAdd(&sh.hist[(k - bound) >> shift], 1u);
+  };
+#pragma unroll
+  for (int s = 0; s < HELD; ++s)
+    if (s < segs) count_key(key[s]);
+  for (int32_t s = HELD; s < segs; ++s) count_key(__ldcg(keys + (int64_t)s * TT));
+  if (warp == 0) {
+    sum = warp_expsum(lane < TNW ? sh.sum[lane] : expsum_empty(), a.c);
+    if (lane == 0) sh.sum[0] = sum;
+  }
+  __syncthreads();
+  {
+    const uint32_t h = sh.hist[TT - 1 - tid];  // from the top step down
+    const uint32_t incl = warp_incl_scan(h);
+    if (lane == 31) sh.steps[warp] = incl;
+    if (tid == 0) sh.raised = bound;
+    __syncthreads();
+    uint32_t before = incl - h;
+    for (int w = 0; w < warp; ++w) before += sh.steps[w];
+    if (before < (uint32_t)a.k && before + h >= (uint32_t)a.k) sh.raised = bound + ((uint32_t)(TT - 1 - tid) << shift);
+    __syncthreads();
+  }
+  sum = sh.sum[0];
+  bound = sh.raised;
 
   // the groups that reach the bound, then the values in them that do
   auto list_group = [&](int32_t s, bool hit) {
@@ -199,22 +230,37 @@ __global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
   __syncthreads();
   const uint32_t groups = sh.groups;
   if (groups <= (uint32_t)TLIST) {
-    for (uint32_t i = tid; i < groups * SEG_V; i += TT) {
-      const uint32_t g = sh.group[i / SEG_V];
-      const int32_t v0 = (int32_t)(g / TT) * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
-      const int32_t v = v0 + (int32_t)(g % TT) + (int32_t)(i % SEG_V) * TT;
-      if (v >= v1) continue;
-      const uint4 q = load_vec(rv, v);
-      if (key_of(vec_max_nan<T>(q)) < bound) continue;
-      float x[EPV];
-      Elem<T>::unpack(q, x);
+    constexpr int AHEAD = 4;  // vectors a thread has in flight
+    for (uint32_t i0 = tid; i0 < groups * SEG_V; i0 += TT * AHEAD) {
+      uint4 q[AHEAD];
+      int32_t v[AHEAD];
 #pragma unroll
-      for (int j = 0; j < EPV; ++j) {
-        const uint32_t kx = key_of(x[j]);
-        const int32_t e = rv.first(v) + j;
-        if (kx >= bound && e >= 0 && e < a.V) {
-          const uint32_t at = atomicAdd(&sh.n, 1u);
-          if (at < (uint32_t)TCAP) sh.list[at] = compose(kx, (uint32_t)e);
+      for (int u = 0; u < AHEAD; ++u) {
+        const uint32_t i = i0 + u * TT;
+        v[u] = -1;
+        if (i < groups * SEG_V) {
+          const uint32_t g = sh.group[i / SEG_V];
+          const int32_t v0 = (int32_t)(g / TT) * a.seg.per;
+          const int32_t at = v0 + group_of((int32_t)(g % TT)) + (int32_t)(i % SEG_V);
+          if (at < min(rv.nvec, v0 + a.seg.per)) {
+            v[u] = at;
+            q[u] = load_vec(rv, at);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (v[u] < 0 || key_of(vec_max_nan<T>(q[u])) < bound) continue;
+        float x[EPV];
+        Elem<T>::unpack(q[u], x);
+#pragma unroll
+        for (int j = 0; j < EPV; ++j) {
+          const uint32_t kx = key_of(x[j]);
+          const int32_t e = rv.first(v[u]) + j;
+          if (kx >= bound && e >= 0 && e < a.V) {
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            if (at < (uint32_t)TCAP) sh.list[at] = compose(kx, (uint32_t)e);
+          }
         }
       }
     }
@@ -274,9 +320,9 @@ struct TopPlan {
   SegPlan seg;
   int64_t keys, bytes;  // offset of the keys in the workspace, and its size
 };
-TopPlan top_plan(int64_t n, int64_t V, int es) {
+TopPlan top_plan(int64_t n, int64_t V, int es, const void* rows, int64_t row_stride) {
   TopPlan p;
-  p.seg = seg_plan(V, es);
+  p.seg = seg_plan(V, es, rows, row_stride);
   p.keys = (n * p.seg.segs * (int64_t)sizeof(ExpSum) + 255) & ~(int64_t)255;
   p.bytes = p.keys + n * p.seg.segs * TT * 4;
   return p;
@@ -296,7 +342,7 @@ extern "C" {
 int64_t pb_top_ws_bytes(int64_t n_rows, int64_t vocab, int dtype) {
   const int es = elem_size(dtype);
   if (n_rows < 0 || vocab <= 0 || !es) return PB_E_INVALID;
-  return top_plan(n_rows, vocab, es).bytes;
+  return top_plan(n_rows, vocab, es, nullptr, 1).bytes;  // (rows of any alignment: the most it takes)
 }
 
 int pb_top_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride, int32_t k,
@@ -311,7 +357,7 @@ int pb_top_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab
   if (!logits || !out_logprob || !out_index || !out_lse) return PB_E_INVALID;
   if (n_rows > (int64_t)(0x7FFFFFFF / 8)) return PB_E_INVALID;
   if (reinterpret_cast<uintptr_t>(logits) % es) return PB_E_INVALID;
-  const TopPlan plan = top_plan(n_rows, vocab, es);
+  const TopPlan plan = top_plan(n_rows, vocab, es, logits, row_stride);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || ws_bytes < plan.bytes) return PB_E_INVALID;
   TopArgs a;
   a.x = logits;
