@@ -140,7 +140,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     L.pb_stop_check.argtypes = [vp, i64, vp, vp, vp, i32, i32, vp, vp]
     L.pb_stop_check.restype = i32
     f32 = ctypes.c_float
-    L.pb_verify_ws_bytes.argtypes = [i64, i64, i32]
+    L.pb_verify_ws_bytes.argtypes = [i64, i64, i64, i32]
     L.pb_verify_ws_bytes.restype = i64
     L.pb_verify.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, i32, i64, i64, i32, vp, vp, vp, vp, i64, vp]
     L.pb_verify.restype = i32

@@ -13,19 +13,47 @@
 // prefix exceeds t; an empty residual is replaced by P. Greedy rows accept the first maximum only.
 // Both steps leave every token distributed as the target's own samples are.
 //
-//   1. expand: each row's parameters from its sequence's.
-//   2. the sampler over the rows (its info record describes the kept set and its mass); rows without
-//      top-k and top-p, whose kept set is the whole row, are summed by mass_kernel instead.
-//   3. pick: one cluster per sequence finds the first rejected row and draws the last token from it.
+// Launches, each of which may start while the one before it ends:
+//   1. expand_kernel: each row's parameters from its sequence's.
+//   2. the sampler over the rows (its info record describes the kept set and its mass). Rows without
+//      top-k and top-p, whose kept set is the whole row, go through max_kernel and mass_kernel instead:
+//      two passes in segments, the largest value and then the sum of the weights.
+//   3. decide_kernel: a CTA per sequence finds the first rejected row.
+//   4. weigh_kernel: that row's weights, summed per tile (256 vectors), a CTA per segment.
+//   5. draw_kernel: a CTA per sequence finds the draw's tile and its element.
+// Weights are exact integers throughout (multiples of 2^-40 below 2^13, which fp64 adds without
+// rounding), so no result depends on an order of addition.
 #include "pb_rows.cuh"
 
 using namespace pb;
 
 namespace {
 
-constexpr int VT = 512;          // threads per CTA
-constexpr int VNW = VT / 32;
-constexpr int VSTEPS = 64;       // parts of a warp's share of a row whose sums are kept for the draw
+constexpr int VT = SEG_T;        // threads per CTA
+constexpr int VNW = SEG_NW;
+constexpr int TILES = SEG_V;     // tiles per segment: tile i holds vectors v0 + i * SEG_T + thread
+
+// A row as the passes over whole rows see it.
+struct RowMeta {
+  float t;           // temperature
+  int32_t whole;     // the row's kept set is the whole row
+  uint32_t max_key;  // key of its largest value (max_kernel)
+  int32_t pad;
+};
+
+// Sums of one tile of the row a sequence draws from, in units of 2^-40. Where top-p cut among the
+// equals of the last kept key, `w` leaves those equals out, `tie_w` is theirs and `ties` counts them.
+struct Tile {
+  uint64_t w, tie_w;
+  int32_t ties, pad;
+};
+
+// Where a sequence stopped.
+struct Decision {
+  int64_t row;
+  int32_t kind;   // EV_*
+  int32_t draws;  // the last token is drawn from the row's weights
+};
 
 struct VerifyArgs {
   const void* x;
@@ -39,10 +67,15 @@ struct VerifyArgs {
   const void* probs;             // [n_probs][V], or null
   int64_t probs_stride, n_probs;
   int32_t probs_dtype;
-  int32_t sampler_runs, mass_runs;
+  int32_t mass_runs;
   pb_row_params* rowp;           // workspace: [n_rows]
   pb_row_info* info;             // workspace: [n_rows]
   int64_t* tok;                  // workspace: [n_rows], the sampler's tokens (greedy rows' maxima)
+  RowMeta* meta;                 // workspace: [n_rows]
+  Decision* decision;            // workspace: [n_seqs]
+  Tile* tiles;                   // workspace: [n_seqs][segs][TILES]
+  SegPlan seg;
+  int32_t all_whole;
   int64_t* out_tokens;           // [n_rows]
   int32_t* out_accepted;         // [n_seqs]
   int32_t* out_status;           // [n_seqs] or null
@@ -66,10 +99,14 @@ __global__ void __launch_bounds__(256) expand_kernel(VerifyArgs a) {
   pb_row_params p = a.params[lo];
   p.uniform = 0.0;  // the sampler's own draw is not used
   p.rng = 0;
+  const bool whole = a.mass_runs && whole_row(p, a.V);
+  a.meta[r] = RowMeta{(float)p.temperature, whole, 0u, 0};
   // mass_kernel sums these; the sampler passes over them as greedy rows, its cheapest kind
-  if (a.mass_runs && a.sampler_runs && whole_row(p, a.V)) p.temperature = 0.0;
+  if (whole) p.temperature = 0.0;
   a.rowp[r] = p;
-  a.info[r].status = PB_ROW_INTERNAL;  // until a launch settles the row
+  pb_row_info* o = a.info + r;
+  o->status = PB_ROW_INTERNAL;  // until a launch settles the row
+  o->z_q = o->kept_q = 0;
   a.tok[r] = -1;
   a.out_tokens[r] = -1;
 }
@@ -87,70 +124,127 @@ struct Scale {
   }
 };
 
-struct MassShared {
-  uint32_t top[VNW];
-  uint64_t sum[VNW];
-  uint32_t pub_max;
-  uint64_t pub_sum;
-};
+// ---- weights ---------------------------------------------------------------------------------
 
-// Mass of a whole row: the largest scaled key, then the sum of the fixed-point weights. One cluster
-// per row; the second pass reads its slice from L2.
-template <typename T>
-__global__ void __launch_bounds__(VT, 2) mass_kernel(VerifyArgs a) {
-  constexpr int EPV = Elem<T>::EPV;
-  __shared__ MassShared sh;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t row = blockIdx.x / C;
-  const int tid = threadIdx.x;
-  int64_t lo = 0, hi = a.n_seqs;
-  while (hi - lo > 1) {
-    const int64_t mid = lo + ((hi - lo) >> 1);
-    if ((int64_t)a.offsets[mid] <= row) lo = mid;
-    else hi = mid;
+// The sampler's weights of a vector's elements, e^(x / T - m) as exp_weight computes it (before its
+// scaling to 2^40), for rows of ordinary values. Every step is the same correctly rounded operation,
+// two elements at a time:
+//  * x / T: a product with the exact reciprocal of a power of two, else by Markstein's division
+//    (IBM J. Res. Dev. 34, 1990): with y = RN(1 / T), two corrections q += (x - q T) y, the remainders
+//    exact in one fused operation each, give RN(x / T) while nothing over- or underflows;
+//  * keys further than 40 below the maximum, whose weight is below 2^-40, are taken as 40 below it.
+struct Weigher {
+  float t, y, inv, m;
+  bool fast;  // the row's values are ordinary enough for the packed steps
+  __device__ Weigher(float t_, float m_, float raw_max) : t(t_), m(m_) {
+    const Scale s(t_);
+    inv = s.inv;
+    y = __frcp_rn(t_);
+    const float a = fabsf(raw_max);
+    fast = a >= 0x1p-40f && a <= 0x1p60f && t_ >= 0x1p-40f && t_ <= 0x1p40f;
   }
-  const pb_row_params p = a.params[lo];
-  if (!whole_row(p, a.V)) return;  // the whole cluster leaves
-  const Scale scaled((float)p.temperature);
-  const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
-  const int32_t v0 = (int32_t)((int64_t)rv.nvec * rank / C), v1 = (int32_t)((int64_t)rv.nvec * (rank + 1) / C);
-  uint32_t mk = 0;
-  for (int32_t v = v0 + tid; v < v1; v += VT) mk = max(mk, key_of(vec_max_nan<T>(load_vec(rv, v))));
-  mk = __reduce_max_sync(0xFFFFFFFFu, mk);
-  if ((tid & 31) == 0) sh.top[tid >> 5] = mk;
-  __syncthreads();
-  mk = 0;
-  for (int w = 0; w < VNW; ++w) mk = max(mk, sh.top[w]);
-  if (C > 1) {
-    if (tid == 0) sh.pub_max = mk;
-    cluster.sync();
-    for (int r = 0; r < C; ++r) mk = max(mk, cluster.map_shared_rank(&sh, r)->pub_max);
-  }
-  const float m = scaled(value_of(mk));
-  const uint32_t sk = key_of(m);
-  const bool ok = mk != 0xFFFFFFFFu && sk < KEY_POS_INF && sk > KEY_NEG_INF;
-  uint64_t z = 0;
-  if (ok) {
-    for (int32_t v = v0 + tid; v < v1; v += VT) {
-      float x[EPV];
-      Elem<T>::unpack(load_vec(rv, v), x);
+  template <typename T>
+  __device__ __forceinline__ void of(uint4 v, float* w) const {
+    constexpr int EPV = Elem<T>::EPV;
+    float x[EPV];
+    Elem<T>::unpack(v, x);
+    if (!fast) {
+      const Scale s(t);
 #pragma unroll
-      for (int q = 0; q < EPV; ++q) z += weight_q(scaled(x[q]), m);  // elements outside the row are -inf: 0
+      for (int q = 0; q < EPV; ++q) w[q] = exp_weight(__fsub_rn(s(x[q]), m));
+      return;
+    }
+    const uint64_t m2 = pack2(-m, -m);
+#pragma unroll
+    for (int q = 0; q < EPV; q += 2) {
+      uint64_t k;
+      if (inv != 0.0f) {
+        k = mul2(pack2(x[q], x[q + 1]), pack2(inv, inv));
+      } else {
+        // (values below -2^100 have no weight: taken as that, so that -inf divides)
+        const uint64_t x2 = pack2(fmaxf(x[q], -0x1p100f), fmaxf(x[q + 1], -0x1p100f)), y2 = pack2(y, y), t2 = pack2(-t, -t);
+        k = mul2(x2, y2);
+        k = fma2(fma2(k, t2, x2), y2, k);
+        k = fma2(fma2(k, t2, x2), y2, k);
+      }
+      float d0, d1;
+      unpack2(add2(k, m2), d0, d1);
+      const uint64_t d = pack2(fmaxf(d0, -40.0f), fmaxf(d1, -40.0f));
+      constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
+      const uint64_t tn = add2(mul2(d, pack2(0x1.715476p+0f, 0x1.715476p+0f)), pack2(MAGIC, MAGIC));
+      const uint64_t n = add2(tn, pack2(-MAGIC, -MAGIC));
+      uint64_t r = fma2(n, pack2(-0x1.62e43p-1f, -0x1.62e43p-1f), d);
+      r = fma2(n, pack2(0x1.05c61p-29f, 0x1.05c61p-29f), r);
+      uint64_t p = pack2(0x1.a01a02p-13f, 0x1.a01a02p-13f);
+      p = fma2(p, r, pack2(0x1.6c16c2p-10f, 0x1.6c16c2p-10f));
+      p = fma2(p, r, pack2(0x1.111112p-7f, 0x1.111112p-7f));
+      p = fma2(p, r, pack2(0x1.555556p-5f, 0x1.555556p-5f));
+      p = fma2(p, r, pack2(0x1.555556p-3f, 0x1.555556p-3f));
+      p = fma2(p, r, pack2(0.5f, 0.5f));
+      p = fma2(p, r, pack2(1.0f, 1.0f));
+      p = fma2(p, r, pack2(1.0f, 1.0f));
+      float p0, p1, n0, n1;
+      unpack2(p, p0, p1);
+      unpack2(tn, n0, n1);
+      // (the low bits of MAGIC + n are n, and MAGIC's own leave the word with the shift)
+      w[q] = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
+      w[q + 1] = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
     }
   }
-  z = warp_sum(z);
-  if ((tid & 31) == 0) sh.sum[tid >> 5] = z;
-  __syncthreads();
-  z = 0;
-  for (int w = 0; w < VNW; ++w) z += sh.sum[w];
-  if (C > 1) {
-    if (tid == 0) sh.pub_sum = z;
-    cluster.sync();
-    if (rank == 0 && tid == 0)
-      for (int r = 1; r < C; ++r) z += cluster.map_shared_rank(&sh, r)->pub_sum;
+};
+
+// Exact sums of weights floored to multiples of 2^-40: a double of 2^12 has its last place there, so
+// adding to it towards minus infinity floors what is added. Room for 4095 weights of 1.
+constexpr double GRID = 4096.0;
+__device__ __forceinline__ double on_grid(float w) { return __dadd_rd(GRID, (double)w); }  // GRID + floor
+__device__ __forceinline__ uint64_t grid_units(double sum) {                               // sum - GRID in 2^-40
+  return (uint64_t)__double_as_longlong(sum) & ((1ull << 52) - 1);
+}
+
+// Key of the largest value of every whole row.
+template <typename T>
+__global__ void __launch_bounds__(VT, SEG_CTAS) max_kernel(VerifyArgs a) {
+  __shared__ uint32_t top[VNW];
+  grid_release();
+  const int64_t row = blockIdx.x;
+  if (!a.all_whole) {
+    grid_wait();
+    if (!a.meta[row].whole) return;
   }
-  if (rank == 0 && tid == 0) {
+  const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
+  const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+  uint4 q[SEG_V];
+  load_segment(rv, v0, v1, q);
+  uint32_t k = __reduce_max_sync(0xFFFFFFFFu, key_of(vecs_max_nan<T, SEG_V>(q)));
+  if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = k;
+  __syncthreads();
+  grid_wait();  // expand_kernel has set the keys to 0
+  if (threadIdx.x < 32) {
+    k = __reduce_max_sync(0xFFFFFFFFu, threadIdx.x < VNW ? top[threadIdx.x] : 0u);
+    if (threadIdx.x == 0) atomicMax(&a.meta[row].max_key, k);
+  }
+}
+
+// Mass of every whole row: the sum of its weights. Rows are taken from the last one back, since the
+// last ones that max_kernel read are still in L2.
+template <typename T>
+__global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
+  constexpr int EPV = Elem<T>::EPV;
+  __shared__ uint64_t part[VNW];
+  grid_release();
+  const int64_t row = a.n_rows - 1 - blockIdx.x;
+  const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
+  const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+  uint4 q[SEG_V];
+  if (a.all_whole) load_segment(rv, v0, v1, q);
+  grid_wait();  // the rows' largest values
+  const RowMeta meta = a.meta[row];
+  if (!meta.whole) return;
+  if (!a.all_whole) load_segment(rv, v0, v1, q);
+  const float raw = value_of(meta.max_key), m = Scale(meta.t)(raw);
+  const uint32_t sk = key_of(m);
+  const bool ok = meta.max_key != 0xFFFFFFFFu && sk < KEY_POS_INF && sk > KEY_NEG_INF;
+  if (blockIdx.y == 0 && threadIdx.x == 0) {
     pb_row_info* o = a.info + row;
     o->thr_key = 0;  // every key is above it
     o->n_tie_kept = 0;
@@ -158,25 +252,34 @@ __global__ void __launch_bounds__(VT, 2) mass_kernel(VerifyArgs a) {
     o->status = ok ? PB_ROW_OK : PB_ROW_NONFINITE;
     o->max_key = m;
     o->flags = PB_PATH_LARGE;
-    o->z_q = z;
-    o->kept_q = z;
   }
-  if (C > 1) cluster.sync();
+  if (!ok) return;
+  const Weigher weigh(meta.t, m, raw);
+  double s0 = GRID, s1 = GRID;  // (at most SEG_V * EPV weights of 1 in both)
+#pragma unroll
+  for (int i = 0; i < SEG_V; ++i) {
+    if (i * SEG_T >= v1 - v0) break;
+    float w[EPV];
+    weigh.template of<T>(q[i], w);  // elements outside the row are -inf: no weight
+#pragma unroll
+    for (int j = 0; j < EPV; j += 2) {
+      s0 = __dadd_rd(s0, (double)w[j]);
+      s1 = __dadd_rd(s1, (double)w[j + 1]);
+    }
+  }
+  uint64_t z = warp_sum(grid_units(s0) + grid_units(s1));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = z;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    z = warp_sum(threadIdx.x < VNW ? part[threadIdx.x] : 0ull);
+    if (threadIdx.x == 0) {  // (whole numbers: the order of the segments does not matter)
+      atomicAdd(reinterpret_cast<unsigned long long*>(&a.info[row].z_q), (unsigned long long)z);
+      atomicAdd(reinterpret_cast<unsigned long long*>(&a.info[row].kept_q), (unsigned long long)z);
+    }
+  }
 }
 
-// ---- pick ----------------------------------------------------------------------------------------
-
-struct PickShared {
-  uint64_t res[VNW][VSTEPS], all[VNW][VSTEPS];  // sums of a warp's parts: residual, target
-  uint64_t wres[VNW], wall[VNW];
-  uint32_t wtie[VNW];
-  uint32_t ctie;
-  int32_t event, kind;
-  // rank 0's decision
-  int32_t owner, use_all;  // cluster-wide warp that holds the draw, which sums it goes by
-  uint64_t left;           // the draw's target inside that warp
-  uint32_t cnt[2];
-};
+// ---- deciding --------------------------------------------------------------------------------
 
 enum : int32_t { EV_REJECT = 0, EV_BAD = 1, EV_TIE = 2, EV_LAST = 3 };
 
@@ -187,45 +290,45 @@ __device__ __forceinline__ float prob_at(const VerifyArgs& a, int64_t d, int64_t
   return Elem<__half>::ld(static_cast<const __half*>(a.probs) + at);
 }
 
-// What the draft's distribution takes of a target weight of mass scale zd: floor(d * Z), 0 for d <= 0
-// or NaN (fp64: d has at most 24 bits and Z is rounded to 53, one rounding of the product).
-__device__ __forceinline__ uint64_t taken_of(float d, double zd) {
-  if (!(d > 0.0f)) return 0;
-  const double t = __dmul_rn((double)d, zd);
-  return (t >= 0x1p63) ? ~0ull : (uint64_t)t;
+// Raw values below this are surely below the scaled key thr (a few roundings of the quotient apart).
+__device__ __forceinline__ float surely_below(uint32_t thr, float tf) {
+  if (!(thr > KEY_NEG_INF && thr < KEY_POS_INF)) return -INFINITY;
+  const float b = value_of(thr) * tf, r = b - fabsf(b) * 0x1p-20f - 0x1p-100f;
+  return (r > -INFINITY) ? r : -INFINITY;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(VT, 2) pick_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(VT, 4) decide_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
-  __shared__ PickShared sh;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t seq = blockIdx.x / C;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ struct {
+    int32_t event;
+    uint32_t cnt[1];
+  } sh;
+  grid_release();
+  const int64_t seq = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int64_t R = a.n_rows;
   const int64_t lo = min(max((int64_t)a.offsets[seq], (int64_t)0), R);
   const int64_t hi = min(max((int64_t)a.offsets[seq + 1], lo), R);
-  if (lo >= hi) {  // a sequence without rows (the whole cluster leaves)
-    if (rank == 0 && tid == 0) {
-      a.out_accepted[seq] = 0;
-      if (a.out_status) a.out_status[seq] = PB_ROW_BAD_PARAMS;
-    }
-    return;
-  }
   const pb_row_params p = a.params[seq];
   const bool greedy = p.temperature == 0.0;
   const float tf = (float)p.temperature;
   const Scale scaled(tf);
+  grid_wait();  // the rows' records
+  if (lo >= hi) {  // a sequence without rows
+    if (tid == 0) {
+      a.out_accepted[seq] = 0;
+      if (a.out_status) a.out_status[seq] = PB_ROW_BAD_PARAMS;
+      a.decision[seq] = Decision{0, EV_BAD, 0};
+    }
+    return;
+  }
 
-  // Every CTA of the cluster finds the first row that is not accepted, by the same steps.
+  // the first row that is not accepted
   int64_t from = lo, stop = hi - 1;
   int32_t kind = EV_LAST;
   while (true) {
-    if (tid == 0) {
-      sh.event = 0x7FFFFFFF;
-      sh.kind = EV_LAST;
-    }
+    if (tid == 0) sh.event = 0x7FFFFFFF;
     __syncthreads();
     for (int64_t r = from + tid; r < hi; r += VT) {
       const pb_row_info f = a.info[r];
@@ -279,13 +382,25 @@ __global__ void __launch_bounds__(VT, 2) pick_kernel(VerifyArgs a) {
     if (tid == 0) sh.cnt[0] = 0;
     __syncthreads();
     uint32_t before = 0;
-    for (int32_t v = tid; v < rv.nvec && rv.first(v) < x; v += VT) {
-      float y[EPV];
-      Elem<T>::unpack(load_vec(rv, v), y);
+    const float lo_raw = surely_below(f.thr_key, tf);
+    for (int32_t v0 = tid; v0 < rv.nvec && rv.first(v0) < x; v0 += VT * SEG_V) {
+      uint4 q4[SEG_V];
 #pragma unroll
-      for (int q = 0; q < EPV; ++q) {
-        const int32_t i = rv.first(v) + q;
-        if (i >= 0 && i < x && key_of(scaled(y[q])) == f.thr_key) ++before;
+      for (int u = 0; u < SEG_V; ++u) {
+        const uint32_t none = Elem<T>::NEG_INF_WORD;
+        q4[u] = make_uint4(none, none, none, none);
+        if (v0 + u * VT < rv.nvec && rv.first(v0 + u * VT) < x) q4[u] = load_vec(rv, v0 + u * VT);
+      }
+#pragma unroll
+      for (int u = 0; u < SEG_V; ++u) {
+        if (!(vec_max_nan<T>(q4[u]) >= lo_raw)) continue;
+        float y[EPV];
+        Elem<T>::unpack(q4[u], y);
+#pragma unroll
+        for (int q = 0; q < EPV; ++q) {
+          const int32_t i = rv.first(v0 + u * VT) + q;
+          if (i >= 0 && i < x && key_of(scaled(y[q])) == f.thr_key) ++before;
+        }
       }
     }
     before = __reduce_add_sync(0xFFFFFFFFu, before);
@@ -302,250 +417,353 @@ __global__ void __launch_bounds__(VT, 2) pick_kernel(VerifyArgs a) {
   const double u_draw = a.uniforms[hi - 1];
   if (kind == EV_REJECT && !greedy && !(u_draw >= 0.0 && u_draw < 1.0)) kind = EV_BAD;
 
-  if (rank == 0) {
-    for (int64_t r = lo + tid; r < stop; r += VT) a.out_tokens[r] = a.drafts[r];
-    if (tid == 0) {
-      a.out_accepted[seq] = (int32_t)(stop - lo);
-      int32_t st = PB_ROW_OK;
-      if (kind == EV_BAD) st = a.info[stop].status != PB_ROW_OK ? a.info[stop].status : PB_ROW_BAD_UNIFORM;
-      if (a.out_status) a.out_status[seq] = st;
-      if (greedy && kind != EV_BAD) a.out_tokens[stop] = a.tok[stop];
-    }
+  for (int64_t r = lo + tid; r < stop; r += VT) a.out_tokens[r] = a.drafts[r];
+  if (tid == 0) {
+    a.out_accepted[seq] = (int32_t)(stop - lo);
+    int32_t st = PB_ROW_OK;
+    if (kind == EV_BAD) st = a.info[stop].status != PB_ROW_OK ? a.info[stop].status : PB_ROW_BAD_UNIFORM;
+    if (a.out_status) a.out_status[seq] = st;
+    if (greedy && kind != EV_BAD) a.out_tokens[stop] = a.tok[stop];
+    a.decision[seq] = Decision{stop, kind, !greedy && kind != EV_BAD};
   }
-  if (greedy || kind == EV_BAD) return;
+}
 
-  // ---- the last token: a draw over row `stop` in index order ----
-  const pb_row_info f = a.info[stop];
-  const float m = f.max_key;
-  const uint32_t thr = f.thr_key;
-  const double zd = __ull2double_rn(f.kept_q);
-  const bool residual = kind == EV_REJECT;
-  const int64_t dx = residual ? a.drafts[stop] : -1;
-  const int64_t drow = stop - seq;
-  const bool dist = residual && a.probs && drow >= 0 && drow < a.n_probs;
-  const bool cut_ties = f.kept_q != f.z_q;
-  // raw values below this are surely below the last kept key (two roundings of the quotient apart)
-  float raw_lo = -INFINITY;
-  if (thr > KEY_NEG_INF && thr < KEY_POS_INF) {
-    const float b = value_of(thr) * tf;
-    raw_lo = b - fabsf(b) * 0x1p-20f - 0x1p-100f;
-    if (!(raw_lo > -INFINITY)) raw_lo = -INFINITY;
+// ---- drawing ---------------------------------------------------------------------------------
+
+// The row a sequence draws its last token from, and the weights of its elements.
+template <typename T>
+struct DrawRow {
+  static constexpr int EPV = Elem<T>::EPV;
+  const VerifyArgs& a;
+  RowView<T> rv;
+  pb_row_info f;
+  Scale scaled;
+  Weigher weigh;
+  double z;          // mass, in the weights' own scale
+  float d_most;      // draft probabilities above this take all of any weight
+  int64_t dx, drow;  // the rejected draft; its row of draft_probs
+  bool residual, dist, cut_ties, whole;
+  float raw_lo;
+  __device__ DrawRow(const VerifyArgs& a_, int64_t seq, const Decision& d, float tf, const pb_row_info& f_)
+      : a(a_), rv(static_cast<const T*>(a_.x) + d.row * a_.row_stride, a_.V), f(f_), scaled(tf),
+        weigh(tf, f_.max_key, f_.max_key * tf) {
+    residual = d.kind == EV_REJECT;
+    dx = residual ? a.drafts[d.row] : -1;
+    drow = d.row - seq;
+    dist = residual && a.probs && drow >= 0 && drow < a.n_probs;
+    cut_ties = f.kept_q != f.z_q;
+    whole = f.thr_key == 0;
+    raw_lo = surely_below(f.thr_key, tf);
+    z = __ull2double_rn(f.kept_q) * 0x1p-40;
+    d_most = (float)(2048.0 / z);
   }
-  const RowView<T> rv(static_cast<const T*>(a.x) + stop * a.row_stride, a.V);
-  const int gw = rank * VNW + warp, GW = C * VNW;
-  const int32_t v0 = (int32_t)((int64_t)rv.nvec * gw / GW), v1 = (int32_t)((int64_t)rv.nvec * (gw + 1) / GW);
-  // the warp's share in parts of `step` vectors (a multiple of 32), at most VSTEPS of them
-  const int32_t step = (((v1 - v0) + VSTEPS - 1) / VSTEPS + 31) & ~31;
-
-  // equals of the last kept key before this warp's share, where top-p cut among them
-  uint32_t tie_base = 0;
-  if (cut_ties) {
-    uint32_t c = 0;
-    for (int32_t v = v0 + lane; v < v1; v += 32) {
-      const uint4 q4 = load_vec(rv, v);
-      if (!(vec_max_nan<T>(q4) >= raw_lo)) continue;
-      float y[EPV];
-      Elem<T>::unpack(q4, y);
+  // Weights of vector v (elements q4): target, or what the draft's distribution leaves of it, in the
+  // grid's scale. `eq` gets a bit per element whose key equals the last kept one, where top-p cut there.
+  __device__ __forceinline__ void of(int32_t v, uint4 q4, bool target, double* r, uint32_t& eq) const {
+    eq = 0;
+#pragma unroll
+    for (int q = 0; q < EPV; ++q) r[q] = 0.0;
+    if (!(vec_max_nan<T>(q4) >= raw_lo)) return;
+    const int32_t e0 = rv.first(v);
+    float w[EPV];
+    uint32_t some = 0;  // elements of weight
+    if (whole) {
+      weigh.template of<T>(q4, w);
+      some = (1u << EPV) - 1u;
+      if (!rv.whole(v)) {
+#pragma unroll
+        for (int q = 0; q < EPV; ++q)
+          if (e0 + q < 0 || e0 + q >= a.V) some &= ~(1u << q);
+      }
+    } else {
+      float x[EPV];
+      Elem<T>::unpack(q4, x);
 #pragma unroll
       for (int q = 0; q < EPV; ++q) {
-        const int32_t i = rv.first(v) + q;
-        if (i >= 0 && i < a.V && key_of(scaled(y[q])) == thr) ++c;
+        w[q] = 0.0f;
+        if (!(x[q] >= raw_lo) || e0 + q < 0 || e0 + q >= a.V) continue;
+        const float y = scaled(x[q]);
+        const uint32_t key = key_of(y);
+        if (key < f.thr_key) continue;
+        w[q] = exp_weight(__fsub_rn(y, f.max_key));
+        some |= 1u << q;
+        if (cut_ties && key == f.thr_key) eq |= 1u << q;
       }
     }
-    c = __reduce_add_sync(0xFFFFFFFFu, c);
-    if (lane == 0) sh.wtie[warp] = c;
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t s = 0;
-      for (int w = 0; w < VNW; ++w) s += sh.wtie[w];
-      sh.ctie = s;
-    }
-    cluster_barrier(C);
-    for (int r = 0; r < rank; ++r) tie_base += cluster.map_shared_rank(&sh, r)->ctie;
-    for (int w = 0; w < warp; ++w) tie_base += sh.wtie[w];
-  }
-
-  // the weights of vector v (all lanes of the warp call together, lanes side by side): target and
-  // residual; `ties` counts the equals before it
-  auto weigh = [&](int32_t v, bool in, uint32_t& ties, uint64_t* P, uint64_t* r) {
+    if (!some) return;
+    float d[EPV];
+    if (dist && !target) {
+      const bool f32 = a.probs_dtype == PB_DTYPE_F32;
+      const float* row32 = static_cast<const float*>(a.probs) + drow * a.probs_stride + e0;
+      if (whole && f32 && some == (1u << EPV) - 1u && (reinterpret_cast<uintptr_t>(row32) & 15) == 0) {
 #pragma unroll
-    for (int q = 0; q < EPV; ++q) P[q] = r[q] = 0;
-    uint4 q4 = make_uint4(0u, 0u, 0u, 0u);
-    if (in) {
-      q4 = load_vec(rv, v);
-      in = vec_max_nan<T>(q4) >= raw_lo;
-    }
-    uint32_t eq = 0;  // a bit per element equal to the last kept key
-    float y[EPV];
-    if (in) {
-      Elem<T>::unpack(q4, y);
-#pragma unroll
-      for (int q = 0; q < EPV; ++q) {
-        const int32_t i = rv.first(v) + q;
-        y[q] = scaled(y[q]);
-        const uint32_t key = key_of(y[q]);
-        if (i >= 0 && i < a.V) {
-          if (key >= thr) P[q] = weight_q(y[q], m);
-          if (key == thr) eq |= 1u << q;
+        for (int q = 0; q < EPV; q += 4) {
+          const float4 p4 = __ldg(reinterpret_cast<const float4*>(row32 + q));
+          d[q] = p4.x;
+          d[q + 1] = p4.y;
+          d[q + 2] = p4.z;
+          d[q + 3] = p4.w;
         }
+      } else {
+#pragma unroll
+        for (int q = 0; q < EPV; ++q) d[q] = ((some >> q) & 1u) ? prob_at(a, drow, e0 + q) : 0.0f;
       }
     }
-    if (cut_ties && __any_sync(0xFFFFFFFFu, eq != 0)) {
-      const uint32_t mine = (uint32_t)__popc(eq), incl = warp_incl_scan(mine);
-      uint32_t at = ties + incl - mine;
+#pragma unroll
+    for (int q = 0; q < EPV; ++q) {
+      const double p = on_grid(w[q]);
+      double taken = GRID;
+      if (!target) {
+        // floor(d * Z): NaN and what is below 0 take nothing
+        if (dist) taken = __dadd_rd(GRID, __dmul_rn((double)fminf(fmaxf(d[q], 0.0f), d_most), z));
+        else if (residual && e0 + q == dx) taken = p;
+      }
+      if ((some >> q) & 1u) r[q] = fmax(p - taken, 0.0);
+    }
+  }
+};
+
+__device__ __forceinline__ uint64_t units(double sum) { return (uint64_t)(sum * 0x1p40); }  // (exact)
+
+// CTA (sequence, segment): the sums of the segment's tiles.
+template <typename T>
+__global__ void __launch_bounds__(VT, 4) weigh_kernel(VerifyArgs a) {
+  constexpr int EPV = Elem<T>::EPV;
+  __shared__ uint64_t w[VNW][TILES], tw[VNW][TILES];
+  __shared__ int32_t tn[VNW][TILES];
+  grid_release();
+  grid_wait();
+  const int64_t seq = blockIdx.x;
+  const Decision d = a.decision[seq];
+  if (!d.draws) return;
+  const pb_row_info f = a.info[d.row];
+  const DrawRow<T> row(a, seq, d, (float)a.params[seq].temperature, f);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(row.rv.nvec, v0 + a.seg.per);
+  uint4 q[SEG_V];
+  load_segment(row.rv, v0, v1, q);
+#pragma unroll 1
+  for (int i = 0; i < SEG_V; ++i) {
+    if (i * SEG_T >= v1 - v0) {
+      if (lane == 0) w[warp][i] = tw[warp][i] = 0, tn[warp][i] = 0;
+      continue;
+    }
+    uint4 qi = q[0];  // q[i], kept in registers
+#pragma unroll
+    for (int j = 1; j < SEG_V; ++j)
+      if (j == i) qi = q[j];
+    double r[EPV], sum = 0.0, tsum = 0.0;
+    uint32_t eq;
+    row.of(v0 + i * SEG_T + (int32_t)threadIdx.x, qi, false, r, eq);
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) {
+      if ((eq >> j) & 1u) tsum += r[j];
+      else sum += r[j];
+    }
+    uint64_t s = warp_sum(units(sum)), t = 0;
+    int32_t n = 0;
+    if (row.cut_ties) {
+      t = warp_sum(units(tsum));
+      n = __reduce_add_sync(0xFFFFFFFFu, __popc(eq));
+    }
+    if (lane == 0) {
+      w[warp][i] = s;
+      tw[warp][i] = t;
+      tn[warp][i] = n;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < TILES) {
+    Tile t{0, 0, 0, 0};
+    for (int k = 0; k < VNW; ++k) {
+      t.w += w[k][threadIdx.x];
+      t.tie_w += tw[k][threadIdx.x];
+      t.ties += tn[k][threadIdx.x];
+    }
+    a.tiles[(seq * a.seg.segs + blockIdx.y) * TILES + threadIdx.x] = t;
+  }
+}
+
+struct DrawShared {
+  uint64_t scan[VNW + 1];
+  uint32_t tscan[VNW + 1];
+  uint64_t total, left;
+  int32_t tile;      // the draw's tile
+  uint32_t before;   // equals of the last kept key before it
+  int32_t cut;       // the tile in which the kept equals end
+  uint32_t cut_before;
+  int32_t found;
+};
+
+// The draw: one CTA per sequence. Tiles are in index order, so is a tile's vectors over the threads.
+template <typename T>
+__global__ void __launch_bounds__(VT, 2) draw_kernel(VerifyArgs a) {
+  constexpr int EPV = Elem<T>::EPV;
+  __shared__ DrawShared sh;
+  grid_wait();
+  const int64_t seq = blockIdx.x;
+  const Decision d = a.decision[seq];
+  if (!d.draws) return;
+  const int tid = threadIdx.x;
+  const pb_row_info f = a.info[d.row];
+  const DrawRow<T> row(a, seq, d, (float)a.params[seq].temperature, f);
+  const int32_t nt = a.seg.segs * TILES;
+  const Tile* tiles = a.tiles + seq * nt;
+  const uint32_t keep = (uint32_t)f.n_tie_kept;
+  const int64_t last = min((int64_t)a.offsets[seq + 1], a.n_rows) - 1;
+  const uint64_t u53 = (uint64_t)(a.uniforms[last] * 0x1p53);
+
+  // this thread's vector of tile k, its weights (those equals that were cut have none), and their sum;
+  // `before`: equals before the tile
+  auto tile_weights = [&](int32_t k, bool target, uint32_t before, double* r) -> uint64_t {
+    const int32_t v0 = (k / TILES) * a.seg.per, v1 = min(row.rv.nvec, v0 + a.seg.per);
+    const int32_t v = v0 + (k % TILES) * SEG_T + tid;
+    uint32_t eq = 0;
+#pragma unroll
+    for (int q = 0; q < EPV; ++q) r[q] = 0.0;
+    if (v < v1) row.of(v, load_vec(row.rv, v), target, r, eq);
+    if (row.cut_ties) {
+      uint32_t total;
+      uint32_t at = before + block_excl_scan<uint32_t, VT>((uint32_t)__popc(eq), sh.tscan, &total);
 #pragma unroll
       for (int q = 0; q < EPV; ++q)
         if ((eq >> q) & 1u) {
-          if (at >= (uint32_t)f.n_tie_kept) P[q] = 0;
+          if (at >= keep) r[q] = 0.0;
           ++at;
         }
-      ties += __shfl_sync(0xFFFFFFFFu, incl, 31);
     }
-    if (in) {
+    double s = 0.0;
 #pragma unroll
-      for (int q = 0; q < EPV; ++q) {
-        const int64_t i = rv.first(v) + q;
-        if (P[q]) {
-          uint64_t t = 0;
-          if (dist) t = taken_of(prob_at(a, drow, i), zd);
-          else if (residual && i == dx) t = P[q];
-          r[q] = (P[q] > t) ? P[q] - t : 0;
-        }
-      }
-    }
+    for (int q = 0; q < EPV; ++q) s += r[q];
+    return units(s);
   };
-
-  uint64_t sum_r = 0, sum_p = 0;
-  uint32_t ties = tie_base;
-  for (int s = 0; s < VSTEPS; ++s) {
-    uint64_t sr = 0, sp = 0;
-    const int32_t vs = v0 + s * step;
-    if (vs < v1) {
-      for (int32_t vb = vs; vb < min(vs + step, v1); vb += 32) {
-        uint64_t P[EPV], r[EPV];
-        weigh(vb + lane, vb + lane < v1, ties, P, r);
-#pragma unroll
-        for (int q = 0; q < EPV; ++q) {
-          sp += P[q];
-          sr += r[q];
-        }
-      }
-      sr = warp_sum(sr);
-      sp = warp_sum(sp);
-    }
-    if (lane == 0) {
-      sh.res[warp][s] = sr;
-      sh.all[warp][s] = sp;
-    }
-    sum_r += sr;
-    sum_p += sp;
+  // sum of tile k with the equals before it known: from its record, or where the kept equals end
+  // inside it, from sh.total (computed once below)
+  if (tid == 0) {
+    sh.tile = sh.cut = -1;
+    sh.found = -1;
+    sh.total = 0;
   }
-  if (lane == 0) {
-    sh.wres[warp] = sum_r;
-    sh.wall[warp] = sum_p;
-  }
-  cluster_barrier(C);
-  if (rank == 0 && tid == 0) {
-    uint64_t tr = 0, tp = 0;
-    for (int r = 0; r < C; ++r) {
-      const PickShared* o = C > 1 ? cluster.map_shared_rank(&sh, r) : &sh;
-      for (int w = 0; w < VNW; ++w) {
-        tr += o->wres[w];
-        tp += o->wall[w];
+  __syncthreads();
+  uint64_t cut_w = 0;  // weight of the tile in which the kept equals end
+  if (row.cut_ties) {
+    uint32_t base = 0;
+    for (int32_t k0 = 0; k0 < nt; k0 += VT) {
+      const uint32_t n = k0 + tid < nt ? (uint32_t)__ldcg(&tiles[k0 + tid].ties) : 0u;
+      uint32_t total;
+      const uint32_t at = base + block_excl_scan<uint32_t, VT>(n, sh.tscan, &total);
+      if (at < keep && at + n > keep) {
+        sh.cut = k0 + tid;
+        sh.cut_before = at;
       }
+      base += total;
     }
-    const int use_all = tr == 0;
-    uint64_t t = scale_u53((uint64_t)(u_draw * 0x1p53), use_all ? tp : tr);
-    int owner = -1;
-    for (int r = 0; r < C && owner < 0; ++r) {
-      const PickShared* o = C > 1 ? cluster.map_shared_rank(&sh, r) : &sh;
-      for (int w = 0; w < VNW; ++w) {
-        const uint64_t c = use_all ? o->wall[w] : o->wres[w];
-        if (t < c) {
-          owner = r * VNW + w;
-          break;
-        }
-        t -= c;
-      }
-    }
-    sh.owner = owner;
-    sh.use_all = use_all;
-    sh.left = t;
-    if (owner < 0) {  // no mass at all: the row's record and its weights disagree
-      if (a.out_status) a.out_status[seq] = PB_ROW_INTERNAL;
+    __syncthreads();
+    if (sh.cut >= 0) {
+      double r[EPV];
+      const uint64_t s = tile_weights(sh.cut, false, sh.cut_before, r);
+      block_excl_scan<uint64_t, VT>(s, sh.scan, &cut_w);
     }
   }
-  cluster_barrier(C);
-  const PickShared* d0 = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
-  const int owner = d0->owner;
-  const bool use_all = d0->use_all != 0;
-  uint64_t left = d0->left;
-  if (owner == gw) {
-    int s = 0;
-    for (; s < VSTEPS; ++s) {
-      const uint64_t c = use_all ? sh.all[warp][s] : sh.res[warp][s];
-      if (left < c) break;
-      left -= c;
-    }
-    // equals of the last kept key in the parts before
-    uint32_t before = tie_base;
-    if (cut_ties) {
-      uint32_t c = 0;
-      for (int32_t v = v0 + lane; v < min(v0 + s * step, v1); v += 32) {
-        float y[EPV];
-        Elem<T>::unpack(load_vec(rv, v), y);
-#pragma unroll
-        for (int q = 0; q < EPV; ++q) {
-          const int32_t i = rv.first(v) + q;
-          if (i >= 0 && i < a.V && key_of(scaled(y[q])) == thr) ++c;
+  const int32_t cut = sh.cut;
+  // over the tiles in order: the total, then the tile whose inclusive prefix first exceeds the target
+  auto walk = [&](bool find, uint64_t target) -> uint64_t {
+    uint64_t run = 0;
+    uint32_t base = 0;
+    for (int32_t k0 = 0; k0 < nt; k0 += VT) {
+      const int32_t k = k0 + tid;
+      uint64_t w = 0;
+      uint32_t n = 0, before = 0, total_n = 0;
+      Tile t{0, 0, 0, 0};
+      if (k < nt) {
+        t.w = __ldcg(&tiles[k].w);
+        if (row.cut_ties) {
+          t.tie_w = __ldcg(&tiles[k].tie_w);
+          t.ties = __ldcg(&tiles[k].ties);
         }
       }
-      before += __reduce_add_sync(0xFFFFFFFFu, c);
+      if (row.cut_ties) {
+        n = (uint32_t)t.ties;
+        before = base + block_excl_scan<uint32_t, VT>(n, sh.tscan, &total_n);
+        base += total_n;
+      }
+      w = (k == cut) ? cut_w : t.w + (before + n <= keep ? t.tie_w : 0ull);
+      uint64_t total;
+      const uint64_t at = run + block_excl_scan<uint64_t, VT>(w, sh.scan, &total);
+      if (find && at <= target && target < at + w) {
+        sh.tile = k;
+        sh.left = target - at;
+        sh.before = before;
+      }
+      run += total;
+      if (find && target < run) break;
     }
-    int64_t found = -1;
-    for (int32_t vb = v0 + s * step; vb < v1; vb += 32) {
-      uint64_t P[EPV], r[EPV], c = 0;
-      weigh(vb + lane, vb + lane < v1, before, P, r);
-#pragma unroll
-      for (int q = 0; q < EPV; ++q) c += use_all ? P[q] : r[q];
-      const uint64_t incl = warp_incl_scan(c), total = __shfl_sync(0xFFFFFFFFu, incl, 31);
-      const uint32_t hit = __ballot_sync(0xFFFFFFFFu, incl > left);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          uint64_t run = incl - c;
-#pragma unroll
-          for (int q = 0; q < EPV; ++q) {
-            run += use_all ? P[q] : r[q];
-            if (found < 0 && run > left) found = rv.first(vb + lane) + q;
-          }
-          a.out_tokens[stop] = found;
+    __syncthreads();
+    return run;
+  };
+  uint64_t total = walk(false, 0);
+  const bool target = total == 0;  // an empty residual: drawn from the target itself
+  if (!target) {
+    walk(true, scale_u53(u53, total));
+  } else {
+    // (rare: tile by tile, the target's weights anew)
+    const uint64_t want = scale_u53(u53, f.kept_q);
+    uint64_t run = 0;
+    uint32_t before = 0;
+    for (int32_t k = 0; k < nt; ++k) {
+      double r[EPV];
+      uint64_t w;
+      block_excl_scan<uint64_t, VT>(tile_weights(k, true, before, r), sh.scan, &w);
+      if (want < run + w) {
+        if (tid == 0) {
+          sh.tile = k;
+          sh.left = want - run;
+          sh.before = before;
         }
         break;
       }
-      left -= total;
+      run += w;
+      if (row.cut_ties) before += (uint32_t)__ldcg(&tiles[k].ties);
     }
+    __syncthreads();
   }
-  if (C > 1) cluster.sync();  // rank 0's decision stays until every CTA has read it
-}
-
-int verify_cluster(int64_t n, int64_t bytes) {
-  const int64_t want = 2 * (int64_t)device_sms();
-  int C = 1;
-  while (C < 8 && n * C < want && bytes / (2 * C) >= 8192) C <<= 1;
-  return C;
+  const int32_t tile = sh.tile;
+  if (tile < 0) {  // no mass at all: the row's record and its weights disagree
+    if (tid == 0 && a.out_status) a.out_status[seq] = PB_ROW_INTERNAL;
+    return;
+  }
+  double r[EPV];
+  const uint64_t s = tile_weights(tile, target, sh.before, r);
+  uint64_t whole;
+  uint64_t run = block_excl_scan<uint64_t, VT>(s, sh.scan, &whole);
+  const uint64_t left = sh.left;
+  if (run <= left && left < run + s) {
+    const int32_t v0 = (tile / TILES) * a.seg.per, v = v0 + (tile % TILES) * SEG_T + tid;
+    int32_t found = -1;
+#pragma unroll
+    for (int q = 0; q < EPV; ++q) {
+      run += units(r[q]);
+      if (found < 0 && run > left) found = row.rv.first(v) + q;
+    }
+    a.out_tokens[d.row] = found;
+  }
 }
 
 constexpr int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 struct VerifyPlan {
-  int64_t rowp, info, tok, sampler, bytes;  // offsets in the workspace, and its size
+  int64_t rowp, info, tok, meta, decision, tiles, sampler, bytes;  // offsets in the workspace, and its size
 };
-VerifyPlan verify_plan(int64_t n_rows, int64_t vocab, int dtype) {
+VerifyPlan verify_plan(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype) {
+  const SegPlan seg = seg_plan(vocab, elem_size(dtype), nullptr, 1);  // (rows of any alignment: the most segments)
   VerifyPlan v;
   v.rowp = 0;
   v.info = up256(n_rows * (int64_t)sizeof(pb_row_params));
   v.tok = v.info + up256(n_rows * (int64_t)sizeof(pb_row_info));
-  v.sampler = v.tok + up256(n_rows * 8);
+  v.meta = v.tok + up256(n_rows * 8);
+  v.decision = v.meta + up256(n_rows * (int64_t)sizeof(RowMeta));
+  v.tiles = v.decision + up256(n_seqs * (int64_t)sizeof(Decision));
+  v.sampler = v.tiles + up256(n_seqs * seg.segs * TILES * (int64_t)sizeof(Tile));
   v.bytes = v.sampler + pb_sample_ws_bytes(n_rows, vocab, dtype);
   return v;
 }
@@ -555,12 +773,17 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
   a.rowp = reinterpret_cast<pb_row_params*>(ws + plan.rowp);
   a.info = reinterpret_cast<pb_row_info*>(ws + plan.info);
   a.tok = reinterpret_cast<int64_t*>(ws + plan.tok);
-  a.sampler_runs = (kinds & (PB_VERIFY_SMALL | PB_VERIFY_OTHER)) != 0;
+  a.meta = reinterpret_cast<RowMeta*>(ws + plan.meta);
+  a.decision = reinterpret_cast<Decision*>(ws + plan.decision);
+  a.tiles = reinterpret_cast<Tile*>(ws + plan.tiles);
+  a.seg = seg_plan(a.V, sizeof(T), a.x, a.row_stride);
+  const bool sampler = (kinds & (PB_VERIFY_SMALL | PB_VERIFY_OTHER)) != 0;
   a.mass_runs = (kinds & PB_VERIFY_WHOLE) != 0;
+  a.all_whole = kinds == PB_VERIFY_WHOLE;
   expand_kernel<<<(unsigned)((a.n_rows + 255) / 256), 256, 0, st>>>(a);
   if (cudaGetLastError() != cudaSuccess) return PB_E_LAUNCH;
   int rc = PB_OK;
-  if (a.sampler_runs) {
+  if (sampler) {
     // rows that pb_sample_ws's two passes settle themselves go through it, a batch with others
     // through pb_sample (the same choice as for sampling)
     if (!(kinds & PB_VERIFY_OTHER))
@@ -570,22 +793,25 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
       rc = pb_sample(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr, st);
     if (rc != PB_OK) return rc;
   }
+  const dim3 rows((unsigned)a.n_rows, (unsigned)a.seg.segs), seqs((unsigned)a.n_seqs), parts((unsigned)a.n_seqs, (unsigned)a.seg.segs);
   if (a.mass_runs) {
-    const int C = verify_cluster(a.n_rows, (int64_t)a.V * sizeof(T));
-    rc = launch_cluster(mass_kernel<T>, a, a.n_rows * C, VT, C, 0, st);
+    rc = launch_after(max_kernel<T>, a, rows, VT, st);
+    if (rc == PB_OK) rc = launch_after(mass_kernel<T>, a, rows, VT, st);
     if (rc != PB_OK) return rc;
   }
-  const int C = verify_cluster(a.n_seqs, (int64_t)a.V * sizeof(T));
-  return launch_cluster(pick_kernel<T>, a, a.n_seqs * C, VT, C, 0, st);
+  rc = launch_after(decide_kernel<T>, a, seqs, VT, st);
+  if (rc == PB_OK) rc = launch_after(weigh_kernel<T>, a, parts, VT, st);
+  if (rc == PB_OK) rc = launch_after(draw_kernel<T>, a, seqs, VT, st);
+  return rc;
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t pb_verify_ws_bytes(int64_t n_rows, int64_t vocab, int dtype) {
-  if (n_rows < 0 || vocab <= 0 || !elem_size(dtype)) return PB_E_INVALID;
-  return verify_plan(n_rows, vocab, dtype).bytes;
+int64_t pb_verify_ws_bytes(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype) {
+  if (n_rows < 0 || n_seqs < 0 || vocab <= 0 || !elem_size(dtype)) return PB_E_INVALID;
+  return verify_plan(n_rows, n_seqs, vocab, dtype).bytes;
 }
 
 int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
@@ -607,7 +833,7 @@ int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int6
     if (!ps || probs_stride < vocab || reinterpret_cast<uintptr_t>(draft_probs) % ps) return PB_E_INVALID;
   }
   if (kinds < 0 || kinds > PB_VERIFY_ANY) return PB_E_INVALID;
-  const VerifyPlan plan = verify_plan(n_rows, vocab, dtype);
+  const VerifyPlan plan = verify_plan(n_rows, n_seqs, vocab, dtype);
   if ((reinterpret_cast<uintptr_t>(workspace) & 255) || ws_bytes < plan.bytes) return PB_E_INVALID;
   VerifyArgs a = {};
   a.x = logits;

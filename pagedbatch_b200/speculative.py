@@ -70,7 +70,7 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs):
     with ops.on_device(dev):
         # a buffer of this call's own: the allocator hands it on in stream order, and a captured
         # graph keeps its copy
-        ws = torch.empty(L.pb_verify_ws_bytes(R, V, code), dtype=torch.uint8, device=dev)
+        ws = torch.empty(L.pb_verify_ws_bytes(R, S, V, code), dtype=torch.uint8, device=dev)
         rc = L.pb_verify(
             logits.data_ptr(), code, R, V, logits.stride(0) if R > 1 else V, params.data_ptr(), S,
             row_offsets.data_ptr(), drafts.data_ptr(), uniforms.data_ptr(),

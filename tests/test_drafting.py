@@ -96,7 +96,7 @@ def test_c_abi_refusals(lib):
     def verify(**kw):
         a = dict(logits=base, dtype=0, n_rows=2, vocab=8, stride=8, params=base, n_seqs=1, offsets=base, drafts=base,
                  uniforms=base, probs=None, pdtype=0, n_probs=1, pstride=8, kinds=0, tokens=base, accepted=base, status=None,
-                 ws=base, ws_bytes=lib.pb_verify_ws_bytes(2, 8, 0), stream=None) | kw
+                 ws=base, ws_bytes=lib.pb_verify_ws_bytes(2, 1, 8, 0), stream=None) | kw
         return lib.pb_verify(*a.values())
 
     for kw in (dict(dtype=9), dict(n_rows=-1), dict(vocab=0), dict(stride=7), dict(logits=None), dict(params=None),
@@ -107,7 +107,7 @@ def test_c_abi_refusals(lib):
         assert verify(**kw) == -1, kw
     assert verify(vocab=1 << 24, stride=1 << 24) == -2
     assert verify(n_rows=0, n_seqs=0) == 0
-    assert lib.pb_verify_ws_bytes(-1, 8, 0) == -1 and lib.pb_verify_ws_bytes(1, 8, 7) == -1
+    assert lib.pb_verify_ws_bytes(-1, 1, 8, 0) == -1 and lib.pb_verify_ws_bytes(1, 1, 8, 7) == -1
 
     def top(**kw):
         a = dict(logits=base, dtype=0, n_rows=2, vocab=8, stride=8, k=2, t=1.0, lp=base, idx=base, lse=base, ws=base, ws_bytes=1 << 20, stream=None) | kw
