@@ -33,6 +33,7 @@
 #include "../../include/pagedbatch_b200.h"
 #include "pb_device.cuh"
 #include "pb_elem.cuh"
+#include "pb_internal.h"
 
 namespace cg = cooperative_groups;
 using namespace pb;
@@ -2650,6 +2651,23 @@ int run_rows_dtype(const Args& a, int dtype, int es, cudaStream_t st) {
   return run_rows<__half>(a, es, st);
 }
 }  // namespace
+
+namespace pb {
+
+GroupKeys sample_ws_keys(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                         const void* workspace, int64_t ws_bytes) {
+  GroupKeys g = {nullptr, 0, 0, 0};
+  const int es = (dtype == PB_DTYPE_F32) ? 4 : 2;
+  const GroupPlan p = group_plan(n_rows, vocab, es);
+  if (!groups_eligible(logits, row_stride, es, n_rows, vocab) || ws_bytes < p.bytes) return g;
+  g.keys = static_cast<const uint32_t*>(workspace);
+  g.stride = (int32_t)p.ngs;
+  g.groups = (int32_t)p.ngr;
+  g.elems = GM_GB / es;
+  return g;
+}
+
+}  // namespace pb
 
 extern "C" {
 

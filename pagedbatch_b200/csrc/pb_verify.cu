@@ -23,6 +23,7 @@
 //   5. draw_kernel: a CTA per sequence finds the draw's tile and its element.
 // Weights are exact integers throughout (multiples of 2^-40 below 2^13, which fp64 adds without
 // rounding), so no result depends on an order of addition.
+#include "pb_internal.h"
 #include "pb_rows.cuh"
 
 using namespace pb;
@@ -75,6 +76,7 @@ struct VerifyArgs {
   Decision* decision;            // workspace: [n_seqs]
   Tile* tiles;                   // workspace: [n_seqs][segs][TILES]
   SegPlan seg;
+  GroupKeys groups;              // of the rows the sampler settled (keys null: none)
   int32_t all_whole;
   int64_t* out_tokens;           // [n_rows]
   int32_t* out_accepted;         // [n_seqs]
@@ -134,24 +136,28 @@ struct Scale {
 //    exact in one fused operation each, give RN(x / T) while nothing over- or underflows;
 //  * keys further than 40 below the maximum, whose weight is below 2^-40, are taken as 40 below it.
 struct Weigher {
-  float t, y, inv, m;
+  float t, recip, inv, m;
   bool fast;  // the row's values are ordinary enough for the packed steps
   __device__ Weigher(float t_, float m_, float raw_max) : t(t_), m(m_) {
     const Scale s(t_);
     inv = s.inv;
-    y = __frcp_rn(t_);
+    recip = __frcp_rn(t_);
     const float a = fabsf(raw_max);
     fast = a >= 0x1p-40f && a <= 0x1p60f && t_ >= 0x1p-40f && t_ <= 0x1p40f;
   }
+  // weights w and scaled values y of a vector's elements
   template <typename T>
-  __device__ __forceinline__ void of(uint4 v, float* w) const {
+  __device__ __forceinline__ void of(uint4 v, float* w, float* y) const {
     constexpr int EPV = Elem<T>::EPV;
     float x[EPV];
     Elem<T>::unpack(v, x);
     if (!fast) {
       const Scale s(t);
 #pragma unroll
-      for (int q = 0; q < EPV; ++q) w[q] = exp_weight(__fsub_rn(s(x[q]), m));
+      for (int q = 0; q < EPV; ++q) {
+        y[q] = s(x[q]);
+        w[q] = exp_weight(__fsub_rn(y[q], m));
+      }
       return;
     }
     const uint64_t m2 = pack2(-m, -m);
@@ -162,11 +168,12 @@ struct Weigher {
         k = mul2(pack2(x[q], x[q + 1]), pack2(inv, inv));
       } else {
         // (values below -2^100 have no weight: taken as that, so that -inf divides)
-        const uint64_t x2 = pack2(fmaxf(x[q], -0x1p100f), fmaxf(x[q + 1], -0x1p100f)), y2 = pack2(y, y), t2 = pack2(-t, -t);
+        const uint64_t x2 = pack2(fmaxf(x[q], -0x1p100f), fmaxf(x[q + 1], -0x1p100f)), y2 = pack2(recip, recip), t2 = pack2(-t, -t);
         k = mul2(x2, y2);
         k = fma2(fma2(k, t2, x2), y2, k);
         k = fma2(fma2(k, t2, x2), y2, k);
       }
+      unpack2(k, y[q], y[q + 1]);
       float d0, d1;
       unpack2(add2(k, m2), d0, d1);
       const uint64_t d = pack2(fmaxf(d0, -40.0f), fmaxf(d1, -40.0f));
@@ -225,8 +232,8 @@ __global__ void __launch_bounds__(VT, SEG_CTAS) max_kernel(VerifyArgs a) {
   }
 }
 
-// Mass of every whole row: the sum of its weights. Rows are taken from the last one back, since the
-// last ones that max_kernel read are still in L2.
+// Mass of every whole row: the sum of its weights. CTAs take the rows and segments in max_kernel's order
+// backwards, since what that read last is still in L2.
 template <typename T>
 __global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
@@ -234,7 +241,7 @@ __global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
   grid_release();
   const int64_t row = a.n_rows - 1 - blockIdx.x;
   const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
-  const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+  const int32_t v0 = (int32_t)(gridDim.y - 1 - blockIdx.y) * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
   uint4 q[SEG_V];
   if (a.all_whole) load_segment(rv, v0, v1, q);
   grid_wait();  // the rows' largest values
@@ -259,8 +266,8 @@ __global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
 #pragma unroll
   for (int i = 0; i < SEG_V; ++i) {
     if (i * SEG_T >= v1 - v0) break;
-    float w[EPV];
-    weigh.template of<T>(q[i], w);  // elements outside the row are -inf: no weight
+    float w[EPV], y[EPV];
+    weigh.template of<T>(q[i], w, y);  // elements outside the row are -inf: no weight
 #pragma unroll
     for (int j = 0; j < EPV; j += 2) {
       s0 = __dadd_rd(s0, (double)w[j]);
@@ -297,13 +304,329 @@ __device__ __forceinline__ float surely_below(uint32_t thr, float tf) {
   return (r > -INFINITY) ? r : -INFINITY;
 }
 
+// The row a sequence draws its last token from, and the weights of its elements.
 template <typename T>
-__global__ void __launch_bounds__(VT, 4) decide_kernel(VerifyArgs a) {
+struct DrawRow {
+  static constexpr int EPV = Elem<T>::EPV;
+  const VerifyArgs& a;
+  RowView<T> rv;
+  pb_row_info f;
+  Scale scaled;
+  Weigher weigh;
+  double z;          // mass, in the weights' own scale
+  float d_most;      // draft probabilities above this take all of any weight
+  int64_t dx, drow;  // the rejected draft; its row of draft_probs
+  bool residual, dist, cut_ties, whole;
+  float raw_lo, thr;  // (a key's order is its value's: the row holds no NaN)
+  __device__ DrawRow(const VerifyArgs& a_, int64_t seq, const Decision& d, float tf, const pb_row_info& f_)
+      : a(a_), rv(static_cast<const T*>(a_.x) + d.row * a_.row_stride, a_.V), f(f_), scaled(tf),
+        weigh(tf, f_.max_key, f_.max_key * tf) {
+    residual = d.kind == EV_REJECT;
+    dx = residual ? a.drafts[d.row] : -1;
+    drow = d.row - seq;
+    dist = residual && a.probs && drow >= 0 && drow < a.n_probs;
+    cut_ties = f.kept_q != f.z_q;
+    whole = f.thr_key == 0;
+    raw_lo = surely_below(f.thr_key, tf);
+    thr = value_of(f.thr_key);
+    z = __ull2double_rn(f.kept_q) * 0x1p-40;
+    d_most = (float)(2048.0 / z);
+  }
+  // The draft's probabilities of a whole vector, where they can be loaded as vectors of their own.
+  __device__ __forceinline__ bool packed_probs(int32_t v) const {
+    return dist && a.probs_dtype == PB_DTYPE_F32 && rv.whole(v) &&
+           (reinterpret_cast<uintptr_t>(static_cast<const float*>(a.probs) + drow * a.probs_stride + rv.first(v)) & 15) == 0;
+  }
+  __device__ __forceinline__ void load_probs(int32_t v, float4* d) const {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.probs) + drow * a.probs_stride + rv.first(v));
+#pragma unroll
+    for (int q = 0; q < EPV / 4; ++q) d[q] = __ldg(p + q);
+  }
+  // GRID + floor(d * Z): NaN and what is below 0 take nothing
+  __device__ __forceinline__ double taken_by(float d) const {
+    return __dadd_rd(GRID, __dmul_rn((double)fminf(fmaxf(d, 0.0f), d_most), z));
+  }
+  // max(p - taken, 0), by the sign bit of the (exact) difference
+  static __device__ __forceinline__ double leaves(double p, double taken) {
+    const long long r = __double_as_longlong(p - taken);
+    return __longlong_as_double(r & ~(r >> 63));
+  }
+  // Weights of vector v (elements q4): target, or what the draft's distribution leaves of it, in the
+  // grid's scale. `eq` gets a bit per element whose key equals the last kept one, where top-p cut
+  // there. `have`: its draft probabilities are in d.
+  __device__ __forceinline__ void of(int32_t v, uint4 q4, bool target, bool have, const float4* d4, double* r,
+                                     uint32_t& eq) const {
+    eq = 0;
+#pragma unroll
+    for (int q = 0; q < EPV; ++q) r[q] = 0.0;
+    if (!(vec_max_nan<T>(q4) >= raw_lo)) return;
+    const int32_t e0 = rv.first(v);
+    float w[EPV], y[EPV];
+    weigh.template of<T>(q4, w, y);
+    uint32_t some = (1u << EPV) - 1u;  // elements of weight
+    if (!rv.whole(v)) {
+#pragma unroll
+      for (int q = 0; q < EPV; ++q)
+        if (e0 + q < 0 || e0 + q >= a.V) some &= ~(1u << q);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int q = 0; q < EPV; ++q) {
+        if (!(y[q] >= thr)) some &= ~(1u << q);
+        if (cut_ties && y[q] == thr) eq |= 1u << q;
+      }
+      eq &= some;
+    }
+    if (!some) return;
+    float d[EPV];
+    if (dist && !target) {
+      if (have) {
+#pragma unroll
+        for (int q = 0; q < EPV; q += 4) {
+          d[q] = d4[q / 4].x;
+          d[q + 1] = d4[q / 4].y;
+          d[q + 2] = d4[q / 4].z;
+          d[q + 3] = d4[q / 4].w;
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < EPV; ++q) d[q] = ((some >> q) & 1u) ? prob_at(a, drow, e0 + q) : 0.0f;
+      }
+    }
+    if (dist && !target && some == (1u << EPV) - 1u) {  // the common case, without selections
+#pragma unroll
+      for (int q = 0; q < EPV; ++q) r[q] = leaves(on_grid(w[q]), taken_by(d[q]));
+      return;
+    }
+#pragma unroll
+    for (int q = 0; q < EPV; ++q) {
+      const double p = on_grid(w[q]);
+      double taken = GRID;
+      if (!target) {
+        if (dist) taken = taken_by(d[q]);
+        else if (residual && e0 + q == dx) taken = p;
+      }
+      if ((some >> q) & 1u) r[q] = leaves(p, taken);
+    }
+  }
+};
+
+// A sum below 2^12 in units of 2^-40.
+__device__ __forceinline__ uint64_t units(double sum) { return grid_units(sum + GRID); }
+
+// Exclusive prefix over the block of one value per thread, and their sum.
+template <typename U>
+__device__ __forceinline__ U block_prefix(U v, U* scratch, U* total) {
+  return block_excl_scan<U, VT>(v, scratch, total);
+}
+
+// A thread's run of consecutive 128-byte groups of a row, looked through by their keys: f(v, vector)
+// for every vector, in index order, of the groups whose largest value may reach raw_lo.
+template <typename T, typename F>
+__device__ __forceinline__ void each_near(const GroupKeys& g, const RowView<T>& rv, int64_t row, float raw_lo, F&& f) {
+  constexpr int GV = 8;  // vectors of a group (such rows start on a 16-byte boundary)
+  const int32_t run = ((g.groups + VT - 1) / VT + 3) & ~3;
+  const int32_t g0 = (int32_t)threadIdx.x * run, g1 = min(g.groups, g0 + run);
+  const uint32_t lo = key_of(raw_lo);
+  const uint32_t* keys = g.keys + row * g.stride;
+  for (int32_t k0 = g0; k0 < g1; k0 += 16) {  // 16 keys at a time (a row's keys have room for whole fours)
+    uint4 k[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      k[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (k0 + 4 * i < g1) k[i] = __ldcg(reinterpret_cast<const uint4*>(keys + k0 + 4 * i));
+    }
+    uint32_t hits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      hits |= (k[i].x >= lo ? 1u : 0u) << (4 * i);
+      hits |= (k[i].y >= lo ? 1u : 0u) << (4 * i + 1);
+      hits |= (k[i].z >= lo ? 1u : 0u) << (4 * i + 2);
+      hits |= (k[i].w >= lo ? 1u : 0u) << (4 * i + 3);
+    }
+    const int32_t left = g1 - k0;
+    if (left < 16) hits &= (1u << left) - 1u;  // (keys past the row's groups were never written)
+    while (hits) {
+      const int32_t v0 = (k0 + __ffs(hits) - 1) * GV;
+      hits &= hits - 1;
+      uint4 q[GV];
+#pragma unroll
+      for (int j = 0; j < GV; ++j) {
+        const uint32_t none = Elem<T>::NEG_INF_WORD;
+        q[j] = make_uint4(none, none, none, none);
+        if (v0 + j < rv.nvec) q[j] = load_vec(rv, v0 + j);
+      }
+#pragma unroll
+      for (int j = 0; j < GV; ++j)
+        if (vec_max_nan<T>(q[j]) >= raw_lo) f(v0 + j, q[j]);
+    }
+  }
+}
+
+constexpr int NEAR_CAP = 1024;  // listed elements of a row drawn from by one CTA
+struct NearShared {
+  uint64_t scan[VNW + 1];
+  uint32_t tscan[VNW + 1];
+  int32_t index[NEAR_CAP];
+  float value[NEAR_CAP];
+};
+
+// The draw over a row whose group keys are known, for rows with few values near the kept ones (as all
+// but odd rows of top-k have): one CTA lists the values that may be kept, in index order (each thread
+// looks through a run of consecutive groups), and weighs the listed ones. Returns the token in the
+// thread that finds it, -1 in the others; false in *fits where the list is too short for the row.
+template <typename T>
+__device__ int32_t draw_listed(const DrawRow<T>& row, const GroupKeys& g, int64_t at_row, uint64_t u53, NearShared& sh,
+                               bool* fits, bool* none) {
+  constexpr int EPV = Elem<T>::EPV, PER = NEAR_CAP / VT;
+  uint32_t mine = 0, n;
+  each_near<T>(g, row.rv, at_row, row.raw_lo, [&](int32_t, uint4 q) {
+    float x[EPV];
+    Elem<T>::unpack(q, x);
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) mine += x[j] >= row.raw_lo;
+  });
+  uint32_t at = block_prefix(mine, sh.tscan, &n);
+  *fits = n <= (uint32_t)NEAR_CAP;
+  *none = false;
+  if (!*fits) return -1;
+  if (mine)
+    each_near<T>(g, row.rv, at_row, row.raw_lo, [&](int32_t v, uint4 q) {
+      float x[EPV];
+      Elem<T>::unpack(q, x);
+#pragma unroll
+      for (int j = 0; j < EPV; ++j)
+        if (x[j] >= row.raw_lo) {  // (elements past the row are -inf, and raw_lo is finite)
+          sh.index[at] = row.rv.first(v) + j;
+          sh.value[at++] = x[j];
+        }
+    });
+  __syncthreads();
+  // entries tid * per .. of the list: target weights, equals of the last kept key, what is left
+  const uint32_t per = (n + VT - 1) / VT, i0 = threadIdx.x * per;
+  uint64_t p[PER], r[PER];
+  uint32_t eq = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    p[j] = r[j] = 0;
+    if ((uint32_t)j < per && i0 + j < n) {
+      const float y = row.scaled(sh.value[i0 + j]);
+      if (y >= row.thr) p[j] = weight_q(y, row.f.max_key);
+      if (row.cut_ties && y == row.thr) eq |= 1u << j;
+    }
+  }
+  if (row.cut_ties) {
+    uint32_t total, before = block_prefix((uint32_t)__popc(eq), sh.tscan, &total);
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if ((eq >> j) & 1u) {
+        if (before >= (uint32_t)row.f.n_tie_kept) p[j] = 0;
+        ++before;
+      }
+  }
+  uint64_t sum = 0, all = 0, total;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (p[j]) {
+      const int32_t e = sh.index[i0 + j];
+      uint64_t taken = 0;
+      if (row.dist) taken = grid_units(row.taken_by(prob_at(row.a, row.drow, e)));
+      else if (row.residual && e == row.dx) taken = p[j];
+      r[j] = p[j] > taken ? p[j] - taken : 0;
+    }
+    sum += r[j];
+    all += p[j];
+  }
+  uint64_t before = block_prefix(sum, sh.scan, &total);
+  const bool target = total == 0;  // an empty residual: drawn from the target itself
+  if (target) {
+    sum = all;
+    before = block_prefix(sum, sh.scan, &total);
+  }
+  *none = total == 0;
+  const uint64_t want = scale_u53(u53, total);
+  if (!(before <= want && want < before + sum)) return -1;
+  int32_t found = -1;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    before += target ? p[j] : r[j];
+    if (found < 0 && before > want) found = sh.index[i0 + j];
+  }
+  return found;
+}
+
+// The same draw for rows of any number of such values (very many equal ones): the runs are looked
+// through again for every sum.
+template <typename T>
+__device__ __noinline__ int32_t draw_near(const DrawRow<T>& row, const GroupKeys& g, int64_t at_row, uint64_t u53,
+                                          NearShared& sh, bool* none) {
+  constexpr int EPV = Elem<T>::EPV;
+  uint32_t base = 0;  // equals of the last kept key before this thread's run
+  if (row.cut_ties) {
+    uint32_t n = 0, total;
+    each_near<T>(g, row.rv, at_row, row.raw_lo, [&](int32_t v, uint4 q) {
+      double r[EPV];
+      uint32_t eq;
+      row.of(v, q, true, false, nullptr, r, eq);
+      n += (uint32_t)__popc(eq);
+    });
+    base = block_prefix(n, sh.tscan, &total);
+  }
+  const uint32_t keep = (uint32_t)row.f.n_tie_kept;
+  // f(first element, weights) of this thread's vectors, equals that were cut without weight
+  auto weights = [&](bool target, auto&& f) {
+    uint32_t at = base;
+    each_near<T>(g, row.rv, at_row, row.raw_lo, [&](int32_t v, uint4 q) {
+      double r[EPV];
+      uint32_t eq;
+      row.of(v, q, target, false, nullptr, r, eq);
+      if (eq) {
+#pragma unroll
+        for (int j = 0; j < EPV; ++j)
+          if ((eq >> j) & 1u) {
+            if (at >= keep) r[j] = 0.0;
+            ++at;
+          }
+      }
+      f(row.rv.first(v), r);
+    });
+  };
+  bool target = false;
+  uint64_t mine, total, before;
+  while (true) {
+    mine = 0;
+    weights(target, [&](int32_t, const double* r) {
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) mine += units(r[j]);
+    });
+    before = block_prefix(mine, sh.scan, &total);
+    if (total || target) break;
+    target = true;  // an empty residual: drawn from the target itself
+  }
+  *none = total == 0;
+  const uint64_t want = scale_u53(u53, total);
+  int32_t found = -1;
+  if (before <= want && want < before + mine) {
+    uint64_t run = before;
+    weights(target, [&](int32_t e0, const double* r) {
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) {
+        run += units(r[j]);
+        if (found < 0 && run > want) found = e0 + j;
+      }
+    });
+  }
+  return found;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
   __shared__ struct {
     int32_t event;
     uint32_t cnt[1];
   } sh;
+  __shared__ NearShared near_sh;
   grid_release();
   const int64_t seq = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31;
@@ -314,6 +637,29 @@ __global__ void __launch_bounds__(VT, 4) decide_kernel(VerifyArgs a) {
   const bool greedy = p.temperature == 0.0;
   const float tf = (float)p.temperature;
   const Scale scaled(tf);
+  // what a draft's row needs of the inputs, loaded before the records are waited for (the first VT
+  // drafts of a sequence; later ones, which hardly exist, load theirs when they are looked at)
+  struct Draft {
+    int64_t x;
+    double u;
+    float logit, prob;
+  };
+  auto draft_of = [&](int64_t r) -> Draft {
+    Draft d{-1, 0.0, 0.0f, 1.0f};
+    if (r >= hi) return d;
+    d.u = a.uniforms[r];
+    if (r == hi - 1) return d;
+    d.x = a.drafts[r];
+    if (greedy || d.x < 0 || d.x >= a.V) return d;
+    d.logit = Elem<T>::ld(static_cast<const T*>(a.x) + r * a.row_stride + d.x);
+    if (a.probs) {
+      const int64_t at = r - seq;
+      d.prob = (at >= 0 && at < a.n_probs) ? prob_at(a, at, d.x) : NAN;
+    }
+    return d;
+  };
+  const Draft first = draft_of(lo + tid);
+  const double u_draw = lo < hi ? a.uniforms[hi - 1] : 0.0;
   grid_wait();  // the rows' records
   if (lo >= hi) {  // a sequence without rows
     if (tid == 0) {
@@ -332,21 +678,21 @@ __global__ void __launch_bounds__(VT, 4) decide_kernel(VerifyArgs a) {
     __syncthreads();
     for (int64_t r = from + tid; r < hi; r += VT) {
       const pb_row_info f = a.info[r];
+      const Draft d = r == lo + tid ? first : draft_of(r);
       int32_t ev = -1;
       if (f.status != PB_ROW_OK) {
         ev = EV_BAD;
-      } else if (!greedy && !(a.uniforms[r] >= 0.0 && a.uniforms[r] < 1.0)) {
+      } else if (!greedy && !(d.u >= 0.0 && d.u < 1.0)) {
         ev = EV_BAD;
       } else if (r == hi - 1) {
         ev = EV_LAST;
       } else {
-        const int64_t x = a.drafts[r];
         bool ok = false;
-        if (x >= 0 && x < a.V) {  // (a draft outside the vocabulary has no mass: rejected)
+        if (d.x >= 0 && d.x < a.V) {  // (a draft outside the vocabulary has no mass: rejected)
           if (greedy) {
-            ok = x == a.tok[r];
+            ok = d.x == a.tok[r];
           } else {
-            const float y = scaled(Elem<T>::ld(static_cast<const T*>(a.x) + r * a.row_stride + x));
+            const float y = scaled(d.logit);
             const uint32_t key = key_of(y);
             bool kept = key > f.thr_key;
             if (key == f.thr_key) {
@@ -355,11 +701,7 @@ __global__ void __launch_bounds__(VT, 4) decide_kernel(VerifyArgs a) {
               else ev = EV_TIE;
             }
             const uint64_t px = (kept || ev == EV_TIE) ? weight_q(y, f.max_key) : 0;
-            double want = a.uniforms[r];
-            if (a.probs) {
-              const int64_t d = r - seq;
-              want = (d >= 0 && d < a.n_probs) ? __dmul_rn(want, (double)prob_at(a, d, x)) : NAN;
-            }
+            const double want = a.probs ? __dmul_rn(d.u, (double)d.prob) : d.u;
             ok = __dmul_rn(want, __ull2double_rn(f.kept_q)) < __ull2double_rn(px);
             if (ev == EV_TIE && !ok) ev = EV_REJECT;  // rejected either way
           }
@@ -383,6 +725,15 @@ __global__ void __launch_bounds__(VT, 4) decide_kernel(VerifyArgs a) {
     __syncthreads();
     uint32_t before = 0;
     const float lo_raw = surely_below(f.thr_key, tf);
+    if (a.groups.keys) {
+      each_near<T>(a.groups, rv, stop, lo_raw, [&](int32_t v, uint4 q4) {
+        float y[EPV];
+        Elem<T>::unpack(q4, y);
+#pragma unroll
+        for (int q = 0; q < EPV; ++q)
+          if (rv.first(v) + q < x && key_of(scaled(y[q])) == f.thr_key) ++before;
+      });
+    } else
     for (int32_t v0 = tid; v0 < rv.nvec && rv.first(v0) < x; v0 += VT * SEG_V) {
       uint4 q4[SEG_V];
 #pragma unroll
@@ -414,7 +765,6 @@ __global__ void __launch_bounds__(VT, 4) decide_kernel(VerifyArgs a) {
     }
     from = stop + 1;  // accepted
   }
-  const double u_draw = a.uniforms[hi - 1];
   if (kind == EV_REJECT && !greedy && !(u_draw >= 0.0 && u_draw < 1.0)) kind = EV_BAD;
 
   for (int64_t r = lo + tid; r < stop; r += VT) a.out_tokens[r] = a.drafts[r];
@@ -424,110 +774,27 @@ __global__ void __launch_bounds__(VT, 4) decide_kernel(VerifyArgs a) {
     if (kind == EV_BAD) st = a.info[stop].status != PB_ROW_OK ? a.info[stop].status : PB_ROW_BAD_UNIFORM;
     if (a.out_status) a.out_status[seq] = st;
     if (greedy && kind != EV_BAD) a.out_tokens[stop] = a.tok[stop];
-    a.decision[seq] = Decision{stop, kind, !greedy && kind != EV_BAD};
+  }
+  // the last token: here, where the row's group keys are known, else by the launches that follow
+  const bool draws = !greedy && kind != EV_BAD, here = a.groups.keys && !whole_row(p, a.V);
+  if (tid == 0) a.decision[seq] = Decision{stop, kind, draws && !here};
+  if (draws && here) {
+    const DrawRow<T> row(a, seq, Decision{stop, kind, 1}, tf, a.info[stop]);
+    const uint64_t u53 = (uint64_t)(u_draw * 0x1p53);
+    bool fits = false, none = false;
+    int32_t found = -1;
+    if (row.raw_lo > -INFINITY) found = draw_listed<T>(row, a.groups, stop, u53, near_sh, &fits, &none);
+    if (!fits) found = draw_near<T>(row, a.groups, stop, u53, near_sh, &none);
+    if (found >= 0) a.out_tokens[stop] = found;
+    if (none && tid == 0 && a.out_status) a.out_status[seq] = PB_ROW_INTERNAL;
   }
 }
 
 // ---- drawing ---------------------------------------------------------------------------------
 
-// The row a sequence draws its last token from, and the weights of its elements.
-template <typename T>
-struct DrawRow {
-  static constexpr int EPV = Elem<T>::EPV;
-  const VerifyArgs& a;
-  RowView<T> rv;
-  pb_row_info f;
-  Scale scaled;
-  Weigher weigh;
-  double z;          // mass, in the weights' own scale
-  float d_most;      // draft probabilities above this take all of any weight
-  int64_t dx, drow;  // the rejected draft; its row of draft_probs
-  bool residual, dist, cut_ties, whole;
-  float raw_lo;
-  __device__ DrawRow(const VerifyArgs& a_, int64_t seq, const Decision& d, float tf, const pb_row_info& f_)
-      : a(a_), rv(static_cast<const T*>(a_.x) + d.row * a_.row_stride, a_.V), f(f_), scaled(tf),
-        weigh(tf, f_.max_key, f_.max_key * tf) {
-    residual = d.kind == EV_REJECT;
-    dx = residual ? a.drafts[d.row] : -1;
-    drow = d.row - seq;
-    dist = residual && a.probs && drow >= 0 && drow < a.n_probs;
-    cut_ties = f.kept_q != f.z_q;
-    whole = f.thr_key == 0;
-    raw_lo = surely_below(f.thr_key, tf);
-    z = __ull2double_rn(f.kept_q) * 0x1p-40;
-    d_most = (float)(2048.0 / z);
-  }
-  // Weights of vector v (elements q4): target, or what the draft's distribution leaves of it, in the
-  // grid's scale. `eq` gets a bit per element whose key equals the last kept one, where top-p cut there.
-  __device__ __forceinline__ void of(int32_t v, uint4 q4, bool target, double* r, uint32_t& eq) const {
-    eq = 0;
-#pragma unroll
-    for (int q = 0; q < EPV; ++q) r[q] = 0.0;
-    if (!(vec_max_nan<T>(q4) >= raw_lo)) return;
-    const int32_t e0 = rv.first(v);
-    float w[EPV];
-    uint32_t some = 0;  // elements of weight
-    if (whole) {
-      weigh.template of<T>(q4, w);
-      some = (1u << EPV) - 1u;
-      if (!rv.whole(v)) {
-#pragma unroll
-        for (int q = 0; q < EPV; ++q)
-          if (e0 + q < 0 || e0 + q >= a.V) some &= ~(1u << q);
-      }
-    } else {
-      float x[EPV];
-      Elem<T>::unpack(q4, x);
-#pragma unroll
-      for (int q = 0; q < EPV; ++q) {
-        w[q] = 0.0f;
-        if (!(x[q] >= raw_lo) || e0 + q < 0 || e0 + q >= a.V) continue;
-        const float y = scaled(x[q]);
-        const uint32_t key = key_of(y);
-        if (key < f.thr_key) continue;
-        w[q] = exp_weight(__fsub_rn(y, f.max_key));
-        some |= 1u << q;
-        if (cut_ties && key == f.thr_key) eq |= 1u << q;
-      }
-    }
-    if (!some) return;
-    float d[EPV];
-    if (dist && !target) {
-      const bool f32 = a.probs_dtype == PB_DTYPE_F32;
-      const float* row32 = static_cast<const float*>(a.probs) + drow * a.probs_stride + e0;
-      if (whole && f32 && some == (1u << EPV) - 1u && (reinterpret_cast<uintptr_t>(row32) & 15) == 0) {
-#pragma unroll
-        for (int q = 0; q < EPV; q += 4) {
-          const float4 p4 = __ldg(reinterpret_cast<const float4*>(row32 + q));
-          d[q] = p4.x;
-          d[q + 1] = p4.y;
-          d[q + 2] = p4.z;
-          d[q + 3] = p4.w;
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < EPV; ++q) d[q] = ((some >> q) & 1u) ? prob_at(a, drow, e0 + q) : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < EPV; ++q) {
-      const double p = on_grid(w[q]);
-      double taken = GRID;
-      if (!target) {
-        // floor(d * Z): NaN and what is below 0 take nothing
-        if (dist) taken = __dadd_rd(GRID, __dmul_rn((double)fminf(fmaxf(d[q], 0.0f), d_most), z));
-        else if (residual && e0 + q == dx) taken = p;
-      }
-      if ((some >> q) & 1u) r[q] = fmax(p - taken, 0.0);
-    }
-  }
-};
-
-__device__ __forceinline__ uint64_t units(double sum) { return (uint64_t)(sum * 0x1p40); }  // (exact)
-
 // CTA (sequence, segment): the sums of the segment's tiles.
 template <typename T>
-__global__ void __launch_bounds__(VT, 4) weigh_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(VT, 3) weigh_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
   __shared__ uint64_t w[VNW][TILES], tw[VNW][TILES];
   __shared__ int32_t tn[VNW][TILES];
@@ -540,25 +807,48 @@ __global__ void __launch_bounds__(VT, 4) weigh_kernel(VerifyArgs a) {
   const DrawRow<T> row(a, seq, d, (float)a.params[seq].temperature, f);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(row.rv.nvec, v0 + a.seg.per);
-  uint4 q[SEG_V];
-  load_segment(row.rv, v0, v1, q);
+  // one vector (and its draft probabilities) is on its way while the one before it is weighed; those
+  // of a whole row's draft distribution are all needed, others only where the target has weight
+  const uint32_t none = Elem<T>::NEG_INF_WORD;
+  const uint4 nothing = make_uint4(none, none, none, none);
+  uint4 next = nothing;
+  float4 next_d[EPV / 4];
+  bool next_have = false;
+  auto fetch = [&](int i) {
+    const int32_t v = v0 + i * SEG_T + (int32_t)threadIdx.x;
+    next = nothing;
+    next_have = false;
+    if (i < SEG_V && v < v1) {
+      next = load_vec(row.rv, v);
+      next_have = row.whole && row.packed_probs(v);
+      if (next_have) row.load_probs(v, next_d);
+    }
+  };
+  fetch(0);
 #pragma unroll 1
   for (int i = 0; i < SEG_V; ++i) {
     if (i * SEG_T >= v1 - v0) {
       if (lane == 0) w[warp][i] = tw[warp][i] = 0, tn[warp][i] = 0;
       continue;
     }
-    uint4 qi = q[0];  // q[i], kept in registers
+    const uint4 qi = next;
+    float4 di[EPV / 4];
 #pragma unroll
-    for (int j = 1; j < SEG_V; ++j)
-      if (j == i) qi = q[j];
+    for (int j = 0; j < EPV / 4; ++j) di[j] = next_d[j];
+    const bool have = next_have;
+    fetch(i + 1);
     double r[EPV], sum = 0.0, tsum = 0.0;
     uint32_t eq;
-    row.of(v0 + i * SEG_T + (int32_t)threadIdx.x, qi, false, r, eq);
+    row.of(v0 + i * SEG_T + (int32_t)threadIdx.x, qi, false, have, di, r, eq);
+    if (eq) {
 #pragma unroll
-    for (int j = 0; j < EPV; ++j) {
-      if ((eq >> j) & 1u) tsum += r[j];
-      else sum += r[j];
+      for (int j = 0; j < EPV; ++j) {
+        if ((eq >> j) & 1u) tsum += r[j];
+        else sum += r[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) sum += r[j];
     }
     uint64_t s = warp_sum(units(sum)), t = 0;
     int32_t n = 0;
@@ -621,7 +911,7 @@ __global__ void __launch_bounds__(VT, 2) draw_kernel(VerifyArgs a) {
     uint32_t eq = 0;
 #pragma unroll
     for (int q = 0; q < EPV; ++q) r[q] = 0.0;
-    if (v < v1) row.of(v, load_vec(row.rv, v), target, r, eq);
+    if (v < v1) row.of(v, load_vec(row.rv, v), target, false, nullptr, r, eq);
     if (row.cut_ties) {
       uint32_t total;
       uint32_t at = before + block_excl_scan<uint32_t, VT>((uint32_t)__popc(eq), sh.tscan, &total);
@@ -786,11 +1076,13 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
   if (sampler) {
     // rows that pb_sample_ws's two passes settle themselves go through it, a batch with others
     // through pb_sample (the same choice as for sampling)
-    if (!(kinds & PB_VERIFY_OTHER))
+    if (!(kinds & PB_VERIFY_OTHER)) {
       rc = pb_sample_ws(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr,
                         ws + plan.sampler, plan.bytes - plan.sampler, st);
-    else
+      a.groups = sample_ws_keys(a.x, dtype, a.n_rows, a.V, a.row_stride, ws + plan.sampler, plan.bytes - plan.sampler);
+    } else {
       rc = pb_sample(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr, st);
+    }
     if (rc != PB_OK) return rc;
   }
   const dim3 rows((unsigned)a.n_rows, (unsigned)a.seg.segs), seqs((unsigned)a.n_seqs), parts((unsigned)a.n_seqs, (unsigned)a.seg.segs);
@@ -800,6 +1092,8 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
     if (rc != PB_OK) return rc;
   }
   rc = launch_after(decide_kernel<T>, a, seqs, VT, st);
+  // (a batch whose every sequence draws in decide_kernel needs no more)
+  if (a.groups.keys && !a.mass_runs) return rc;
   if (rc == PB_OK) rc = launch_after(weigh_kernel<T>, a, parts, VT, st);
   if (rc == PB_OK) rc = launch_after(draw_kernel<T>, a, seqs, VT, st);
   return rc;
