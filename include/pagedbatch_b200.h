@@ -297,14 +297,15 @@ PB_API int pb_stop_check(const int64_t* tokens, int64_t n_rows, const int32_t* r
  *   draw from P at the last row; where those weights are all 0, from P.
  *   draw: the first index, ascending, whose inclusive prefix of the weights exceeds
  *   floor(u * 2^53 * sum / 2^53), u of the sequence's last row (the sampler draws in the order of falling probability instead).
- * workspace: pb_verify_ws_bytes(n_rows, n_seqs, vocab, dtype) bytes of device memory, 256-byte aligned, of any
+ * workspace: pb_verify_ws_bytes(n_rows, n_seqs, vocab, dtype, kinds) bytes of device memory, 256-byte aligned, of any
  * content, not used by another call while this one runs.
  */
 #define PB_VERIFY_SMALL 1 /* greedy, or 0 < top_k <= 128 */
 #define PB_VERIFY_WHOLE 2 /* neither top-k nor top-p */
 #define PB_VERIFY_OTHER 4 /* any other parameters */
-#define PB_VERIFY_ANY 7
-PB_API int64_t pb_verify_ws_bytes(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype);
+#define PB_VERIFY_TOPP 8  /* top-p alone */
+#define PB_VERIFY_ANY 15
+PB_API int64_t pb_verify_ws_bytes(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype, int kinds);
 PB_API int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
                      const pb_row_params* params, int64_t n_seqs, const int32_t* row_offsets, const int64_t* drafts,
                      const double* uniforms, const void* draft_probs, int probs_dtype, int64_t n_probs,

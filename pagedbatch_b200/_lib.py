@@ -24,7 +24,7 @@ ROW_FALLBACK = 32
 CAND_FALLBACK, CAND_GREEDY, CAND_MAX_CAP = 0x100, 0x200, 2048
 PATH_GREEDY, PATH_SMALL, PATH_LARGE, PATH_STREAM = 1, 2, 4, 8
 FINISH_NONE, FINISH_STOP, FINISH_LENGTH = 0, 1, 2
-VERIFY_SMALL, VERIFY_WHOLE, VERIFY_OTHER, VERIFY_ANY = 1, 2, 4, 7
+VERIFY_SMALL, VERIFY_WHOLE, VERIFY_OTHER, VERIFY_TOPP, VERIFY_ANY = 1, 2, 4, 8, 15
 TOP_MAX = 256
 DISTILL_MAX_ENTRIES, DISTILL_MAX_VOCAB = 1024, 1 << 20
 MAX_VOCAB = 1 << 24
@@ -140,7 +140,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     L.pb_stop_check.argtypes = [vp, i64, vp, vp, vp, i32, i32, vp, vp]
     L.pb_stop_check.restype = i32
     f32 = ctypes.c_float
-    L.pb_verify_ws_bytes.argtypes = [i64, i64, i64, i32]
+    L.pb_verify_ws_bytes.argtypes = [i64, i64, i64, i32, i32]
     L.pb_verify_ws_bytes.restype = i64
     L.pb_verify.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, i32, i64, i64, i32, vp, vp, vp, vp, i64, vp]
     L.pb_verify.restype = i32

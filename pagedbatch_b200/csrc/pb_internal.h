@@ -3,6 +3,8 @@
 
 #include <stdint.h>
 
+#include "../../include/pagedbatch_b200.h"
+
 namespace pb {
 
 // Group keys that pb_sample_ws leaves in its workspace: for every row, the key of the largest value of
@@ -17,5 +19,10 @@ struct GroupKeys {
 // other launch, which leaves none.
 GroupKeys sample_ws_keys(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
                          const void* workspace, int64_t ws_bytes);
+
+// The cluster kernel over the rows whose status in `info` is PB_ROW_FALLBACK (vocab < 2^24, valid
+// arguments): their tokens and records are written, the other rows' are left as they are.
+int sample_fallback_rows(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                         const pb_row_params* params, int64_t* out_token, pb_row_info* info, void* stream);
 
 }  // namespace pb

@@ -2667,6 +2667,30 @@ GroupKeys sample_ws_keys(const void* logits, int dtype, int64_t n_rows, int64_t 
   return g;
 }
 
+int sample_fallback_rows(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                         const pb_row_params* params, int64_t* out_token, pb_row_info* info, void* stream) {
+  Args a;
+  a.logits = static_cast<const char*>(logits);
+  a.n_rows = n_rows;
+  a.vocab = vocab;
+  a.row_stride = row_stride;
+  a.row_index = nullptr;
+  a.params = params;
+  a.out_token = out_token;
+  a.out_info = info;
+  a.out_probs = nullptr;
+  a.only_fallback = info;
+  a.complement = 0;
+  a.cand_out = nullptr;
+  a.cand_cap = 0;
+  a.vocab_offset = 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int C = cluster_size_for(n_rows, vocab, dtype == PB_DTYPE_F32 ? 4 : 2);
+  if (dtype == PB_DTYPE_F32) return launch<float>(a, C, st);
+  if (dtype == PB_DTYPE_BF16) return launch<__nv_bfloat16>(a, C, st);
+  return launch<__half>(a, C, st);
+}
+
 }  // namespace pb
 
 extern "C" {

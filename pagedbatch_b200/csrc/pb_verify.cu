@@ -15,9 +15,13 @@
 //
 // Launches, each of which may start while the one before it ends:
 //   1. expand_kernel: each row's parameters from its sequence's.
-//   2. the sampler over the rows (its info record describes the kept set and its mass). Rows without
-//      top-k and top-p, whose kept set is the whole row, go through max_kernel and mass_kernel instead:
-//      two passes in segments, the largest value and then the sum of the weights.
+//   2. each row's kept set and its mass, as the sampler's info record describes them. Greedy and small
+//      top-k rows: pb_sample_ws. Rows without filters, whose kept set is the whole row: max_kernel and
+//      mass_kernel, two passes in segments, the largest value and then the sum of the weights. Rows
+//      with top-p alone: max_kernel, then hist_kernel sums the weights in 512 steps of the key,
+//      cut_kernel finds the step in which the mass passes top-p, gather_kernel lists its elements and
+//      order_kernel finds the last kept one among them. Every other row (large top-k, a step of too
+//      many elements, rejected parameters): the sampler's cluster kernel.
 //   3. decide_kernel: a CTA per sequence finds the first rejected row.
 //   4. weigh_kernel: that row's weights, summed per tile (256 vectors), a CTA per segment.
 //   5. draw_kernel: a CTA per sequence finds the draw's tile and its element.
@@ -32,15 +36,25 @@ namespace {
 
 constexpr int VT = SEG_T;        // threads per CTA
 constexpr int VNW = SEG_NW;
+constexpr int SMALL_K = 128;      // largest top_k that pb_sample_ws's two passes settle
 constexpr int TILES = SEG_V;     // tiles per segment: tile i holds vectors v0 + i * SEG_T + thread
 
 // A row as the passes over whole rows see it.
+enum : int32_t { ROW_SMALL = 0, ROW_WHOLE = 1, ROW_MASS = 2, ROW_OTHER = 3 };  // what settles a row
 struct RowMeta {
   float t;           // temperature
-  int32_t whole;     // the row's kept set is the whole row
+  int32_t kind;      // ROW_*
   uint32_t max_key;  // key of its largest value (max_kernel)
-  int32_t pad;
+  uint32_t listed;   // ROW_MASS: elements of the step where top-p cuts (gather_kernel)
+  uint64_t above;    // ... mass above the step
+  uint64_t cut;      // ... floor(top_p * mass)
+  int32_t step;      // ... the step
+  float top_p;
 };
+
+constexpr int STEPS = 512;             // histogram steps of a row's key
+constexpr float STEP_SCALE = STEPS / 28.0f;  // keys further than 27.73 below the maximum have no weight
+constexpr int LIST = 2048;             // elements order_kernel takes from one step
 
 // Sums of one tile of the row a sequence draws from, in units of 2^-40. Where top-p cut among the
 // equals of the last kept key, `w` leaves those equals out, `tie_w` is theirs and `ties` counts them.
@@ -68,8 +82,10 @@ struct VerifyArgs {
   const void* probs;             // [n_probs][V], or null
   int64_t probs_stride, n_probs;
   int32_t probs_dtype;
-  int32_t mass_runs;
-  pb_row_params* rowp;           // workspace: [n_rows]
+  pb_row_params* rowp;           // workspace: [n_rows], what pb_sample_ws sees
+  pb_row_params* rowq;           // workspace: [n_rows], the rows' own
+  uint64_t* hist;                // workspace: [n_rows][STEPS] (a batch with ROW_MASS rows)
+  uint64_t* list;                // ... [n_rows][LIST]
   pb_row_info* info;             // workspace: [n_rows]
   int64_t* tok;                  // workspace: [n_rows], the sampler's tokens (greedy rows' maxima)
   RowMeta* meta;                 // workspace: [n_rows]
@@ -77,16 +93,19 @@ struct VerifyArgs {
   Tile* tiles;                   // workspace: [n_seqs][segs][TILES]
   SegPlan seg;
   GroupKeys groups;              // of the rows the sampler settled (keys null: none)
-  int32_t all_whole;
+  int32_t kinds;                 // PB_VERIFY_* of the batch, as the caller names them
+  int32_t one_kind;              // ROW_WHOLE or ROW_MASS where every row is of that kind, else -1
   int64_t* out_tokens;           // [n_rows]
   int32_t* out_accepted;         // [n_seqs]
   int32_t* out_status;           // [n_seqs] or null
 };
 
-// Rows whose kept set is the whole row: valid parameters, no greedy, no top-k, no top-p.
-__device__ __forceinline__ bool whole_row(const pb_row_params& p, int32_t V) {
-  const bool ok = p.temperature > 0.0 && p.top_p > 0.0 && p.top_p <= 1.0 && p.top_k >= 0;
-  return ok && !(p.top_k > 0 && p.top_k < V) && !((float)p.top_p < 1.0f);
+// What settles a row of these parameters.
+__device__ __forceinline__ int32_t row_kind(const pb_row_params& p, int32_t V) {
+  if (!(p.temperature >= 0.0) || !(p.top_p > 0.0 && p.top_p <= 1.0) || p.top_k < 0) return ROW_OTHER;  // rejected there
+  if (p.temperature == 0.0) return ROW_SMALL;
+  if (p.top_k > 0 && p.top_k < V) return p.top_k <= SMALL_K ? ROW_SMALL : ROW_OTHER;
+  return (float)p.top_p < 1.0f ? ROW_MASS : ROW_WHOLE;
 }
 
 __global__ void __launch_bounds__(256) expand_kernel(VerifyArgs a) {
@@ -101,10 +120,11 @@ __global__ void __launch_bounds__(256) expand_kernel(VerifyArgs a) {
   pb_row_params p = a.params[lo];
   p.uniform = 0.0;  // the sampler's own draw is not used
   p.rng = 0;
-  const bool whole = a.mass_runs && whole_row(p, a.V);
-  a.meta[r] = RowMeta{(float)p.temperature, whole, 0u, 0};
-  // mass_kernel sums these; the sampler passes over them as greedy rows, its cheapest kind
-  if (whole) p.temperature = 0.0;
+  const int32_t kind = row_kind(p, a.V);
+  a.meta[r] = RowMeta{(float)p.temperature, kind, 0u, 0u, 0ull, 0ull, 0, (float)p.top_p};
+  a.rowq[r] = p;
+  // rows of other kinds pass through pb_sample_ws as greedy ones, its cheapest
+  if (kind != ROW_SMALL) p.temperature = 0.0, p.top_p = 1.0, p.top_k = 0;
   a.rowp[r] = p;
   pb_row_info* o = a.info + r;
   o->status = PB_ROW_INTERNAL;  // until a launch settles the row
@@ -125,6 +145,13 @@ struct Scale {
     return (inv != 0.0f) ? __fmul_rn(x, inv) : __fdiv_rn(x, t);
   }
 };
+
+// Raw values below this are surely below the scaled key thr (a few roundings of the quotient apart).
+__device__ __forceinline__ float surely_below(uint32_t thr, float tf) {
+  if (!(thr > KEY_NEG_INF && thr < KEY_POS_INF)) return -INFINITY;
+  const float b = value_of(thr) * tf, r = b - fabsf(b) * 0x1p-20f - 0x1p-100f;
+  return (r > -INFINITY) ? r : -INFINITY;
+}
 
 // ---- weights ---------------------------------------------------------------------------------
 
@@ -208,15 +235,17 @@ __device__ __forceinline__ uint64_t grid_units(double sum) {                    
   return (uint64_t)__double_as_longlong(sum) & ((1ull << 52) - 1);
 }
 
-// Key of the largest value of every whole row.
+// Key of the largest value of every row that is summed here; clears the histograms of those with one.
 template <typename T>
 __global__ void __launch_bounds__(VT, SEG_CTAS) max_kernel(VerifyArgs a) {
   __shared__ uint32_t top[VNW];
   grid_release();
   const int64_t row = blockIdx.x;
-  if (!a.all_whole) {
+  int32_t kind = a.one_kind;
+  if (kind < 0) {
     grid_wait();
-    if (!a.meta[row].whole) return;
+    kind = a.meta[row].kind;
+    if (kind != ROW_WHOLE && !(kind == ROW_MASS && a.hist)) return;
   }
   const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
   const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
@@ -226,6 +255,8 @@ __global__ void __launch_bounds__(VT, SEG_CTAS) max_kernel(VerifyArgs a) {
   if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = k;
   __syncthreads();
   grid_wait();  // expand_kernel has set the keys to 0
+  if (kind == ROW_MASS && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < STEPS; i += VT) a.hist[row * STEPS + i] = 0;
   if (threadIdx.x < 32) {
     k = __reduce_max_sync(0xFFFFFFFFu, threadIdx.x < VNW ? top[threadIdx.x] : 0u);
     if (threadIdx.x == 0) atomicMax(&a.meta[row].max_key, k);
@@ -243,11 +274,11 @@ __global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
   const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
   const int32_t v0 = (int32_t)(gridDim.y - 1 - blockIdx.y) * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
   uint4 q[SEG_V];
-  if (a.all_whole) load_segment(rv, v0, v1, q);
+  if (a.one_kind == ROW_WHOLE) load_segment(rv, v0, v1, q);
   grid_wait();  // the rows' largest values
   const RowMeta meta = a.meta[row];
-  if (!meta.whole) return;
-  if (!a.all_whole) load_segment(rv, v0, v1, q);
+  if (meta.kind != ROW_WHOLE) return;
+  if (a.one_kind != ROW_WHOLE) load_segment(rv, v0, v1, q);
   const float raw = value_of(meta.max_key), m = Scale(meta.t)(raw);
   const uint32_t sk = key_of(m);
   const bool ok = meta.max_key != 0xFFFFFFFFu && sk < KEY_POS_INF && sk > KEY_NEG_INF;
@@ -286,6 +317,199 @@ __global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
   }
 }
 
+// ---- top-p alone -----------------------------------------------------------------------------
+
+// Step of a scaled value y in its row's histogram: it does not fall as y falls.
+__device__ __forceinline__ int32_t step_of(float y, float m) {
+  return min(STEPS - 1, (int32_t)__fmul_rn(__fsub_rn(m, y), STEP_SCALE));
+}
+
+// Sums of the weights of every ROW_MASS row, by step.
+template <typename T>
+__global__ void __launch_bounds__(VT, 3) hist_kernel(VerifyArgs a) {
+  constexpr int EPV = Elem<T>::EPV;
+  __shared__ uint32_t lo[STEPS], hi[STEPS];  // 64-bit sums in two words (a carry is rare)
+  grid_release();
+  const int64_t row = a.n_rows - 1 - blockIdx.x;
+  const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
+  const int32_t v0 = (int32_t)(gridDim.y - 1 - blockIdx.y) * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+  uint4 q[SEG_V];
+  if (a.one_kind == ROW_MASS) load_segment(rv, v0, v1, q);
+  for (int i = threadIdx.x; i < STEPS; i += VT) lo[i] = hi[i] = 0;
+  grid_wait();  // the rows' largest values
+  const RowMeta meta = a.meta[row];
+  if (meta.kind != ROW_MASS) return;
+  if (a.one_kind != ROW_MASS) load_segment(rv, v0, v1, q);
+  const float raw = value_of(meta.max_key), m = Scale(meta.t)(raw);
+  const uint32_t sk = key_of(m);
+  if (meta.max_key == 0xFFFFFFFFu || sk >= KEY_POS_INF || sk <= KEY_NEG_INF) return;  // (no distribution)
+  const Weigher weigh(meta.t, m, raw);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < SEG_V; ++i) {
+    if (i * SEG_T >= v1 - v0) break;
+    float w[EPV], y[EPV];
+    weigh.template of<T>(q[i], w, y);
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) {
+      const uint64_t u = grid_units(on_grid(w[j]));
+      if (!u) continue;
+      const int32_t s = step_of(y[j], m);
+      const uint32_t l = (uint32_t)u, old = atomicAdd(&lo[s], l);
+      const uint32_t h = (uint32_t)(u >> 32) + (old + l < old ? 1u : 0u);
+      if (h) atomicAdd(&hi[s], h);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < STEPS; i += VT) {
+    const unsigned long long u = (uint64_t)hi[i] << 32 | lo[i];
+    if (u) atomicAdd(reinterpret_cast<unsigned long long*>(a.hist + row * STEPS + i), u);
+  }
+}
+
+// The step in which a ROW_MASS row's mass passes top-p: the last one that holds weight and has at most
+// floor(top_p * mass) above it. All weights of the steps above it are kept, none of those below.
+__global__ void __launch_bounds__(VT) cut_kernel(VerifyArgs a) {
+  __shared__ uint64_t scan[VNW + 1];
+  __shared__ int32_t last;
+  grid_release();
+  const int64_t row = blockIdx.x;
+  if (threadIdx.x == 0) last = 0;
+  grid_wait();
+  const RowMeta meta = a.meta[row];
+  if (meta.kind != ROW_MASS) return;
+  const float m = Scale(meta.t)(value_of(meta.max_key));
+  const uint32_t sk = key_of(m);
+  if (meta.max_key == 0xFFFFFFFFu || sk >= KEY_POS_INF || sk <= KEY_NEG_INF) {
+    if (threadIdx.x == 0) a.info[row].status = PB_ROW_NONFINITE;
+    return;
+  }
+  constexpr int PER = STEPS / VT;
+  const uint64_t* h = a.hist + row * STEPS + threadIdx.x * PER;
+  uint64_t v[PER], sum = 0, z;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum += v[i] = __ldcg(h + i);
+  uint64_t above = block_excl_scan<uint64_t, VT>(sum, scan, &z);
+  const uint64_t cut = mul_floor(meta.top_p, z), first = above;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (v[i] && above <= cut) atomicMax(&last, (int32_t)threadIdx.x * PER + i);
+    above += v[i];
+  }
+  __syncthreads();
+  if ((int32_t)threadIdx.x == last / PER) {
+    above = first;
+    for (int i = 0; i < last % PER; ++i) above += v[i];
+    RowMeta* o = a.meta + row;
+    o->above = above;
+    o->cut = cut;
+    o->step = last;
+    o->listed = 0;
+    a.info[row].z_q = z;
+    a.info[row].max_key = m;
+  }
+}
+
+// The elements of that step, in any order.
+template <typename T>
+__global__ void __launch_bounds__(VT, 4) gather_kernel(VerifyArgs a) {
+  constexpr int EPV = Elem<T>::EPV;
+  grid_release();
+  const int64_t row = blockIdx.x;
+  const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
+  const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+  uint4 q[SEG_V];
+  if (a.one_kind == ROW_MASS) load_segment(rv, v0, v1, q);
+  grid_wait();
+  const RowMeta meta = a.meta[row];
+  if (meta.kind != ROW_MASS || a.info[row].status == PB_ROW_NONFINITE) return;
+  if (a.one_kind != ROW_MASS) load_segment(rv, v0, v1, q);
+  const Scale scaled(meta.t);
+  const float m = a.info[row].max_key;
+  // raw values that are surely below the step
+  const float raw_lo = surely_below(key_of(m - ((float)meta.step + 1.5f) / STEP_SCALE), meta.t);
+#pragma unroll
+  for (int i = 0; i < SEG_V; ++i) {
+    if (!(vec_max_nan<T>(q[i]) >= raw_lo)) continue;
+    float x[EPV];
+    Elem<T>::unpack(q[i], x);
+    const int32_t e0 = rv.first(v0 + i * SEG_T + (int32_t)threadIdx.x);
+#pragma unroll 1
+    for (int j = 0; j < EPV; ++j) {
+      const float xj = Elem<T>::elem(q[i], j);
+      if (!(xj >= raw_lo)) continue;
+      const float y = scaled(xj);
+      if (e0 + j < 0 || e0 + j >= a.V || step_of(y, m) != meta.step || !weight_q(y, m)) continue;
+      const uint32_t at = atomicAdd(&a.meta[row].listed, 1u);
+      if (at < (uint32_t)LIST) a.list[row * LIST + at] = compose(key_of(y), (uint32_t)(e0 + j));
+    }
+  }
+}
+
+// The last kept element among them, in the order (key descending, index ascending): what the row's
+// record needs. Rows of other kinds, and steps of more elements than the list holds (or none: no step
+// was looked for), are left to the sampler.
+__global__ void __launch_bounds__(VT) order_kernel(VerifyArgs a) {
+  __shared__ uint64_t list[LIST];
+  __shared__ uint64_t scan[VNW + 1];
+  __shared__ int32_t kept;
+  __shared__ uint64_t kept_q;
+  grid_wait();
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const RowMeta meta = a.meta[row];
+  pb_row_info* o = a.info + row;
+  if (meta.kind == ROW_OTHER || (meta.kind == ROW_MASS && o->status != PB_ROW_NONFINITE && (meta.listed == 0 || meta.listed > (uint32_t)LIST))) {
+    if (tid == 0) o->status = PB_ROW_FALLBACK;
+    return;
+  }
+  if (meta.kind != ROW_MASS || o->status == PB_ROW_NONFINITE) return;
+  const int32_t n = (int32_t)meta.listed;
+  uint32_t size = 2;
+  while (size < (uint32_t)n) size <<= 1;
+  for (uint32_t i = tid; i < size; i += VT) list[i] = i < (uint32_t)n ? __ldcg(a.list + row * LIST + i) : 0ull;
+  if (tid == 0) kept = 0, kept_q = 0;
+  __syncthreads();
+  for (uint32_t k = 2; k <= size; k <<= 1)
+    for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+      for (uint32_t i = tid; i < size / 2; i += VT) {
+        const uint32_t p = ((i & ~(j - 1)) << 1) | (i & (j - 1)), p2 = p | j;
+        const uint64_t x = list[p], y = list[p2];
+        if ((x < y) == ((p & k) == 0)) {
+          list[p] = y;
+          list[p2] = x;
+        }
+      }
+      __syncthreads();
+    }
+  // kept: those whose exclusive prefix of the mass is at most the cut (a prefix of the list)
+  const float m = o->max_key;
+  uint64_t base = meta.above;
+  for (int32_t i0 = 0; i0 < n; i0 += VT) {
+    const int32_t i = i0 + tid;
+    const uint64_t q = i < n ? weight_q(value_of(comp_key(list[i])), m) : 0;
+    uint64_t total;
+    const uint64_t before = base + block_excl_scan<uint64_t, VT>(q, scan, &total);
+    if (i < n && before <= meta.cut) {
+      atomicMax(&kept, i + 1);
+      atomicMax(reinterpret_cast<unsigned long long*>(&kept_q), (unsigned long long)(before + q));
+    }
+    base += total;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    const uint32_t thr = comp_key(list[kept - 1]);
+    int32_t first = kept - 1;
+    while (first > 0 && comp_key(list[first - 1]) == thr) --first;
+    o->thr_key = thr;
+    o->n_tie_kept = kept - first;
+    o->kept_count = 0;  // (not needed here)
+    o->status = PB_ROW_OK;
+    o->flags = PB_PATH_LARGE;
+    o->kept_q = kept_q;
+  }
+}
+
 // ---- deciding --------------------------------------------------------------------------------
 
 enum : int32_t { EV_REJECT = 0, EV_BAD = 1, EV_TIE = 2, EV_LAST = 3 };
@@ -297,12 +521,6 @@ __device__ __forceinline__ float prob_at(const VerifyArgs& a, int64_t d, int64_t
   return Elem<__half>::ld(static_cast<const __half*>(a.probs) + at);
 }
 
-// Raw values below this are surely below the scaled key thr (a few roundings of the quotient apart).
-__device__ __forceinline__ float surely_below(uint32_t thr, float tf) {
-  if (!(thr > KEY_NEG_INF && thr < KEY_POS_INF)) return -INFINITY;
-  const float b = value_of(thr) * tf, r = b - fabsf(b) * 0x1p-20f - 0x1p-100f;
-  return (r > -INFINITY) ? r : -INFINITY;
-}
 
 // The row a sequence draws its last token from, and the weights of its elements.
 template <typename T>
@@ -659,6 +877,11 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
     return d;
   };
   const Draft first = draft_of(lo + tid);
+  // whether a launch settles rows of this kind (the one for other kinds takes top-p's too)
+  const int32_t row_is = row_kind(p, a.V);
+  const int32_t takes = row_is == ROW_SMALL ? PB_VERIFY_SMALL : row_is == ROW_WHOLE ? PB_VERIFY_WHOLE
+                        : row_is == ROW_MASS ? PB_VERIFY_TOPP | PB_VERIFY_OTHER : PB_VERIFY_OTHER;
+  const bool settled = (a.kinds & takes) != 0;
   const double u_draw = lo < hi ? a.uniforms[hi - 1] : 0.0;
   grid_wait();  // the rows' records
   if (lo >= hi) {  // a sequence without rows
@@ -680,7 +903,7 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
       const pb_row_info f = a.info[r];
       const Draft d = r == lo + tid ? first : draft_of(r);
       int32_t ev = -1;
-      if (f.status != PB_ROW_OK) {
+      if (!settled || f.status != PB_ROW_OK) {
         ev = EV_BAD;
       } else if (!greedy && !(d.u >= 0.0 && d.u < 1.0)) {
         ev = EV_BAD;
@@ -725,7 +948,7 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
     __syncthreads();
     uint32_t before = 0;
     const float lo_raw = surely_below(f.thr_key, tf);
-    if (a.groups.keys) {
+    if (a.groups.keys && row_is == ROW_SMALL) {
       each_near<T>(a.groups, rv, stop, lo_raw, [&](int32_t v, uint4 q4) {
         float y[EPV];
         Elem<T>::unpack(q4, y);
@@ -771,12 +994,13 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
   if (tid == 0) {
     a.out_accepted[seq] = (int32_t)(stop - lo);
     int32_t st = PB_ROW_OK;
-    if (kind == EV_BAD) st = a.info[stop].status != PB_ROW_OK ? a.info[stop].status : PB_ROW_BAD_UNIFORM;
+    if (!settled) st = PB_ROW_INTERNAL;
+    else if (kind == EV_BAD) st = a.info[stop].status != PB_ROW_OK ? a.info[stop].status : PB_ROW_BAD_UNIFORM;
     if (a.out_status) a.out_status[seq] = st;
     if (greedy && kind != EV_BAD) a.out_tokens[stop] = a.tok[stop];
   }
   // the last token: here, where the row's group keys are known, else by the launches that follow
-  const bool draws = !greedy && kind != EV_BAD, here = a.groups.keys && !whole_row(p, a.V);
+  const bool draws = !greedy && kind != EV_BAD, here = a.groups.keys && row_is == ROW_SMALL;
   if (tid == 0) a.decision[seq] = Decision{stop, kind, draws && !here};
   if (draws && here) {
     const DrawRow<T> row(a, seq, Decision{stop, kind, 1}, tf, a.info[stop]);
@@ -1042,59 +1266,72 @@ __global__ void __launch_bounds__(VT, 2) draw_kernel(VerifyArgs a) {
 constexpr int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 struct VerifyPlan {
-  int64_t rowp, info, tok, meta, decision, tiles, sampler, bytes;  // offsets in the workspace, and its size
+  int64_t rowp, rowq, info, tok, meta, decision, tiles, hist, list, sampler, bytes;  // offsets in the workspace, its size
 };
-VerifyPlan verify_plan(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype) {
+VerifyPlan verify_plan(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype, int kinds) {
   const SegPlan seg = seg_plan(vocab, elem_size(dtype), nullptr, 1);  // (rows of any alignment: the most segments)
   VerifyPlan v;
-  v.rowp = 0;
-  v.info = up256(n_rows * (int64_t)sizeof(pb_row_params));
-  v.tok = v.info + up256(n_rows * (int64_t)sizeof(pb_row_info));
-  v.meta = v.tok + up256(n_rows * 8);
-  v.decision = v.meta + up256(n_rows * (int64_t)sizeof(RowMeta));
-  v.tiles = v.decision + up256(n_seqs * (int64_t)sizeof(Decision));
-  v.sampler = v.tiles + up256(n_seqs * seg.segs * TILES * (int64_t)sizeof(Tile));
-  v.bytes = v.sampler + pb_sample_ws_bytes(n_rows, vocab, dtype);
+  int64_t at = 0;
+  auto take = [&at](int64_t bytes) {
+    const int64_t from = at;
+    at += up256(bytes);
+    return from;
+  };
+  v.rowp = take(n_rows * (int64_t)sizeof(pb_row_params));
+  v.rowq = take(n_rows * (int64_t)sizeof(pb_row_params));
+  v.info = take(n_rows * (int64_t)sizeof(pb_row_info));
+  v.tok = take(n_rows * 8);
+  v.meta = take(n_rows * (int64_t)sizeof(RowMeta));
+  v.decision = take(n_seqs * (int64_t)sizeof(Decision));
+  v.tiles = take(n_seqs * seg.segs * TILES * (int64_t)sizeof(Tile));
+  v.hist = take(kinds & PB_VERIFY_TOPP ? n_rows * STEPS * 8 : 0);
+  v.list = take(kinds & PB_VERIFY_TOPP ? n_rows * LIST * 8 : 0);
+  v.sampler = at;
+  v.bytes = at + (kinds & PB_VERIFY_SMALL ? pb_sample_ws_bytes(n_rows, vocab, dtype) : 0);
   return v;
 }
 
 template <typename T>
 int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan& plan, cudaStream_t st) {
   a.rowp = reinterpret_cast<pb_row_params*>(ws + plan.rowp);
+  a.rowq = reinterpret_cast<pb_row_params*>(ws + plan.rowq);
   a.info = reinterpret_cast<pb_row_info*>(ws + plan.info);
   a.tok = reinterpret_cast<int64_t*>(ws + plan.tok);
   a.meta = reinterpret_cast<RowMeta*>(ws + plan.meta);
   a.decision = reinterpret_cast<Decision*>(ws + plan.decision);
   a.tiles = reinterpret_cast<Tile*>(ws + plan.tiles);
+  if (kinds & PB_VERIFY_TOPP) {
+    a.hist = reinterpret_cast<uint64_t*>(ws + plan.hist);
+    a.list = reinterpret_cast<uint64_t*>(ws + plan.list);
+  }
   a.seg = seg_plan(a.V, sizeof(T), a.x, a.row_stride);
-  const bool sampler = (kinds & (PB_VERIFY_SMALL | PB_VERIFY_OTHER)) != 0;
-  a.mass_runs = (kinds & PB_VERIFY_WHOLE) != 0;
-  a.all_whole = kinds == PB_VERIFY_WHOLE;
+  a.kinds = kinds;
+  a.one_kind = kinds == PB_VERIFY_WHOLE ? ROW_WHOLE : kinds == PB_VERIFY_TOPP ? ROW_MASS : -1;
+  const dim3 rows((unsigned)a.n_rows, (unsigned)a.seg.segs), each_row((unsigned)a.n_rows);
+  const dim3 seqs((unsigned)a.n_seqs), parts((unsigned)a.n_seqs, (unsigned)a.seg.segs);
   expand_kernel<<<(unsigned)((a.n_rows + 255) / 256), 256, 0, st>>>(a);
-  if (cudaGetLastError() != cudaSuccess) return PB_E_LAUNCH;
-  int rc = PB_OK;
-  if (sampler) {
-    // rows that pb_sample_ws's two passes settle themselves go through it, a batch with others
-    // through pb_sample (the same choice as for sampling)
-    if (!(kinds & PB_VERIFY_OTHER)) {
-      rc = pb_sample_ws(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr,
-                        ws + plan.sampler, plan.bytes - plan.sampler, st);
-      a.groups = sample_ws_keys(a.x, dtype, a.n_rows, a.V, a.row_stride, ws + plan.sampler, plan.bytes - plan.sampler);
-    } else {
-      rc = pb_sample(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr, st);
-    }
-    if (rc != PB_OK) return rc;
+  int rc = cudaGetLastError() == cudaSuccess ? PB_OK : PB_E_LAUNCH;
+  if (rc == PB_OK && (kinds & PB_VERIFY_SMALL)) {
+    rc = pb_sample_ws(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr,
+                      ws + plan.sampler, plan.bytes - plan.sampler, st);
+    a.groups = sample_ws_keys(a.x, dtype, a.n_rows, a.V, a.row_stride, ws + plan.sampler, plan.bytes - plan.sampler);
   }
-  const dim3 rows((unsigned)a.n_rows, (unsigned)a.seg.segs), seqs((unsigned)a.n_seqs), parts((unsigned)a.n_seqs, (unsigned)a.seg.segs);
-  if (a.mass_runs) {
-    rc = launch_after(max_kernel<T>, a, rows, VT, st);
-    if (rc == PB_OK) rc = launch_after(mass_kernel<T>, a, rows, VT, st);
-    if (rc != PB_OK) return rc;
+  if (rc == PB_OK && (kinds & (PB_VERIFY_WHOLE | PB_VERIFY_TOPP))) rc = launch_after(max_kernel<T>, a, rows, VT, st);
+  if (rc == PB_OK && (kinds & PB_VERIFY_WHOLE)) rc = launch_after(mass_kernel<T>, a, rows, VT, st);
+  if (rc == PB_OK && (kinds & PB_VERIFY_TOPP)) {
+    rc = launch_after(hist_kernel<T>, a, rows, VT, st);
+    if (rc == PB_OK) rc = launch_after(cut_kernel, a, each_row, VT, st);
+    if (rc == PB_OK) rc = launch_after(gather_kernel<T>, a, rows, VT, st);
   }
-  rc = launch_after(decide_kernel<T>, a, seqs, VT, st);
+  if (rc == PB_OK && (kinds & (PB_VERIFY_TOPP | PB_VERIFY_OTHER))) {
+    rc = launch_after(order_kernel, a, each_row, VT, st);
+    if (rc == PB_OK)
+      rc = sample_fallback_rows(a.x, dtype, a.n_rows, a.V, a.row_stride, a.rowq, a.tok, a.info, st);
+  }
+  if (rc == PB_OK) rc = launch_after(decide_kernel<T>, a, seqs, VT, st);
   // (a batch whose every sequence draws in decide_kernel needs no more)
-  if (a.groups.keys && !a.mass_runs) return rc;
-  if (rc == PB_OK) rc = launch_after(weigh_kernel<T>, a, parts, VT, st);
+  if (rc != PB_OK || (kinds == PB_VERIFY_SMALL && a.groups.keys)) return rc;
+  rc = launch_after(weigh_kernel<T>, a, parts, VT, st);
   if (rc == PB_OK) rc = launch_after(draw_kernel<T>, a, seqs, VT, st);
   return rc;
 }
@@ -1103,9 +1340,9 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
 
 extern "C" {
 
-int64_t pb_verify_ws_bytes(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype) {
-  if (n_rows < 0 || n_seqs < 0 || vocab <= 0 || !elem_size(dtype)) return PB_E_INVALID;
-  return verify_plan(n_rows, n_seqs, vocab, dtype).bytes;
+int64_t pb_verify_ws_bytes(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype, int kinds) {
+  if (n_rows < 0 || n_seqs < 0 || vocab <= 0 || !elem_size(dtype) || kinds < 0 || kinds > PB_VERIFY_ANY) return PB_E_INVALID;
+  return verify_plan(n_rows, n_seqs, vocab, dtype, kinds ? kinds : PB_VERIFY_ANY).bytes;
 }
 
 int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
@@ -1127,7 +1364,8 @@ int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int6
     if (!ps || probs_stride < vocab || reinterpret_cast<uintptr_t>(draft_probs) % ps) return PB_E_INVALID;
   }
   if (kinds < 0 || kinds > PB_VERIFY_ANY) return PB_E_INVALID;
-  const VerifyPlan plan = verify_plan(n_rows, n_seqs, vocab, dtype);
+  const int k = kinds ? kinds : PB_VERIFY_ANY;
+  const VerifyPlan plan = verify_plan(n_rows, n_seqs, vocab, dtype, k);
   if ((reinterpret_cast<uintptr_t>(workspace) & 255) || ws_bytes < plan.bytes) return PB_E_INVALID;
   VerifyArgs a = {};
   a.x = logits;
@@ -1146,7 +1384,6 @@ int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int6
   a.out_tokens = out_tokens;
   a.out_accepted = out_accepted;
   a.out_status = out_status;
-  const int k = kinds ? kinds : PB_VERIFY_ANY;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == PB_DTYPE_F32) return verify_run<float>(a, dtype, k, ws, plan, st);

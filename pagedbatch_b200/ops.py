@@ -92,9 +92,10 @@ def row_kinds(rec: np.ndarray) -> tuple[int, int]:
     valid = (t >= 0.0) & (p > 0.0) & (p <= 1.0) & (k >= 0)
     greedy = valid & (t == 0.0)
     small = greedy | (valid & (k > 0) & (k <= GROUP_KMAX))
-    whole = valid & ~small & (k == 0) & (p.astype(np.float32) >= 1.0)
+    cuts = p.astype(np.float32) < 1.0
+    whole, topp = (valid & ~small & (k == 0) & c for c in (~cuts, cuts))
     bits = (_lib.VERIFY_SMALL * bool(small.any()) | _lib.VERIFY_WHOLE * bool(whole.any())
-            | _lib.VERIFY_OTHER * bool((~small & ~whole).any()))
+            | _lib.VERIFY_TOPP * bool(topp.any()) | _lib.VERIFY_OTHER * bool((~small & ~whole & ~topp).any()))
     return bits, int(k[~greedy].max()) if np.any(~greedy) else 0
 
 

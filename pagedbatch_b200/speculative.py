@@ -70,13 +70,14 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs):
     with ops.on_device(dev):
         # a buffer of this call's own: the allocator hands it on in stream order, and a captured
         # graph keeps its copy
-        ws = torch.empty(L.pb_verify_ws_bytes(R, S, V, code), dtype=torch.uint8, device=dev)
+        kinds = _kinds(params, V)
+        ws = torch.empty(L.pb_verify_ws_bytes(R, S, V, code, kinds), dtype=torch.uint8, device=dev)
         rc = L.pb_verify(
             logits.data_ptr(), code, R, V, logits.stride(0) if R > 1 else V, params.data_ptr(), S,
             row_offsets.data_ptr(), drafts.data_ptr(), uniforms.data_ptr(),
             draft_probs.data_ptr() if draft_probs is not None and R > S else None,
             ops._DTYPE_CODE[draft_probs.dtype] if draft_probs is not None else 0, R - S,
-            draft_probs.stride(0) if draft_probs is not None and R - S > 1 else V, _kinds(params, V),
+            draft_probs.stride(0) if draft_probs is not None and R - S > 1 else V, kinds,
             tokens.data_ptr(), accepted.data_ptr(), status.data_ptr(), ws.data_ptr(), ws.numel(),
             torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(rc, "pb_verify")

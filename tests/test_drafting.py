@@ -96,18 +96,18 @@ def test_c_abi_refusals(lib):
     def verify(**kw):
         a = dict(logits=base, dtype=0, n_rows=2, vocab=8, stride=8, params=base, n_seqs=1, offsets=base, drafts=base,
                  uniforms=base, probs=None, pdtype=0, n_probs=1, pstride=8, kinds=0, tokens=base, accepted=base, status=None,
-                 ws=base, ws_bytes=lib.pb_verify_ws_bytes(2, 1, 8, 0), stream=None) | kw
+                 ws=base, ws_bytes=lib.pb_verify_ws_bytes(2, 1, 8, 0, 0), stream=None) | kw
         return lib.pb_verify(*a.values())
 
     for kw in (dict(dtype=9), dict(n_rows=-1), dict(vocab=0), dict(stride=7), dict(logits=None), dict(params=None),
                dict(offsets=None), dict(drafts=None), dict(uniforms=None), dict(tokens=None), dict(accepted=None),
-               dict(ws=None), dict(ws=base + 8), dict(ws_bytes=0), dict(n_seqs=0), dict(n_seqs=3), dict(kinds=8),
+               dict(ws=None), dict(ws=base + 8), dict(ws_bytes=0), dict(n_seqs=0), dict(n_seqs=3), dict(kinds=16),
                dict(kinds=-1), dict(probs=base, pdtype=5), dict(probs=base, pstride=7), dict(probs=base + 1),
                dict(logits=base + 2)):
         assert verify(**kw) == -1, kw
     assert verify(vocab=1 << 24, stride=1 << 24) == -2
     assert verify(n_rows=0, n_seqs=0) == 0
-    assert lib.pb_verify_ws_bytes(-1, 1, 8, 0) == -1 and lib.pb_verify_ws_bytes(1, 1, 8, 7) == -1
+    assert lib.pb_verify_ws_bytes(-1, 1, 8, 0, 0) == -1 and lib.pb_verify_ws_bytes(1, 1, 8, 7, 0) == -1 and lib.pb_verify_ws_bytes(1, 1, 8, 0, 16) == -1
 
     def top(**kw):
         a = dict(logits=base, dtype=0, n_rows=2, vocab=8, stride=8, k=2, t=1.0, lp=base, idx=base, lse=base, ws=base, ws_bytes=1 << 20, stream=None) | kw
@@ -151,9 +151,9 @@ def test_kinds_of_sequences():
     assert kinds([0.0, 1.0], [1.0, 0.9], [0, 50]) == (_lib.VERIFY_SMALL, 50)
     assert kinds([1.0], [1.0], [0]) == (_lib.VERIFY_WHOLE, 0)
     assert kinds([1.0], [1.0 - 1e-12], [0]) == (_lib.VERIFY_WHOLE, 0)  # rounds to 1 in fp32: no filter
-    assert kinds([1.0], [0.9], [0]) == (_lib.VERIFY_OTHER, 0)
+    assert kinds([1.0], [0.9], [0]) == (_lib.VERIFY_TOPP, 0)
     assert kinds([1.0], [1.0], [129]) == (_lib.VERIFY_OTHER, 129)
-    assert kinds([0.0, 1.0, 1.0], [1.0, 1.0, 0.5], [0, 0, 0]) == (_lib.VERIFY_ANY, 0)
+    assert kinds([0.0, 1.0, 1.0, 1.0], [1.0, 1.0, 0.5, 1.0], [0, 0, 0, 500]) == (_lib.VERIFY_ANY, 500)
     assert kinds([-1.0], [1.0], [0])[0] == _lib.VERIFY_OTHER
 
 

@@ -150,6 +150,40 @@ def test_flat_rows(cuda):
     _check(x, params, lens, _drafts(x, lens, 5), u)
 
 
+def test_kinds_named_wrongly(cuda):
+    """A kind that the params' note leaves out is not settled (status 8), and nothing else is disturbed."""
+    S, V = 12, 1000
+    x = workloads.head_boosted(S, V, seed=1)
+    params = [((0.0, 1.0, 0), (1.0, 1.0, 0), (1.0, 0.9, 0), (1.0, 1.0, 500))[i % 4] for i in range(S)]
+    d, off = torch.zeros(S, dtype=torch.int64).cuda(), _offsets([0] * S)
+    u = np.random.default_rng(1).random(S)
+    want, _, _ = oracle.verify.verify(x, params, [0] * S, np.zeros(S, np.int64), u)
+    bit = [_lib.VERIFY_SMALL, _lib.VERIFY_WHOLE, _lib.VERIFY_TOPP, _lib.VERIFY_OTHER]
+    for kinds in range(1, 16):
+        pt = _params(params)
+        pt._pb_kinds = (kinds, 0)
+        tok, _, st = pb.verify(x.cuda(), pt, d, off, torch.from_numpy(u).cuda(), with_status=True)
+        for i in range(S):
+            # (the launch for other kinds takes top-p rows too)
+            named = kinds & bit[i % 4] or (i % 4 == 2 and kinds & _lib.VERIFY_OTHER)
+            assert (tok[i] == want[i] and st[i] == 0) if named else (tok[i] == -1 and st[i] == _lib.ROW_INTERNAL)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_top_p_steps(cuda, dtype):
+    """Top-p cuts in every part of a row: near the top, in the body, at the end, among many equals, in
+    rows so flat that one step of the histogram holds them, and with temperatures at the ends."""
+    V = 20011
+    rows = [workloads.head_boosted(6, V, seed=1), workloads.flat(4, V, seed=2), torch.zeros(2, V),
+            workloads.head_boosted(4, V, seed=3).round(), workloads.head_boosted(4, V, seed=4) * 1e-3]
+    x = torch.cat(rows).to(dtype)
+    S = len(x)
+    for k, p in enumerate((1e-6, 0.1, 0.5, 0.9, 0.999, 1.0 - 1e-7)):
+        params = [((1.0, 0.3, 2.5, 1e-3)[(i + k) % 4], p, 0) for i in range(S)]
+        u = np.random.default_rng(k).random(S)
+        _check(x, params, [0] * S, np.zeros(S, np.int64), u)
+
+
 def test_strides_and_offsets(cuda):
     """Rows that start anywhere, rows apart, and draft distributions with rows apart."""
     S, V = 9, 1003
