@@ -426,19 +426,23 @@ __global__ void __launch_bounds__(VT, 4) gather_kernel(VerifyArgs a) {
   if (a.one_kind != ROW_MASS) load_segment(rv, v0, v1, q);
   const Scale scaled(meta.t);
   const float m = a.info[row].max_key;
-  // raw values that are surely below the step
+  // raw values that are surely below the step, or above it
   const float raw_lo = surely_below(key_of(m - ((float)meta.step + 1.5f) / STEP_SCALE), meta.t);
+  const float above = (m - ((float)meta.step - 0.5f) / STEP_SCALE) * meta.t;
+  const float raw_hi = above + fabsf(above) * 0x1p-20f + 0x1p-100f;  // (NaN or infinite: no bound)
 #pragma unroll
   for (int i = 0; i < SEG_V; ++i) {
     if (!(vec_max_nan<T>(q[i]) >= raw_lo)) continue;
     float x[EPV];
     Elem<T>::unpack(q[i], x);
+    uint32_t near = 0;
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) near |= (x[j] >= raw_lo && !(x[j] > raw_hi) ? 1u : 0u) << j;
     const int32_t e0 = rv.first(v0 + i * SEG_T + (int32_t)threadIdx.x);
-#pragma unroll 1
-    for (int j = 0; j < EPV; ++j) {
-      const float xj = Elem<T>::elem(q[i], j);
-      if (!(xj >= raw_lo)) continue;
-      const float y = scaled(xj);
+    while (near) {
+      const int j = __ffs(near) - 1;
+      near &= near - 1;
+      const float y = scaled(Elem<T>::elem(q[i], j));
       if (e0 + j < 0 || e0 + j >= a.V || step_of(y, m) != meta.step || !weight_q(y, m)) continue;
       const uint32_t at = atomicAdd(&a.meta[row].listed, 1u);
       if (at < (uint32_t)LIST) a.list[row * LIST + at] = compose(key_of(y), (uint32_t)(e0 + j));
@@ -532,7 +536,7 @@ struct DrawRow {
   Scale scaled;
   Weigher weigh;
   double z;          // mass, in the weights' own scale
-  float d_most;      // draft probabilities above this take all of any weight
+  float d_most;      // draft probabilities above this take all of any weight, and stay on the grid below
   int64_t dx, drow;  // the rejected draft; its row of draft_probs
   bool residual, dist, cut_ties, whole;
   float raw_lo, thr;  // (a key's order is its value's: the row holds no NaN)
@@ -560,11 +564,12 @@ struct DrawRow {
 #pragma unroll
     for (int q = 0; q < EPV / 4; ++q) d[q] = __ldg(p + q);
   }
-  // GRID + floor(d * Z): NaN and what is below 0 take nothing
+  // GRID + floor(d * Z): NaN and what is below 0 take nothing. (Beyond the grid the floor is coarser,
+  // and more than any weight all the same.)
   __device__ __forceinline__ double taken_by(float d) const {
-    return __dadd_rd(GRID, __dmul_rn((double)fminf(fmaxf(d, 0.0f), d_most), z));
+    return __dadd_rd(GRID, __dmul_rn((double)fmaxf(d, 0.0f), z));
   }
-  // max(p - taken, 0), by the sign bit of the (exact) difference
+  // max(p - taken, 0), by the sign bit of the difference (exact where it is not negative)
   static __device__ __forceinline__ double leaves(double p, double taken) {
     const long long r = __double_as_longlong(p - taken);
     return __longlong_as_double(r & ~(r >> 63));
@@ -748,7 +753,7 @@ __device__ int32_t draw_listed(const DrawRow<T>& row, const GroupKeys& g, int64_
     if (p[j]) {
       const int32_t e = sh.index[i0 + j];
       uint64_t taken = 0;
-      if (row.dist) taken = grid_units(row.taken_by(prob_at(row.a, row.drow, e)));
+      if (row.dist) taken = grid_units(row.taken_by(fminf(prob_at(row.a, row.drow, e), row.d_most)));
       else if (row.residual && e == row.dx) taken = p[j];
       r[j] = p[j] > taken ? p[j] - taken : 0;
     }
@@ -1016,12 +1021,14 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
 
 // ---- drawing ---------------------------------------------------------------------------------
 
-// CTA (sequence, segment): the sums of the segment's tiles.
+// CTA (sequence, segment): the sums of the segment's tiles. Every thread leaves its own sum of each
+// tile in shared memory; the warps then take a tile each.
 template <typename T>
 __global__ void __launch_bounds__(VT, 3) weigh_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
-  __shared__ uint64_t w[VNW][TILES], tw[VNW][TILES];
-  __shared__ int32_t tn[VNW][TILES];
+  static_assert(TILES == VNW, "a warp per tile");
+  __shared__ double part[TILES][VT], tie_part[TILES][VT];
+  __shared__ uint8_t ties[TILES][VT];
   grid_release();
   grid_wait();
   const int64_t seq = blockIdx.x;
@@ -1029,73 +1036,77 @@ __global__ void __launch_bounds__(VT, 3) weigh_kernel(VerifyArgs a) {
   if (!d.draws) return;
   const pb_row_info f = a.info[d.row];
   const DrawRow<T> row(a, seq, d, (float)a.params[seq].temperature, f);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(row.rv.nvec, v0 + a.seg.per);
-  // one vector (and its draft probabilities) is on its way while the one before it is weighed; those
-  // of a whole row's draft distribution are all needed, others only where the target has weight
+  // one vector (and its draft probabilities) is on its way while the one before it is weighed
   const uint32_t none = Elem<T>::NEG_INF_WORD;
   const uint4 nothing = make_uint4(none, none, none, none);
   uint4 next = nothing;
   float4 next_d[EPV / 4];
   bool next_have = false;
   auto fetch = [&](int i) {
-    const int32_t v = v0 + i * SEG_T + (int32_t)threadIdx.x;
+    const int32_t v = v0 + i * SEG_T + tid;
     next = nothing;
     next_have = false;
-    if (i < SEG_V && v < v1) {
+    if (i < TILES && v < v1) {
       next = load_vec(row.rv, v);
-      next_have = row.whole && row.packed_probs(v);
+      next_have = row.packed_probs(v);
       if (next_have) row.load_probs(v, next_d);
     }
   };
   fetch(0);
 #pragma unroll 1
-  for (int i = 0; i < SEG_V; ++i) {
-    if (i * SEG_T >= v1 - v0) {
-      if (lane == 0) w[warp][i] = tw[warp][i] = 0, tn[warp][i] = 0;
-      continue;
-    }
+  for (int i = 0; i < TILES; ++i) {
     const uint4 qi = next;
     float4 di[EPV / 4];
 #pragma unroll
     for (int j = 0; j < EPV / 4; ++j) di[j] = next_d[j];
     const bool have = next_have;
     fetch(i + 1);
-    double r[EPV], sum = 0.0, tsum = 0.0;
-    uint32_t eq;
-    row.of(v0 + i * SEG_T + (int32_t)threadIdx.x, qi, false, have, di, r, eq);
-    if (eq) {
+    double sum = 0.0, tsum = 0.0;
+    uint32_t eq = 0;
+    if (have && row.whole) {  // the common case of a whole row: every element counts
+      float w[EPV], y[EPV];
+      row.weigh.template of<T>(qi, w, y);
+#pragma unroll
+      for (int j = 0; j < EPV; j += 4) {
+        sum += row.leaves(on_grid(w[j]), row.taken_by(di[j / 4].x));
+        sum += row.leaves(on_grid(w[j + 1]), row.taken_by(di[j / 4].y));
+        sum += row.leaves(on_grid(w[j + 2]), row.taken_by(di[j / 4].z));
+        sum += row.leaves(on_grid(w[j + 3]), row.taken_by(di[j / 4].w));
+      }
+    } else if (v0 + i * SEG_T + tid < v1) {
+      double r[EPV];
+      row.of(v0 + i * SEG_T + tid, qi, false, have, di, r, eq);
 #pragma unroll
       for (int j = 0; j < EPV; ++j) {
         if ((eq >> j) & 1u) tsum += r[j];
         else sum += r[j];
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < EPV; ++j) sum += r[j];
     }
-    uint64_t s = warp_sum(units(sum)), t = 0;
-    int32_t n = 0;
+    part[i][tid] = sum;
     if (row.cut_ties) {
-      t = warp_sum(units(tsum));
-      n = __reduce_add_sync(0xFFFFFFFFu, __popc(eq));
-    }
-    if (lane == 0) {
-      w[warp][i] = s;
-      tw[warp][i] = t;
-      tn[warp][i] = n;
+      tie_part[i][tid] = tsum;
+      ties[i][tid] = (uint8_t)__popc(eq);
     }
   }
   __syncthreads();
-  if (threadIdx.x < TILES) {
-    Tile t{0, 0, 0, 0};
-    for (int k = 0; k < VNW; ++k) {
-      t.w += w[k][threadIdx.x];
-      t.tie_w += tw[k][threadIdx.x];
-      t.ties += tn[k][threadIdx.x];
+  Tile t{0, 0, 0, 0};
+  double sum = 0.0, tsum = 0.0;  // (64 weights of at most 1)
+#pragma unroll
+  for (int j = 0; j < VT / 32; ++j) {
+    sum += part[warp][j * 32 + lane];
+    if (row.cut_ties) {
+      tsum += tie_part[warp][j * 32 + lane];
+      t.ties += ties[warp][j * 32 + lane];
     }
-    a.tiles[(seq * a.seg.segs + blockIdx.y) * TILES + threadIdx.x] = t;
   }
+  t.w = warp_sum(units(sum));
+  if (row.cut_ties) {
+    t.tie_w = warp_sum(units(tsum));
+    t.ties = __reduce_add_sync(0xFFFFFFFFu, t.ties);
+  }
+  if (lane == 0) a.tiles[(seq * a.seg.segs + blockIdx.y) * TILES + warp] = t;
 }
 
 struct DrawShared {
