@@ -19,56 +19,47 @@ __all__ = ["distill_loss"]
 STATS = 32  # bytes of a row's statistics (pb_distill_stats_bytes)
 
 
-class _Rows:
-    """The arguments of one call: student rows, teacher entries, row weights."""
+def _arguments(z, lp, idx, temperature):
+    """What the forward and the backward call have in common."""
+    n, V = z.shape
+    return (z.data_ptr(), ops._DTYPE_CODE[z.dtype], n, V, z.stride(0), lp.data_ptr(), lp.stride(0), idx.data_ptr(),
+            idx.stride(0), 8 if idx.dtype == torch.int64 else 4, idx.shape[1], temperature)
 
-    __slots__ = ("z", "lp", "idx", "weight", "temperature", "args")
 
-    def __init__(self, z, lp, idx, weight, temperature):
-        self.z, self.lp, self.idx, self.weight, self.temperature = z, lp, idx, weight, temperature
-        self.args = (z.data_ptr(), ops._DTYPE_CODE[z.dtype], z.shape[0], z.shape[1], z.stride(0), lp.data_ptr(),
-                     lp.stride(0), idx.data_ptr(), idx.stride(0), idx.element_size(), idx.shape[1], temperature)
+def _forward(z, lp, idx, weight, temperature, tail, total):
+    """The rows' losses (or their sum), and a buffer that starts with their statistics."""
+    L = _lib.load()
+    dev = z.device
+    args = _arguments(z, lp, idx, temperature)
+    n = args[2]
+    n_ws = L.pb_distill_ws_bytes(n, args[3], args[1])
+    buf = torch.empty(n * STATS + n_ws, dtype=torch.uint8, device=dev)  # statistics, then the launch's own workspace
+    loss = torch.empty(n, dtype=torch.float32, device=dev)
+    base, stream = buf.data_ptr(), ops.raw_stream(dev)
+    with ops.on_device(dev):
+        _lib.check(L.pb_distill_forward(*args, tail, None if weight is None else weight.data_ptr(), loss.data_ptr(), base,
+                                        base + n * STATS, n_ws, stream), "pb_distill_forward")
+        if total:
+            rows, loss = loss, torch.empty((), dtype=torch.float32, device=dev)
+            _lib.check(L.pb_distill_sum(rows.data_ptr(), n, loss.data_ptr(), stream), "pb_distill_sum")
+    return loss, buf
 
-    def weight_ptr(self):
-        return None if self.weight is None else self.weight.data_ptr()
 
-    def forward(self, tail, total=False):
-        """The rows' losses (or their sum) and statistics."""
-        z = self.z
-        n, V = z.shape
-        L = _lib.load()
-        n_ws = L.pb_distill_ws_bytes(n, V, self.args[1])
-        # one buffer: statistics, losses, and the launch's own workspace
-        keep = n * (STATS + 4)
-        buf = torch.empty(-(-keep // 16) * 16 + n_ws, dtype=torch.uint8, device=z.device)
-        loss = buf[n * STATS : keep].view(torch.float32)
-        with ops.on_device(z.device):
-            stream = torch.cuda.current_stream(z.device).cuda_stream
-            base = buf.data_ptr()
-            rc = L.pb_distill_forward(*self.args, int(tail), self.weight_ptr(), base + n * STATS, base,
-                                      base + buf.numel() - n_ws, n_ws, stream)
-            _lib.check(rc, "pb_distill_forward")
-            if total:
-                loss = torch.empty((), dtype=torch.float32, device=z.device)
-                _lib.check(L.pb_distill_sum(base + n * STATS, n, loss.data_ptr(), stream), "pb_distill_sum")
-        return loss, buf
-
-    def backward(self, stats, grad_loss):
-        z = self.z
-        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        with ops.on_device(z.device):
-            rc = _lib.load().pb_distill_backward(
-                *self.args, self.weight_ptr(), stats.data_ptr(), grad_loss.data_ptr(),
-                grad_loss.stride(0) if grad_loss.dim() else 0, dz.data_ptr(),
-                torch.cuda.current_stream(z.device).cuda_stream)
-        _lib.check(rc, "pb_distill_backward")
-        return dz
+def _backward(z, lp, idx, weight, stats, temperature, grad_loss):
+    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    # a gradient of one value for all rows (from a sum or mean) is read through its stride of 0
+    with ops.on_device(z.device):
+        _lib.check(_lib.load().pb_distill_backward(
+            *_arguments(z, lp, idx, temperature), None if weight is None else weight.data_ptr(), stats.data_ptr(),
+            grad_loss.data_ptr(), grad_loss.stride(0) if grad_loss.dim() else 0, dz.data_ptr(), ops.raw_stream(z.device)),
+            "pb_distill_backward")
+    return dz
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, lp, idx, weight, temperature, tail, total):
-        loss, stats = _Rows(z, lp, idx, weight, temperature).forward(tail, total)
+        loss, stats = _forward(z, lp, idx, weight, temperature, tail, total)
         ctx.save_for_backward(z, lp, idx, weight, stats)
         ctx.temperature = temperature
         return loss
@@ -76,9 +67,7 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss):
-        z, lp, idx, weight, stats = ctx.saved_tensors
-        # a gradient of one value for all rows (from a sum or mean) is read through its stride of 0
-        dz = _Rows(z, lp, idx, weight, ctx.temperature).backward(stats, grad_loss)
+        dz = _backward(*ctx.saved_tensors, ctx.temperature, grad_loss)
         return dz, None, None, None, None, None, None
 
 
@@ -119,13 +108,14 @@ def distill_loss(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, t
         raise ValueError("the teacher's entries and the row weights take no gradient: detach them")
     if row_weight is not None and (row_weight.dtype != torch.float32 or row_weight.shape != (n,)):
         raise ValueError(f"row_weight must be a float32 tensor of {n} values")
-    for name, t in (("teacher_logprobs", lp), ("teacher_indices", idx), ("row_weight", row_weight)):
-        if t is not None and t.device != z.device:
-            raise ValueError(f"{name} must be on the logits' device {z.device}")
+    dev = z.device
+    if lp.device != dev or idx.device != dev or (row_weight is not None and row_weight.device != dev):
+        raise ValueError(f"the teacher's entries and the row weights must be on the logits' device {dev}")
     if reduction not in ("none", "sum"):
         raise ValueError(f"reduction must be 'none' or 'sum', got {reduction!r}")
     t = check_temperature(temperature)
-    lp = lp.float()
+    if lp.dtype != torch.float32:
+        lp = lp.float()
     if lp.stride(1) != 1:
         lp = lp.contiguous()
     if idx.stride(1) != 1:
@@ -134,5 +124,5 @@ def distill_loss(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, t
         row_weight = row_weight.contiguous()
     total = reduction == "sum"
     if not (z.requires_grad and torch.is_grad_enabled()):
-        return _Rows(z, lp, idx, row_weight, t).forward(tail, total)[0]
+        return _forward(z, lp, idx, row_weight, t, bool(tail), total)[0]
     return _Distill.apply(z, lp, idx, row_weight, t, bool(tail), total)

@@ -49,10 +49,10 @@ def _launch(logits: torch.Tensor, k: int, temperature: float):
     L = _lib.load()
     with ops.on_device(dev):
         code = ops._DTYPE_CODE[logits.dtype]
-        ws = torch.empty(L.pb_top_ws_bytes(n, V, code), dtype=torch.uint8, device=dev)
+        n_ws = L.pb_top_ws_bytes(n, V, code)
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
         rc = L.pb_top_logprobs(logits.data_ptr(), code, n, V, logits.stride(0), k, t, lp.data_ptr(), idx.data_ptr(),
-                               lse.data_ptr(), ws.data_ptr(), ws.numel(),
-                               torch.cuda.current_stream(dev).cuda_stream)
+                               lse.data_ptr(), ws.data_ptr(), n_ws, ops.raw_stream(dev))
     _lib.check(rc, "pb_top_logprobs")
     return lp, idx, lse
 

@@ -47,6 +47,12 @@ def pack_params(temperature, top_p, top_k, uniform, seeds=None, steps=None) -> n
     return rec
 
 
+def raw_stream(dev: torch.device) -> int:
+    """The handle of ``dev``'s current stream (torch's own accessor behind ``current_stream``, without
+    the Python object around it)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 class on_device:
     """``torch.cuda.device(dev)``, at no cost where ``dev`` is the current device already."""
 

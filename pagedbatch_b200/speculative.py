@@ -45,12 +45,10 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs):
     S = params.numel() // _lib.ROW_PARAMS.itemsize
     for name, t, dtype, n in (("drafts", drafts, torch.int64, R), ("row_offsets", row_offsets, torch.int32, S + 1),
                               ("uniforms", uniforms, torch.float64, R)):
-        if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values")
-    for name, t in (("params", params), ("drafts", drafts), ("row_offsets", row_offsets), ("uniforms", uniforms),
-                    ("draft_probs", draft_probs)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} must be on the logits' device {dev}")
+        if t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values on the logits' device {dev}")
+    if params.device != dev or (draft_probs is not None and draft_probs.device != dev):
+        raise ValueError(f"params and draft_probs must be on the logits' device {dev}")
     if S > R:
         raise ValueError(f"{S} sequences for {R} rows: every sequence has at least one row")
     if draft_probs is not None:
@@ -71,15 +69,15 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs):
         # a buffer of this call's own: the allocator hands it on in stream order, and a captured
         # graph keeps its copy
         kinds = _kinds(params, V)
-        ws = torch.empty(L.pb_verify_ws_bytes(R, S, V, code, kinds), dtype=torch.uint8, device=dev)
+        n_ws = L.pb_verify_ws_bytes(R, S, V, code, kinds)
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
         rc = L.pb_verify(
             logits.data_ptr(), code, R, V, logits.stride(0) if R > 1 else V, params.data_ptr(), S,
             row_offsets.data_ptr(), drafts.data_ptr(), uniforms.data_ptr(),
             draft_probs.data_ptr() if draft_probs is not None and R > S else None,
             ops._DTYPE_CODE[draft_probs.dtype] if draft_probs is not None else 0, R - S,
             draft_probs.stride(0) if draft_probs is not None and R - S > 1 else V, kinds,
-            tokens.data_ptr(), accepted.data_ptr(), status.data_ptr(), ws.data_ptr(), ws.numel(),
-            torch.cuda.current_stream(dev).cuda_stream)
+            tokens.data_ptr(), accepted.data_ptr(), status.data_ptr(), ws.data_ptr(), n_ws, ops.raw_stream(dev))
     _lib.check(rc, "pb_verify")
     return tokens, accepted, status
 
