@@ -130,6 +130,39 @@ def test_many_rows(cuda, tail):
 
 
 @pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype,V,K", [(torch.float32, 1, 1), (torch.float32, 7, 3), (torch.float16, 1003, 40),
+                                       (torch.bfloat16, 4096, 1000), (torch.float32, 50021, 33), (torch.float32, 65533, 20),
+                                       (torch.bfloat16, 128256, 64), (torch.float16, 131057, 64)])
+def test_sums_of_many_rows(cuda, tail, dtype, V, K):
+    """A sum over more rows than the device has SMs, with rows that do not count and entries that repeat;
+    then scaled, and once more."""
+    n = 150 if V > 20000 else 333
+    z = torch.randn(n, V, generator=torch.Generator().manual_seed(V)).to(dtype) * 2
+    lp, idx = entries(z, K, 1)
+    if K > 4:
+        idx[5:9, 2:4] = idx[5:9, :1]
+        idx[10, ::3] = idx[10, 1]
+    w = torch.rand(n, generator=torch.Generator().manual_seed(1)) + 0.25
+    w[3], w[149] = 0.0, 0.0
+    z[3, 0] = torch.nan
+    z[n - 1, V // 2] = -torch.inf if V > 1 else 0.0
+    loss64, grad64, l_err, g_err = formula(z, lp, idx, 1.25, tail, w)
+    dev = z.cuda().requires_grad_()
+    loss = pb.distill_loss(dev, lp.cuda(), idx.cuda(), temperature=1.25, tail=tail, row_weight=w.cuda(), reduction="sum")
+    if torch.isinf(loss64).any():  # (the masked logit was an entry's)
+        assert loss.item() == float("inf")
+    else:
+        assert abs(loss.item() - float(loss64.sum())) <= float(l_err.sum()) + U * n * float(loss64.abs().sum())
+    f = torch.finfo(dtype)
+    for scale in (1.0, 1.0, 0.375, 0.0):
+        (g,) = torch.autograd.grad(loss * scale, dev, retain_graph=True)
+        want = grad64 * scale
+        lim = g_err * scale + (f.eps / 2) * want.abs() * 1.01 + f.smallest_normal * f.eps
+        d = (g.cpu().double() - want).abs()
+        assert (d <= lim).all(), (scale, (d - lim).max(), (d > lim).nonzero()[:4])
+
+
+@pytest.mark.parametrize("tail", [False, True])
 def test_gradient_against_differences(cuda, tail):
     z = workloads.head_boosted(3, 500, seed=3).double().float()
     lp, idx = entries(z, 12, 4, short=False)
