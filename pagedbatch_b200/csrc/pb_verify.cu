@@ -109,6 +109,7 @@ __device__ __forceinline__ int32_t row_kind(const pb_row_params& p, int32_t V) {
 }
 
 __global__ void __launch_bounds__(256) expand_kernel(VerifyArgs a) {
+  grid_release();
   const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (r >= a.n_rows) return;
   int64_t lo = 0, hi = a.n_seqs;  // the last sequence that starts at or before row r
@@ -552,7 +553,7 @@ struct DrawRow {
     raw_lo = surely_below(f.thr_key, tf);
     thr = value_of(f.thr_key);
     z = __ull2double_rn(f.kept_q) * 0x1p-40;
-    d_most = (float)(2048.0 / z);
+    d_most = 2048.0f / (float)z;  // (anywhere between 1 / Z and 4095 / Z would do)
   }
   // The draft's probabilities of a whole vector, where they can be loaded as vectors of their own.
   __device__ __forceinline__ bool packed_probs(int32_t v) const {
@@ -686,96 +687,164 @@ __device__ __forceinline__ void each_near(const GroupKeys& g, const RowView<T>& 
   }
 }
 
-constexpr int NEAR_CAP = 1024;  // listed elements of a row drawn from by one CTA
+constexpr int NEAR_CAP = 256;   // listed elements of a row drawn from by one CTA
+constexpr int NEAR_GROUPS = 512;  // ... and the groups they are looked for in
 struct NearShared {
   uint64_t scan[VNW + 1];
   uint32_t tscan[VNW + 1];
-  int32_t index[NEAR_CAP];
-  float value[NEAR_CAP];
+  uint32_t n, groups;
+  int32_t group[NEAR_GROUPS];
+  int32_t index[NEAR_CAP], sorted[NEAR_CAP];
+  float value[NEAR_CAP], sorted_value[NEAR_CAP];
+  int32_t found;
+  bool none;
 };
 
+// The values of a row at or above raw_lo (finite), by its group keys: the CTA lists the groups whose
+// largest value is, then the values, in any order. Returns their number, or -1 where a list is too
+// short for the row. (Few instructions, each run once: one CTA a sequence waits for code as for data.)
+template <typename T>
+__device__ int32_t list_near(const RowView<T>& rv, const GroupKeys& g, int64_t at_row, float raw_lo, NearShared& sh) {
+  constexpr int EPV = Elem<T>::EPV;
+  const int tid = threadIdx.x;
+  if (tid == 0) sh.n = sh.groups = 0;
+  __syncthreads();
+  constexpr int GV = 8;  // vectors of a group (such rows start on a 16-byte boundary)
+  const uint32_t lo = key_of(raw_lo);
+  const uint32_t* keys = g.keys + at_row * g.stride;
+  for (int32_t k0 = tid; k0 < g.groups; k0 += VT * 16) {
+    uint32_t hits = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (k0 + i * VT < g.groups) hits |= (__ldcg(keys + k0 + i * VT) >= lo ? 1u : 0u) << i;
+    while (hits) {
+      const uint32_t at = atomicAdd(&sh.groups, 1u);
+      if (at < (uint32_t)NEAR_GROUPS) sh.group[at] = k0 + (__ffs(hits) - 1) * VT;
+      hits &= hits - 1;
+    }
+  }
+  __syncthreads();
+  const int32_t nv = (int32_t)min(sh.groups, (uint32_t)NEAR_GROUPS) * GV;
+  if (sh.groups > (uint32_t)NEAR_GROUPS) return -1;
+  constexpr int AHEAD = 4;  // vectors a thread has in flight
+  for (int32_t i0 = tid; i0 < nv; i0 += VT * AHEAD) {
+    uint4 q[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int32_t i = i0 + u * VT, v = i < nv ? sh.group[i / GV] * GV + i % GV : rv.nvec;
+      const uint32_t none_word = Elem<T>::NEG_INF_WORD;
+      q[u] = make_uint4(none_word, none_word, none_word, none_word);
+      if (v < rv.nvec) q[u] = load_vec(rv, v);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (!(vec_max_nan<T>(q[u]) >= raw_lo)) continue;
+      const int32_t i = i0 + u * VT, e0 = rv.first(sh.group[i / GV] * GV + i % GV);
+#pragma unroll 1
+      for (int j = 0; j < EPV; ++j) {
+        const float x = Elem<T>::elem(q[u], j);
+        if (!(x >= raw_lo)) continue;  // (elements past the row are -inf, and raw_lo is finite)
+        const uint32_t at = atomicAdd(&sh.n, 1u);
+        if (at < (uint32_t)NEAR_CAP) {
+          sh.index[at] = e0 + j;
+          sh.value[at] = x;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  return sh.n <= (uint32_t)NEAR_CAP ? (int32_t)sh.n : -1;
+}
+
 // The draw over a row whose group keys are known, for rows with few values near the kept ones (as all
-// but odd rows of top-k have): one CTA lists the values that may be kept, in index order (each thread
-// looks through a run of consecutive groups), and weighs the listed ones. Returns the token in the
-// thread that finds it, -1 in the others; false in *fits where the list is too short for the row.
+// but odd rows of top-k have): the listed values are put in index order by counting, then one warp
+// weighs them, which needs no more barriers. Returns the token (every thread), -1 where there is no
+// weight at all; false in *fits where the list is too short for the row.
 template <typename T>
 __device__ int32_t draw_listed(const DrawRow<T>& row, const GroupKeys& g, int64_t at_row, uint64_t u53, NearShared& sh,
                                bool* fits, bool* none) {
-  constexpr int EPV = Elem<T>::EPV, PER = NEAR_CAP / VT;
-  uint32_t mine = 0, n;
-  each_near<T>(g, row.rv, at_row, row.raw_lo, [&](int32_t, uint4 q) {
-    float x[EPV];
-    Elem<T>::unpack(q, x);
-#pragma unroll
-    for (int j = 0; j < EPV; ++j) mine += x[j] >= row.raw_lo;
-  });
-  uint32_t at = block_prefix(mine, sh.tscan, &n);
-  *fits = n <= (uint32_t)NEAR_CAP;
+  constexpr int PER = NEAR_CAP / 32;
+  const int tid = threadIdx.x;
+  const int32_t n = list_near(row.rv, g, at_row, row.raw_lo, sh);
   *none = false;
-  if (!*fits) return -1;
-  if (mine)
-    each_near<T>(g, row.rv, at_row, row.raw_lo, [&](int32_t v, uint4 q) {
-      float x[EPV];
-      Elem<T>::unpack(q, x);
-#pragma unroll
-      for (int j = 0; j < EPV; ++j)
-        if (x[j] >= row.raw_lo) {  // (elements past the row are -inf, and raw_lo is finite)
-          sh.index[at] = row.rv.first(v) + j;
-          sh.value[at++] = x[j];
-        }
-    });
-  __syncthreads();
-  // entries tid * per .. of the list: target weights, equals of the last kept key, what is left
-  const uint32_t per = (n + VT - 1) / VT, i0 = threadIdx.x * per;
-  uint64_t p[PER], r[PER];
-  uint32_t eq = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    p[j] = r[j] = 0;
-    if ((uint32_t)j < per && i0 + j < n) {
-      const float y = row.scaled(sh.value[i0 + j]);
-      if (y >= row.thr) p[j] = weight_q(y, row.f.max_key);
-      if (row.cut_ties && y == row.thr) eq |= 1u << j;
-    }
+  *fits = n >= 0;
+  if (n < 0) return -1;
+  if (tid < n) {
+    const int32_t e = sh.index[tid];
+    int32_t before = 0;
+    for (int32_t j = 0; j < n; ++j) before += sh.index[j] < e ? 1 : 0;
+    sh.sorted[before] = e;
+    sh.sorted_value[before] = sh.value[tid];
   }
-  if (row.cut_ties) {
-    uint32_t total, before = block_prefix((uint32_t)__popc(eq), sh.tscan, &total);
+  __syncthreads();
+  if (tid < 32) {
+    // entries lane * per .. of the list: target weights, equals of the last kept key, what is left
+    const int32_t per = (n + 31) / 32, i0 = tid * per;
+    uint64_t p[PER], r[PER];
+    float d[PER];
+    uint32_t eq = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      p[j] = r[j] = 0;
+      d[j] = 0.0f;
+      if (j < per && i0 + j < n && row.dist) d[j] = prob_at(row.a, row.drow, sh.sorted[i0 + j]);
+    }
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if ((eq >> j) & 1u) {
-        if (before >= (uint32_t)row.f.n_tie_kept) p[j] = 0;
-        ++before;
+      if (j < per && i0 + j < n) {
+        const float y = row.scaled(sh.sorted_value[i0 + j]);
+        if (y >= row.thr) p[j] = weight_q(y, row.f.max_key);
+        if (row.cut_ties && y == row.thr) eq |= 1u << j;
       }
-  }
-  uint64_t sum = 0, all = 0, total;
+    if (row.cut_ties) {
+      const uint32_t mine = (uint32_t)__popc(eq);
+      uint32_t before = warp_incl_scan(mine) - mine;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    if (p[j]) {
-      const int32_t e = sh.index[i0 + j];
-      uint64_t taken = 0;
-      if (row.dist) taken = grid_units(row.taken_by(fminf(prob_at(row.a, row.drow, e), row.d_most)));
-      else if (row.residual && e == row.dx) taken = p[j];
-      r[j] = p[j] > taken ? p[j] - taken : 0;
+      for (int j = 0; j < PER; ++j)
+        if ((eq >> j) & 1u) {
+          if (before >= (uint32_t)row.f.n_tie_kept) p[j] = 0;
+          ++before;
+        }
     }
-    sum += r[j];
-    all += p[j];
-  }
-  uint64_t before = block_prefix(sum, sh.scan, &total);
-  const bool target = total == 0;  // an empty residual: drawn from the target itself
-  if (target) {
-    sum = all;
-    before = block_prefix(sum, sh.scan, &total);
-  }
-  *none = total == 0;
-  const uint64_t want = scale_u53(u53, total);
-  if (!(before <= want && want < before + sum)) return -1;
-  int32_t found = -1;
+    uint64_t sum = 0, all = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    before += target ? p[j] : r[j];
-    if (found < 0 && before > want) found = sh.index[i0 + j];
+    for (int j = 0; j < PER; ++j) {
+      if (p[j]) {
+        uint64_t taken = 0;
+        if (row.dist) taken = grid_units(row.taken_by(fminf(d[j], row.d_most)));
+        else if (row.residual && sh.sorted[i0 + j] == row.dx) taken = p[j];
+        r[j] = p[j] > taken ? p[j] - taken : 0;
+      }
+      sum += r[j];
+      all += p[j];
+    }
+    uint64_t incl = warp_incl_scan(sum), total = __shfl_sync(0xFFFFFFFFu, incl, 31);
+    const bool target = total == 0;  // an empty residual: drawn from the target itself
+    if (target) {
+      sum = all;
+      incl = warp_incl_scan(sum);
+      total = __shfl_sync(0xFFFFFFFFu, incl, 31);
+    }
+    if (tid == 0) {
+      sh.found = -1;
+      sh.none = total == 0;
+    }
+    __syncwarp();
+    const uint64_t want = scale_u53(u53, total);
+    uint64_t run = incl - sum;
+    if (run <= want && want < incl) {
+      int32_t found = -1;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        run += target ? p[j] : r[j];
+        if (found < 0 && run > want) found = sh.sorted[i0 + j];
+      }
+      sh.found = found;
+    }
   }
-  return found;
+  __syncthreads();
+  *none = sh.none;
+  return sh.found;
 }
 
 // The same draw for rows of any number of such values (very many equal ones): the runs are looked
@@ -953,7 +1022,11 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
     __syncthreads();
     uint32_t before = 0;
     const float lo_raw = surely_below(f.thr_key, tf);
-    if (a.groups.keys && row_is == ROW_SMALL) {
+    const bool keyed = a.groups.keys && row_is == ROW_SMALL;
+    const int32_t near = keyed && lo_raw > -INFINITY ? list_near(rv, a.groups, stop, lo_raw, near_sh) : -1;
+    if (near >= 0) {
+      if (tid < near) before = near_sh.index[tid] < x && key_of(scaled(near_sh.value[tid])) == f.thr_key;
+    } else if (keyed) {
       each_near<T>(a.groups, rv, stop, lo_raw, [&](int32_t v, uint4 q4) {
         float y[EPV];
         Elem<T>::unpack(q4, y);
@@ -1014,7 +1087,7 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
     int32_t found = -1;
     if (row.raw_lo > -INFINITY) found = draw_listed<T>(row, a.groups, stop, u53, near_sh, &fits, &none);
     if (!fits) found = draw_near<T>(row, a.groups, stop, u53, near_sh, &none);
-    if (found >= 0) a.out_tokens[stop] = found;
+    if (found >= 0 && (!fits || tid == 0)) a.out_tokens[stop] = found;
     if (none && tid == 0 && a.out_status) a.out_status[seq] = PB_ROW_INTERNAL;
   }
 }
@@ -1323,9 +1396,12 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
   expand_kernel<<<(unsigned)((a.n_rows + 255) / 256), 256, 0, st>>>(a);
   int rc = cudaGetLastError() == cudaSuccess ? PB_OK : PB_E_LAUNCH;
   if (rc == PB_OK && (kinds & PB_VERIFY_SMALL)) {
-    rc = pb_sample_ws(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr,
-                      ws + plan.sampler, plan.bytes - plan.sampler, st);
+    // the two-pass launch where the rows suit it, else pb_sample's own launches (the workspace's other
+    // launch cuts rows into pieces for large batches: 72 rows of 50021 fp16 take it 31 us, these 27 us)
     a.groups = sample_ws_keys(a.x, dtype, a.n_rows, a.V, a.row_stride, ws + plan.sampler, plan.bytes - plan.sampler);
+    rc = a.groups.keys ? pb_sample_ws(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr,
+                                      ws + plan.sampler, plan.bytes - plan.sampler, st)
+                       : pb_sample(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr, st);
   }
   if (rc == PB_OK && (kinds & (PB_VERIFY_WHOLE | PB_VERIFY_TOPP))) rc = launch_after(max_kernel<T>, a, rows, VT, st);
   if (rc == PB_OK && (kinds & PB_VERIFY_WHOLE)) rc = launch_after(mass_kernel<T>, a, rows, VT, st);
