@@ -1138,7 +1138,9 @@ __global__ void __launch_bounds__(VT, 3) weigh_kernel(VerifyArgs a) {
     fetch(i + 1);
     double sum = 0.0, tsum = 0.0;
     uint32_t eq = 0;
-    if (have && row.whole) {  // the common case of a whole row: every element counts
+    const int32_t at = v0 + i * SEG_T + tid, e0 = row.rv.first(at);
+    const bool simple = at < v1 && row.whole && row.rv.whole(at);  // every element of the vector counts
+    if (simple && have) {
       float w[EPV], y[EPV];
       row.weigh.template of<T>(qi, w, y);
 #pragma unroll
@@ -1148,9 +1150,19 @@ __global__ void __launch_bounds__(VT, 3) weigh_kernel(VerifyArgs a) {
         sum += row.leaves(on_grid(w[j + 2]), row.taken_by(di[j / 4].z));
         sum += row.leaves(on_grid(w[j + 3]), row.taken_by(di[j / 4].w));
       }
-    } else if (v0 + i * SEG_T + tid < v1) {
+    } else if (simple && !row.dist && !(row.dx >= e0 && row.dx < e0 + EPV)) {
+      float w[EPV], y[EPV];
+      row.weigh.template of<T>(qi, w, y);
+      double s0 = GRID, s1 = GRID;
+#pragma unroll
+      for (int j = 0; j < EPV; j += 2) {
+        s0 = __dadd_rd(s0, (double)w[j]);
+        s1 = __dadd_rd(s1, (double)w[j + 1]);
+      }
+      sum = (s0 - GRID) + (s1 - GRID);
+    } else if (at < v1) {
       double r[EPV];
-      row.of(v0 + i * SEG_T + tid, qi, false, have, di, r, eq);
+      row.of(at, qi, false, have, di, r, eq);
 #pragma unroll
       for (int j = 0; j < EPV; ++j) {
         if ((eq >> j) & 1u) tsum += r[j];
