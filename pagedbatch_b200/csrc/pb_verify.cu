@@ -204,9 +204,12 @@ struct Weigher {
       unpack2(k, y[q], y[q + 1]);
       float d0, d1;
       unpack2(add2(k, m2), d0, d1);
-      const uint64_t d = pack2(fmaxf(d0, -40.0f), fmaxf(d1, -40.0f));
+      d0 = fmaxf(d0, -40.0f), d1 = fmaxf(d1, -40.0f);
+      const uint64_t d = pack2(d0, d1);
       constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
-      const uint64_t tn = add2(mul2(d, pack2(0x1.715476p+0f, 0x1.715476p+0f)), pack2(MAGIC, MAGIC));
+      // (the product in two scalar operations: a packed product and sum of .rn each were seen joined into
+      // one rounding, which takes another n where d log2(e) rounds to a half)
+      const uint64_t tn = add2(pack2(__fmul_rn(d0, 0x1.715476p+0f), __fmul_rn(d1, 0x1.715476p+0f)), pack2(MAGIC, MAGIC));
       const uint64_t n = add2(tn, pack2(-MAGIC, -MAGIC));
       uint64_t r = fma2(n, pack2(-0x1.62e43p-1f, -0x1.62e43p-1f), d);
       r = fma2(n, pack2(0x1.05c61p-29f, 0x1.05c61p-29f), r);

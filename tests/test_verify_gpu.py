@@ -184,6 +184,32 @@ def test_top_p_steps(cuda, dtype):
         _check(x, params, [0] * S, np.zeros(S, np.int64), u)
 
 
+def test_weights_whose_reduction_is_a_tie(cuda):
+    """Distances d from the maximum whose d log2(e), rounded, is a half: the weight's reduction must round
+    the product before it rounds to a whole number. One rounding for both takes another whole number at
+    some of them and ends in another last bit, so the draws are made where that bit decides."""
+    log2e = np.float32(float.fromhex("0x1.715476p+0"))
+    rows, us = [], []
+    for k in range(3, 24):
+        near = np.float32(-(k + 0.5) / float(log2e))
+        for step in range(-3, 4):
+            d = near
+            for _ in range(abs(step)):
+                d = np.nextafter(d, np.float32(np.inf if step > 0 else -np.inf))
+            x = np.float32(1.0) + d
+            if d * log2e != -(k + 0.5) or x - np.float32(1.0) != d:
+                continue
+            n = min(int(np.exp(float(-d))), 200000)
+            q = oracle.verify.weights(np.array([d], dtype=np.float32), 0.0)[0]
+            edge = n * int(q) / (n * int(q) + 2**40)  # where the draw passes from the tied values to the maximum
+            rows += [np.append(np.full(n, x, dtype=np.float32), np.float32(1.0))] * 2
+            us += [edge * (1 - 2e-9), edge * (1 + 2e-9)]
+    assert len(rows) > 20
+    for row, u in zip(rows, us, strict=True):
+        x = torch.from_numpy(row)[None]
+        _check(x, [(1.0, 1.0, 0)], [0], np.zeros(1, dtype=np.int64), np.array([u]))
+
+
 def test_strides_and_offsets(cuda):
     """Rows that start anywhere, rows apart, and draft distributions with rows apart."""
     S, V = 9, 1003
