@@ -205,6 +205,20 @@ __global__ void __launch_bounds__(SEG_T, SEG_CTAS) part_kernel(DistillArgs a) {
     }
   }
   __syncthreads();
+  if (TAIL && any_dup) {
+    // which of an element's entries came first above is a matter of chance, and with it the order of the
+    // sums: the terms anew, each by the first of its entries
+    mem = expsum_empty();
+    for (int i = tid; i < a.K; i += SEG_T) {
+      const int64_t ei = entry_index(a, row, i);
+      if (ei < e0 || ei >= e1) continue;
+      bool again = false;
+      for (int j = 0; j < i && !again; ++j) again = entry_index(a, row, j) == ei;
+      if (again) continue;
+      const float z = Elem<T>::ld(rv.row + ei), m = fmaxf(LOWEST, z);
+      mem = expsum_join(mem, ExpSum{m, ex2((z - m) * a.c)}, a.c);
+    }
+  }
 
   if constexpr (TAIL) {
     uint32_t mk = marked[tid];

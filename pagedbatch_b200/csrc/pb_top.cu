@@ -131,6 +131,35 @@ __device__ __noinline__ void select_slow(const RowView<T>& rv, int k, TopShared&
   __syncthreads();
 }
 
+// Adds to the sh.n listed candidates those of the row's elements of this key that have the lowest
+// indices, up to k candidates.
+template <typename T>
+__device__ __noinline__ void add_equals(const RowView<T>& rv, uint32_t key, uint32_t k, TopShared& sh) {
+  constexpr int EPV = Elem<T>::EPV;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t n = sh.n;
+  for (int32_t v0 = 0; v0 < rv.nvec && n < k; v0 += TT) {  // (every thread has the same n)
+    const int32_t v = v0 + tid, e0 = rv.first(v);
+    uint32_t eq = 0;
+    if (v < rv.nvec) {
+      float x[EPV];
+      Elem<T>::unpack(load_vec(rv, v), x);
+#pragma unroll
+      for (int q = 0; q < EPV; ++q) eq |= (key_of(x[q]) == key && e0 + q >= 0 && e0 + q < rv.V ? 1u : 0u) << q;
+    }
+    const uint32_t mine = (uint32_t)__popc(eq), incl = warp_incl_scan(mine);
+    if (lane == 31) sh.steps[warp] = incl;
+    __syncthreads();
+    uint32_t at = n + incl - mine;
+    for (int w = 0; w < TNW; ++w) {
+      if (w < warp) at += sh.steps[w];
+      n += sh.steps[w];
+    }
+    for (; eq && at < k; eq &= eq - 1, ++at) sh.list[at] = compose(key, (uint32_t)(e0 + __ffs(eq) - 1));
+    __syncthreads();
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(TT, SEG_CTAS) part_kernel(TopArgs a) {
   __shared__ ExpSum scratch[TNW];
@@ -214,58 +243,70 @@ __global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
   sum = sh.sum[0];
   bound = sh.raised;
 
-  // the groups that reach the bound, then the values in them that do
-  auto list_group = [&](int32_t s, bool hit) {
-    const uint32_t b = __ballot_sync(0xFFFFFFFFu, hit);
-    if (!b) return;
-    uint32_t at = 0;
-    if (lane == 0) at = atomicAdd(&sh.groups, (uint32_t)__popc(b));
-    at = __shfl_sync(0xFFFFFFFFu, at, 0) + (uint32_t)__popc(b & lanemask_lt());
-    if (hit && at < (uint32_t)TLIST) sh.group[at] = (uint32_t)(s * TT + tid);
-  };
+  // the groups that reach the bound, then the values in them that do. Where they are too many, most of
+  // them equal the bound (masked values, as a rule): those above it are listed instead.
+  uint32_t least = bound, n;
+  bool fits;
+  while (true) {
+    auto list_group = [&](int32_t s, bool hit) {
+      const uint32_t b = __ballot_sync(0xFFFFFFFFu, hit);
+      if (!b) return;
+      uint32_t at = 0;
+      if (lane == 0) at = atomicAdd(&sh.groups, (uint32_t)__popc(b));
+      at = __shfl_sync(0xFFFFFFFFu, at, 0) + (uint32_t)__popc(b & lanemask_lt());
+      if (hit && at < (uint32_t)TLIST) sh.group[at] = (uint32_t)(s * TT + tid);
+    };
 #pragma unroll
-  for (int s = 0; s < HELD; ++s)
-    if (s < segs) list_group(s, key[s] >= bound);
-  for (int32_t s = HELD; s < segs; ++s) list_group(s, __ldcg(keys + (int64_t)s * TT) >= bound);
-  __syncthreads();
-  const uint32_t groups = sh.groups;
-  if (groups <= (uint32_t)TLIST) {
-    constexpr int AHEAD = 4;  // vectors a thread has in flight
-    for (uint32_t i0 = tid; i0 < groups * SEG_V; i0 += TT * AHEAD) {
-      uint4 q[AHEAD];
-      int32_t v[AHEAD];
+    for (int s = 0; s < HELD; ++s)
+      if (s < segs) list_group(s, key[s] >= least);
+    for (int32_t s = HELD; s < segs; ++s) list_group(s, __ldcg(keys + (int64_t)s * TT) >= least);
+    __syncthreads();
+    const uint32_t groups = sh.groups;
+    if (groups <= (uint32_t)TLIST) {
+      constexpr int AHEAD = 4;  // vectors a thread has in flight
+      for (uint32_t i0 = tid; i0 < groups * SEG_V; i0 += TT * AHEAD) {
+        uint4 q[AHEAD];
+        int32_t v[AHEAD];
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const uint32_t i = i0 + u * TT;
-        v[u] = -1;
-        if (i < groups * SEG_V) {
-          const uint32_t g = sh.group[i / SEG_V];
-          const int32_t v0 = (int32_t)(g / TT) * a.seg.per;
-          const int32_t at = v0 + group_of((int32_t)(g % TT)) + (int32_t)(i % SEG_V);
-          if (at < min(rv.nvec, v0 + a.seg.per)) {
-            v[u] = at;
-            q[u] = load_vec(rv, at);
+        for (int u = 0; u < AHEAD; ++u) {
+          const uint32_t i = i0 + u * TT;
+          v[u] = -1;
+          if (i < groups * SEG_V) {
+            const uint32_t g = sh.group[i / SEG_V];
+            const int32_t v0 = (int32_t)(g / TT) * a.seg.per;
+            const int32_t at = v0 + group_of((int32_t)(g % TT)) + (int32_t)(i % SEG_V);
+            if (at < min(rv.nvec, v0 + a.seg.per)) {
+              v[u] = at;
+              q[u] = load_vec(rv, at);
+            }
           }
         }
-      }
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        if (v[u] < 0 || key_of(vec_max_nan<T>(q[u])) < bound) continue;
-        float x[EPV];
-        Elem<T>::unpack(q[u], x);
+        for (int u = 0; u < AHEAD; ++u) {
+          if (v[u] < 0 || key_of(vec_max_nan<T>(q[u])) < least) continue;
+          float x[EPV];
+          Elem<T>::unpack(q[u], x);
 #pragma unroll
-        for (int j = 0; j < EPV; ++j) {
-          const uint32_t kx = key_of(x[j]);
-          const int32_t e = rv.first(v[u]) + j;
-          if (kx >= bound && e >= 0 && e < a.V) {
-            const uint32_t at = atomicAdd(&sh.n, 1u);
-            if (at < (uint32_t)TCAP) sh.list[at] = compose(kx, (uint32_t)e);
+          for (int j = 0; j < EPV; ++j) {
+            const uint32_t kx = key_of(x[j]);
+            const int32_t e = rv.first(v[u]) + j;
+            if (kx >= least && e >= 0 && e < a.V) {
+              const uint32_t at = atomicAdd(&sh.n, 1u);
+              if (at < (uint32_t)TCAP) sh.list[at] = compose(kx, (uint32_t)e);
+            }
           }
         }
       }
     }
+    __syncthreads();
+    n = sh.n;
+    fits = groups <= (uint32_t)TLIST && n <= (uint32_t)TCAP;
+    if (fits || least != bound || bound == 0xFFFFFFFFu) break;
+    __syncthreads();
+    if (tid == 0) sh.groups = sh.n = 0;
+    least = bound + 1;
+    __syncthreads();
   }
-  __syncthreads();
   constexpr float LN2 = 0.6931471805599453f;
   // NaN or +inf in the row (the sum is NaN then), or nothing above -inf: no distribution
   const float l = (sum.s == 0.0f) ? NAN : log2f(sum.s);
@@ -274,10 +315,10 @@ __global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
     a.logprob[row * a.k + at] = (value_of(comp_key(e)) - sum.m) / a.temperature - l * LN2;
     a.index[row * a.k + at] = (int32_t)comp_idx(e);
   };
-  uint32_t n = sh.n;
-  if (n > (uint32_t)TCAP || groups > (uint32_t)TLIST) {
+  if (!fits || n < (uint32_t)a.k) {
     __syncthreads();
-    select_slow<T>(rv, a.k, sh);
+    if (!fits) select_slow<T>(rv, a.k, sh);
+    else add_equals<T>(rv, bound, (uint32_t)a.k, sh);
     n = (uint32_t)a.k;
   }
   if (n <= (uint32_t)TRANK) {

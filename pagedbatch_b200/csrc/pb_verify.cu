@@ -529,7 +529,6 @@ __device__ __forceinline__ float prob_at(const VerifyArgs& a, int64_t d, int64_t
   return Elem<__half>::ld(static_cast<const __half*>(a.probs) + at);
 }
 
-
 // The row a sequence draws its last token from, and the weights of its elements.
 template <typename T>
 struct DrawRow {
@@ -543,7 +542,7 @@ struct DrawRow {
   float d_most;      // draft probabilities above this take all of any weight, and stay on the grid below
   int64_t dx, drow;  // the rejected draft; its row of draft_probs
   bool residual, dist, cut_ties, whole;
-  float raw_lo, thr;  // (a key's order is its value's: the row holds no NaN)
+  float raw_lo, thr;  // raw values below raw_lo have no weight (a key's order is its value's: the row holds no NaN)
   __device__ DrawRow(const VerifyArgs& a_, int64_t seq, const Decision& d, float tf, const pb_row_info& f_)
       : a(a_), rv(static_cast<const T*>(a_.x) + d.row * a_.row_stride, a_.V), f(f_), scaled(tf),
         weigh(tf, f_.max_key, f_.max_key * tf) {
@@ -553,7 +552,8 @@ struct DrawRow {
     dist = residual && a.probs && drow >= 0 && drow < a.n_probs;
     cut_ties = f.kept_q != f.z_q;
     whole = f.thr_key == 0;
-    raw_lo = surely_below(f.thr_key, tf);
+    // (a key more than 28 below the largest has no weight, kept or not: masked values among a top-k)
+    raw_lo = fmaxf(surely_below(f.thr_key, tf), surely_below(key_of(f.max_key - 28.0f), tf));
     thr = value_of(f.thr_key);
     z = __ull2double_rn(f.kept_q) * 0x1p-40;
     d_most = 2048.0f / (float)z;  // (anywhere between 1 / Z and 4095 / Z would do)

@@ -305,6 +305,24 @@ def test_types_of_the_record(cuda):
         assert torch.equal(a, pb.distill_loss(z.cuda(), lp.to(dtype).float().cuda(), idx.cuda()))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_repeated_entries_give_the_same_bits(cuda, dtype):
+    """However the threads meet at an element that several entries name."""
+    n, V, K = 64, 1000, 1024
+    g = torch.Generator().manual_seed(9)
+    z = (3 * torch.randn(n, V, generator=g)).to(dtype).cuda()
+    idx = torch.randint(0, 300, (n, K), generator=g).cuda()
+    lp = (torch.randn(n, K, generator=g) - 9).cuda()
+    want = None
+    for _ in range(10):
+        x = z.detach().requires_grad_()
+        loss = pb.distill_loss(x, lp, idx, tail=True)
+        loss.sum().backward()
+        got = (loss.detach(), x.grad)
+        want = want or got
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_gradient_scale_and_repeats(cuda):
     """Scaled, zero and repeated backward passes, and the same bits each time."""
     z = workloads.head_boosted(40, 4099, seed=1, dtype=torch.bfloat16).cuda().requires_grad_()

@@ -104,6 +104,27 @@ def test_masked_rows(cuda):
         check(x, 64, 2.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,shift", [(50021, 0), (50021, 3), (600, 1)])
+def test_few_allowed_tokens(cuda, dtype, V, shift):
+    """Rows of which a mask (-inf, the type's lowest value, any value) leaves a few tokens, fewer or more
+    than k: the lowest ids of the masked ones follow them."""
+    g = torch.Generator().manual_seed(V)
+    low = (-torch.inf, torch.finfo(dtype).min, -30.0)
+    left = (0, 1, 5, 30, 255, 300)
+    x = torch.empty(len(low) * len(left), V, dtype=dtype)
+    for r in range(len(x)):
+        n = left[r % len(left)]
+        x[r] = low[r // len(left)]
+        x[r, torch.randperm(V, generator=g)[:n]] = torch.randn(n, generator=g).to(dtype)
+    x[4, -1] = 1.0  # the row's last token
+    buf = torch.zeros(len(x), V + 8, dtype=dtype, device="cuda")
+    view = buf[:, shift : shift + V]
+    view.copy_(x)
+    for k in (1, 20, 50, 256):
+        check(x, k, view=view)
+
+
 def test_strides(cuda):
     V = 1003
     for dtype in (torch.float32, torch.float16):

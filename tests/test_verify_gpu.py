@@ -267,6 +267,32 @@ def test_masked_rows(cuda):
         _check(x, params, lens, _drafts(x, lens, 3), u, _probs(x.clamp(min=-1e4), lens, params, 4))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,shift", [(50024, 0), (50021, 3)])
+def test_few_allowed_tokens(cuda, dtype, V, shift):
+    """Rows of which a mask leaves fewer tokens than top_k keeps, or one: masked ones are never drawn."""
+    g = torch.Generator().manual_seed(V)
+    S, n = 10, 2
+    x = torch.empty(S * (n + 1), V, dtype=dtype)
+    for r in range(len(x)):
+        few = (1, 5, 30, 200)[r % 4]
+        x[r] = (-torch.inf, torch.finfo(dtype).min, -60.0)[r % 3]
+        x[r, torch.randperm(V, generator=g)[:few]] = torch.randn(few, generator=g).to(dtype)
+    buf = torch.zeros(len(x), V + 8, dtype=dtype, device="cuda")
+    view = buf[:, shift : shift + V]
+    view.copy_(x)
+    for kind in ("topk", "topp", "mixed"):
+        params = [KINDS[kind](i) for i in range(S)]
+        for seed in range(2):
+            u = np.random.default_rng(seed).random(len(x))
+            probs = _probs(x.clamp(min=-1e4), [n] * S, params, seed) if seed else None
+            tok, _, st = _check(x, params, [n] * S, _drafts(x, [n] * S, seed), u, probs, view=view)
+            assert not st.any()
+            drawn = torch.from_numpy(tok)
+            at = drawn >= 0
+            assert (x[at, drawn[at]] > -20).all()
+
+
 def test_invalid_rows_and_numbers(cuda):
     """A row without a distribution fails its sequence only where the sequence reaches it; so does a
     random number outside [0, 1); a draft outside the vocabulary is rejected."""
