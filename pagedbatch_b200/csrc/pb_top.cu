@@ -131,6 +131,75 @@ __device__ __noinline__ void select_slow(const RowView<T>& rv, int k, TopShared&
   __syncthreads();
 }
 
+// Lists a group where it is a hit (all lanes of a warp call it).
+__device__ __forceinline__ void list_group(TopShared& sh, uint32_t group, bool hit) {
+  const uint32_t b = __ballot_sync(0xFFFFFFFFu, hit);
+  if (!b) return;
+  uint32_t at = 0;
+  if ((threadIdx.x & 31) == 0) at = atomicAdd(&sh.groups, (uint32_t)__popc(b));
+  at = __shfl_sync(0xFFFFFFFFu, at, 0) + (uint32_t)__popc(b & lanemask_lt());
+  if (hit && at < (uint32_t)TLIST) sh.group[at] = group;
+}
+
+// Lists the listed groups' values at or above a key. One barrier.
+template <typename T>
+__device__ __forceinline__ void list_values(const RowView<T>& rv, int32_t per, uint32_t least, TopShared& sh) {
+  constexpr int EPV = Elem<T>::EPV;
+  constexpr int AHEAD = 4;  // vectors a thread has in flight
+  const uint32_t tid = threadIdx.x, groups = sh.groups;
+  if (groups <= (uint32_t)TLIST) {
+    for (uint32_t i0 = tid; i0 < groups * SEG_V; i0 += TT * AHEAD) {
+      uint4 q[AHEAD];
+      int32_t v[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const uint32_t i = i0 + u * TT;
+        v[u] = -1;
+        if (i < groups * SEG_V) {
+          const uint32_t g = sh.group[i / SEG_V];
+          const int32_t v0 = (int32_t)(g / TT) * per;
+          const int32_t at = v0 + group_of((int32_t)(g % TT)) + (int32_t)(i % SEG_V);
+          if (at < min(rv.nvec, v0 + per)) {
+            v[u] = at;
+            q[u] = load_vec(rv, at);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (v[u] < 0 || key_of(vec_max_nan<T>(q[u])) < least) continue;
+        float x[EPV];
+        Elem<T>::unpack(q[u], x);
+#pragma unroll
+        for (int j = 0; j < EPV; ++j) {
+          const uint32_t kx = key_of(x[j]);
+          const int32_t e = rv.first(v[u]) + j;
+          if (kx >= least && e >= 0 && e < rv.V) {
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            if (at < (uint32_t)TCAP) sh.list[at] = compose(kx, (uint32_t)e);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// The lists once more, for a key above the one that too many values reach: most of those equal it
+// (masked values, as a rule). Whether they fit now.
+template <typename T>
+__device__ __noinline__ bool list_above(const RowView<T>& rv, SegPlan seg, const uint32_t* keys, uint32_t least,
+                                        TopShared& sh) {
+  __syncthreads();
+  if (threadIdx.x == 0) sh.groups = sh.n = 0;
+  __syncthreads();
+  for (int32_t s = 0; s < seg.segs; ++s)
+    list_group(sh, (uint32_t)s * TT + threadIdx.x, __ldcg(keys + (int64_t)s * TT) >= least);
+  __syncthreads();
+  list_values<T>(rv, seg.per, least, sh);
+  return sh.groups <= (uint32_t)TLIST && sh.n <= (uint32_t)TCAP;
+}
+
 // Adds to the sh.n listed candidates those of the row's elements of this key that have the lowest
 // indices, up to k candidates.
 template <typename T>
@@ -243,70 +312,15 @@ __global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
   sum = sh.sum[0];
   bound = sh.raised;
 
-  // the groups that reach the bound, then the values in them that do. Where they are too many, most of
-  // them equal the bound (masked values, as a rule): those above it are listed instead.
-  uint32_t least = bound, n;
-  bool fits;
-  while (true) {
-    auto list_group = [&](int32_t s, bool hit) {
-      const uint32_t b = __ballot_sync(0xFFFFFFFFu, hit);
-      if (!b) return;
-      uint32_t at = 0;
-      if (lane == 0) at = atomicAdd(&sh.groups, (uint32_t)__popc(b));
-      at = __shfl_sync(0xFFFFFFFFu, at, 0) + (uint32_t)__popc(b & lanemask_lt());
-      if (hit && at < (uint32_t)TLIST) sh.group[at] = (uint32_t)(s * TT + tid);
-    };
+  // the groups that reach the bound, then the values in them that do
 #pragma unroll
-    for (int s = 0; s < HELD; ++s)
-      if (s < segs) list_group(s, key[s] >= least);
-    for (int32_t s = HELD; s < segs; ++s) list_group(s, __ldcg(keys + (int64_t)s * TT) >= least);
-    __syncthreads();
-    const uint32_t groups = sh.groups;
-    if (groups <= (uint32_t)TLIST) {
-      constexpr int AHEAD = 4;  // vectors a thread has in flight
-      for (uint32_t i0 = tid; i0 < groups * SEG_V; i0 += TT * AHEAD) {
-        uint4 q[AHEAD];
-        int32_t v[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          const uint32_t i = i0 + u * TT;
-          v[u] = -1;
-          if (i < groups * SEG_V) {
-            const uint32_t g = sh.group[i / SEG_V];
-            const int32_t v0 = (int32_t)(g / TT) * a.seg.per;
-            const int32_t at = v0 + group_of((int32_t)(g % TT)) + (int32_t)(i % SEG_V);
-            if (at < min(rv.nvec, v0 + a.seg.per)) {
-              v[u] = at;
-              q[u] = load_vec(rv, at);
-            }
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          if (v[u] < 0 || key_of(vec_max_nan<T>(q[u])) < least) continue;
-          float x[EPV];
-          Elem<T>::unpack(q[u], x);
-#pragma unroll
-          for (int j = 0; j < EPV; ++j) {
-            const uint32_t kx = key_of(x[j]);
-            const int32_t e = rv.first(v[u]) + j;
-            if (kx >= least && e >= 0 && e < a.V) {
-              const uint32_t at = atomicAdd(&sh.n, 1u);
-              if (at < (uint32_t)TCAP) sh.list[at] = compose(kx, (uint32_t)e);
-            }
-          }
-        }
-      }
-    }
-    __syncthreads();
-    n = sh.n;
-    fits = groups <= (uint32_t)TLIST && n <= (uint32_t)TCAP;
-    if (fits || least != bound || bound == 0xFFFFFFFFu) break;
-    __syncthreads();
-    if (tid == 0) sh.groups = sh.n = 0;
-    least = bound + 1;
-    __syncthreads();
-  }
+  for (int s = 0; s < HELD; ++s)
+    if (s < segs) list_group(sh, (uint32_t)(s * TT + tid), key[s] >= bound);
+  for (int32_t s = HELD; s < segs; ++s) list_group(sh, (uint32_t)(s * TT + tid), __ldcg(keys + (int64_t)s * TT) >= bound);
+  __syncthreads();
+  list_values<T>(rv, a.seg.per, bound, sh);
+  bool fits = sh.groups <= (uint32_t)TLIST && sh.n <= (uint32_t)TCAP;
+  if (!fits && bound != 0xFFFFFFFFu) fits = list_above<T>(rv, a.seg, keys, bound + 1, sh);
   constexpr float LN2 = 0.6931471805599453f;
   // NaN or +inf in the row (the sum is NaN then), or nothing above -inf: no distribution
   const float l = (sum.s == 0.0f) ? NAN : log2f(sum.s);
@@ -315,6 +329,7 @@ __global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
     a.logprob[row * a.k + at] = (value_of(comp_key(e)) - sum.m) / a.temperature - l * LN2;
     a.index[row * a.k + at] = (int32_t)comp_idx(e);
   };
+  uint32_t n = sh.n;
   if (!fits || n < (uint32_t)a.k) {
     __syncthreads();
     if (!fits) select_slow<T>(rv, a.k, sh);
