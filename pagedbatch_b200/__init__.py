@@ -3,9 +3,9 @@
 Drop-in for ``pagedbatch.sampling.sample_token`` plus the batched ``sample_tokens`` the engine
 calls once per step, and the operators of drafted decoding: ``verify`` / ``verify_tokens`` (drafted
 tokens against the target's rows), ``top_logprobs`` (a teacher's record of a row) and ``distill_loss``
-(which trains a draft model on such records). The compute path is the C-ABI library ``_pb_sample.so`` built from
-``csrc/`` (see ``include/pagedbatch_b200.h``); importing this package does not load it, the
-first sampling call does, and fails loudly if it is missing.
+(which trains a draft model on such records). The compute path is the C-ABI library ``_pb_sample.so``
+built from ``csrc/`` (see ``include/pagedbatch_b200.h``); importing this package does not load it,
+the first call does, and fails loudly if it is missing.
 """
 
 from .config import SamplingParams

@@ -16,7 +16,10 @@
 // loss from the row's entries. For the tail bucket the entries are kept out of the sums exactly (a bit
 // per element of the segment in shared memory), so S has no cancellation however sure the student is.
 // Backward: one launch, z in and dz out, on the statistics of the forward. Both passes are bound by
-// HBM: V * es bytes a row forward, twice that backward.
+// HBM: V * es bytes a row forward, twice that backward. [4096, 128256] bf16 with a tail, summed: 567 us,
+// floor 326 us if the backward pass found the logits on chip, 488 us as they are read twice. (A persistent
+// kernel that takes both passes over a few rows at a time, the second from L2, took 570 us: its halves wait
+// for one another.)
 #include "pb_rows.cuh"
 
 using namespace pb;
@@ -165,7 +168,9 @@ struct GradRow {
   }
 };
 
-// CTA (row, segment): the sums of the segment's exponentials.
+// CTA (row, segment): the sums of the segment's exponentials. [4096, 128256] bf16 with a tail (1.05 GB) in
+// 217 us, 4.8 TB/s: its loads stand still while the entries are marked. (Entries matched by each warp for
+// itself, without the marks, took a quarter longer.)
 template <typename T, bool TAIL>
 __global__ void __launch_bounds__(SEG_T, SEG_CTAS) part_kernel(DistillArgs a) {
   constexpr int EPV = Elem<T>::EPV;
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(SEG_T, SEG_CTAS) part_kernel(DistillArgs a) {
 }
 
 // One warp per row: joins the row's segments, takes the loss from its entries, and leaves what the
-// backward pass needs.
+// backward pass needs. Its loads of entries go ahead of the wait for the segments. 6.5 us for 4096 rows.
 template <typename T, bool TAIL>
 __global__ void __launch_bounds__(256) finish_kernel(DistillArgs a) {
   const int lane = threadIdx.x & 31;
@@ -361,7 +366,8 @@ __global__ void __launch_bounds__(256) finish_kernel(DistillArgs a) {
   }
 }
 
-// CTA (row, segment): the gradient of the segment, then of the entries in it.
+// CTA (row, segment): the gradient of the segment, then of the entries in it. Bound by HBM: [4096, 128256]
+// bf16, 2.1 GB read and written in 345 us, 6.1 TB/s (94% of the measured copy rate).
 template <typename T>
 __global__ void __launch_bounds__(SEG_T, 4) backward_kernel(DistillArgs a) {
   const int64_t row = blockIdx.x;
@@ -390,7 +396,7 @@ __global__ void __launch_bounds__(SEG_T, 4) backward_kernel(DistillArgs a) {
   }
 }
 
-// Sum of the rows' losses, in 64 bits and a fixed order, by one CTA.
+// Sum of the rows' losses, in 64 bits and a fixed order, by one CTA (3 us for 4096).
 __global__ void __launch_bounds__(1024) distill_sum_kernel(const float* loss, int64_t n, float* out) {
   __shared__ double part[32];
   double s = 0.0;

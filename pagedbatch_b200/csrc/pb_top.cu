@@ -14,9 +14,11 @@
 // histogram of the group keys above that bound (256 equal steps up to the largest key) raises it to
 // the step that k of them reach. Only the groups whose key reaches the raised bound are read again
 // (from L2); their values at or above it are the candidates, a little more than k, put in order by
-// counting for each the candidates before it, or where they are many by a bitonic network. A row with more candidates than the list holds (very many
-// equal values) is selected by bisection over (value, index).
-// HBM-bound: V * es bytes a row, and 1/32 of that written as keys.
+// counting for each the candidates before it, or where they are many by a bitonic network. A row with more
+// candidates than the list holds, nearly all of them equal as a mask makes them, has those above that
+// value listed and the first of its equals added; any other is selected by bisection over (value, index).
+// HBM-bound: V * es bytes a row, and 1/32 of that written as keys. [1024, 128256] bf16, k 128: 77 us, the
+// read's floor 41 us; one CTA or cluster a row, which selects while others read, took 187 us.
 #include "pb_rows.cuh"
 
 using namespace pb;
@@ -229,6 +231,8 @@ __device__ __noinline__ void add_equals(const RowView<T>& rv, uint32_t key, uint
   }
 }
 
+// CTA (row, segment): the keys of its groups and its sum. Bound by HBM: [1024, 128256] bf16 (263 MB) in 46
+// us, 5.8 TB/s (89% of the measured copy rate).
 template <typename T>
 __global__ void __launch_bounds__(TT, SEG_CTAS) part_kernel(TopArgs a) {
   __shared__ ExpSum scratch[TNW];
@@ -244,6 +248,9 @@ __global__ void __launch_bounds__(TT, SEG_CTAS) part_kernel(TopArgs a) {
   if (threadIdx.x == 0) a.parts[part] = sum;
 }
 
+// A CTA per row, as above. Latency (the keys, the bound, the groups, the order, each after the one before),
+// 592 rows at a time: 9 us for 256 rows of k 50, 31 us for 1024 of k 128. (Six CTAs to an SM did not shorten
+// it.)
 template <typename T>
 __global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
   constexpr int EPV = Elem<T>::EPV;
