@@ -170,6 +170,7 @@ __device__ __forceinline__ float surely_below(uint32_t thr, float tf) {
 struct Weigher {
   float t, recip, inv, m;
   bool fast;  // the row's values are ordinary enough for the packed steps
+  static constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
   __device__ Weigher(float t_, float m_, float raw_max) : t(t_), m(m_) {
     const Scale s(t_);
     inv = s.inv;
@@ -210,7 +211,6 @@ struct Weigher {
       unpack2(add2(k, m2), d0, d1);
       d0 = fmaxf(d0, -40.0f), d1 = fmaxf(d1, -40.0f);
       const uint64_t d = pack2(d0, d1);
-      constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
       // (the product in two scalar operations: a packed product and sum of .rn each were seen joined into
       // one rounding, which takes another n where d log2(e) rounds to a half)
       const uint64_t tn = add2(pack2(__fmul_rn(d0, 0x1.715476p+0f), __fmul_rn(d1, 0x1.715476p+0f)), pack2(MAGIC, MAGIC));
@@ -331,9 +331,29 @@ __global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
 
 // ---- top-p alone -----------------------------------------------------------------------------
 
-// Step of a scaled value y in its row's histogram: it does not fall as y falls.
-__device__ __forceinline__ int32_t step_of(float y, float m) {
-  return min(STEPS - 1, (int32_t)__fmul_rn(__fsub_rn(m, y), STEP_SCALE));
+// Step in its row's histogram of a key d below the largest (d = RN(y - m), not below -28): the whole number
+// next to -d * STEP_SCALE, which does not fall as the key falls.
+__device__ __forceinline__ int32_t step_of(float d) {
+  return __float_as_int(__fmaf_rn(d, -STEP_SCALE, Weigher::MAGIC)) - __float_as_int(Weigher::MAGIC);
+}
+
+// lo[0] + 2^32 lo[STEPS] += u, in shared memory (nothing for u = 0; a carry is rare).
+__device__ __forceinline__ void add_to_step(uint32_t* lo, uint64_t u) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(lo);
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      ".reg .u32 l, h, old;\n"
+      "mov.b64 {l, h}, %1;\n"
+      "mov.u32 old, 0;\n"
+      "setp.ne.u64 p, %1, 0;\n"
+      "@p atom.shared.add.u32 old, [%0], l;\n"
+      "add.cc.u32 l, old, l;\n"
+      "addc.u32 h, h, 0;\n"
+      "setp.ne.u32 q, h, 0;\n"
+      "@q red.shared.add.u32 [%0 + %2], h;\n"
+      "}\n" ::"r"(at), "l"(u), "n"(STEPS * 4)
+      : "memory");
 }
 
 // Sums of the weights of every ROW_MASS row, by step: shared-memory atomics for the segment, then one
@@ -343,14 +363,14 @@ __device__ __forceinline__ int32_t step_of(float y, float m) {
 template <typename T>
 __global__ void __launch_bounds__(VT, 3) hist_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
-  __shared__ uint32_t lo[STEPS], hi[STEPS];  // 64-bit sums in two words (a carry is rare)
+  __shared__ uint32_t lo[2 * STEPS];  // 64-bit sums: low words, then high words
   grid_release();
   const int64_t row = a.n_rows - 1 - blockIdx.x;
   const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
   const int32_t v0 = (int32_t)(gridDim.y - 1 - blockIdx.y) * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
   uint4 q[SEG_V];
   if (a.one_kind == ROW_MASS) load_segment(rv, v0, v1, q);
-  for (int i = threadIdx.x; i < STEPS; i += VT) lo[i] = hi[i] = 0;
+  for (int i = threadIdx.x; i < 2 * STEPS; i += VT) lo[i] = 0;
   grid_wait();  // the rows' largest values
   const RowMeta meta = a.meta[row];
   if (meta.kind != ROW_MASS) return;
@@ -367,17 +387,14 @@ __global__ void __launch_bounds__(VT, 3) hist_kernel(VerifyArgs a) {
     weigh.template of<T>(q[i], w, y);
 #pragma unroll
     for (int j = 0; j < EPV; ++j) {
-      const uint64_t u = grid_units(on_grid(w[j]));
-      if (!u) continue;
-      const int32_t s = step_of(y[j], m);
-      const uint32_t l = (uint32_t)u, old = atomicAdd(&lo[s], l);
-      const uint32_t h = (uint32_t)(u >> 32) + (old + l < old ? 1u : 0u);
-      if (h) atomicAdd(&hi[s], h);
+      // (below -28 there is no weight and nothing is added: the address is any)
+      const int32_t s = step_of(fmaxf(__fsub_rn(y[j], m), -27.75f));
+      add_to_step(lo + s, grid_units(on_grid(w[j])));
     }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < STEPS; i += VT) {
-    const unsigned long long u = (uint64_t)hi[i] << 32 | lo[i];
+    const unsigned long long u = (uint64_t)lo[STEPS + i] << 32 | lo[i];
     if (u) atomicAdd(reinterpret_cast<unsigned long long*>(a.hist + row * STEPS + i), u);
   }
 }
@@ -426,12 +443,14 @@ __global__ void __launch_bounds__(VT) cut_kernel(VerifyArgs a) {
   }
 }
 
-// The elements of that step, in any order. A vector is left after one comparison of its largest element;
+// The elements of that step, in any order, listed by each CTA for itself and then added to the row's list. A vector is left after one comparison of its largest element;
 // elements surely outside the step by their raw values after two. 256 rows of 49152 bf16 in 16 us, the rows
 // from L2, bound by issue.
 template <typename T>
 __global__ void __launch_bounds__(VT, 4) gather_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
+  __shared__ uint64_t list[LIST];
+  __shared__ uint32_t found, base;
   grid_release();
   const int64_t row = blockIdx.x;
   const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
@@ -444,9 +463,11 @@ __global__ void __launch_bounds__(VT, 4) gather_kernel(VerifyArgs a) {
   if (a.one_kind != ROW_MASS) load_segment(rv, v0, v1, q);
   const Scale scaled(meta.t);
   const float m = a.info[row].max_key;
+  if (threadIdx.x == 0) found = 0;
+  __syncthreads();
   // raw values that are surely below the step, or above it
-  const float raw_lo = surely_below(key_of(m - ((float)meta.step + 1.5f) / STEP_SCALE), meta.t);
-  const float above = (m - ((float)meta.step - 0.5f) / STEP_SCALE) * meta.t;
+  const float raw_lo = surely_below(key_of(m - ((float)meta.step + 1.0f) / STEP_SCALE), meta.t);
+  const float above = (m - ((float)meta.step - 1.0f) / STEP_SCALE) * meta.t;
   const float raw_hi = above + fabsf(above) * 0x1p-20f + 0x1p-100f;  // (NaN or infinite: no bound)
 #pragma unroll
   for (int i = 0; i < SEG_V; ++i) {
@@ -461,11 +482,16 @@ __global__ void __launch_bounds__(VT, 4) gather_kernel(VerifyArgs a) {
       const int j = __ffs(near) - 1;
       near &= near - 1;
       const float y = scaled(Elem<T>::elem(q[i], j));
-      if (e0 + j < 0 || e0 + j >= a.V || step_of(y, m) != meta.step || !weight_q(y, m)) continue;
-      const uint32_t at = atomicAdd(&a.meta[row].listed, 1u);
-      if (at < (uint32_t)LIST) a.list[row * LIST + at] = compose(key_of(y), (uint32_t)(e0 + j));
+      if (e0 + j < 0 || e0 + j >= a.V || !weight_q(y, m) || step_of(__fsub_rn(y, m)) != meta.step) continue;
+      const uint32_t at = atomicAdd(&found, 1u);
+      if (at < (uint32_t)LIST) list[at] = compose(key_of(y), (uint32_t)(e0 + j));
     }
   }
+  __syncthreads();
+  const uint32_t n = found;
+  if (threadIdx.x == 0 && n) base = atomicAdd(&a.meta[row].listed, n);
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < n && base + i < (uint32_t)LIST; i += VT) a.list[row * LIST + base + i] = list[i];
 }
 
 // The last kept element among them, in the order (key descending, index ascending): what the row's
