@@ -16,15 +16,16 @@
 // Launches, each of which may start while the one before it ends:
 //   1. expand_kernel: each row's parameters from its sequence's.
 //   2. each row's kept set and its mass, as the sampler's info record describes them. Greedy and small
-//      top-k rows: pb_sample_ws. Rows without filters, whose kept set is the whole row: max_kernel and
-//      mass_kernel, two passes in segments, the largest value and then the sum of the weights. Rows
+//      top-k rows: pb_sample_ws. Rows without filters, whose kept set is the whole row: max_kernel, the
+//      largest value and a sum of exponentials near the mass, all that most decisions need. Rows
 //      with top-p alone: max_kernel, then hist_kernel sums the weights in 512 steps of the key,
 //      cut_kernel finds the step in which the mass passes top-p, gather_kernel lists its elements and
 //      order_kernel finds the last kept one among them. Every other row (large top-k, a step of too
 //      many elements, rejected parameters): the sampler's cluster kernel.
 //   3. decide_kernel: a CTA per sequence finds the first rejected row.
-//   4. weigh_kernel: that row's weights, summed per tile (256 vectors), a CTA per segment.
-//   5. draw_kernel: a CTA per sequence finds the draw's tile and its element.
+//   4. mass_kernel: that row's mass, where it has no filters.
+//   5. weigh_kernel: that row's weights, summed per tile (256 vectors), a CTA per segment.
+//   6. draw_kernel: a CTA per sequence finds the draw's tile and its element.
 // Weights are exact integers throughout (multiples of 2^-40 below 2^13, which fp64 adds without
 // rounding), so no result depends on an order of addition.
 #include "pb_internal.h"
@@ -64,7 +65,8 @@ struct Tile {
   int32_t ties, pad;
 };
 
-// Where a sequence stopped.
+// Where a sequence stopped: EV_TIE is a draft whose row has to be looked at again before it is decided.
+enum : int32_t { EV_REJECT = 0, EV_BAD = 1, EV_TIE = 2, EV_LAST = 3 };
 struct Decision {
   int64_t row;
   int32_t kind;   // EV_*
@@ -90,6 +92,7 @@ struct VerifyArgs {
   pb_row_info* info;             // workspace: [n_rows]
   int64_t* tok;                  // workspace: [n_rows], the sampler's tokens (greedy rows' maxima)
   RowMeta* meta;                 // workspace: [n_rows]
+  ExpSum* sums;                  // workspace: [n_rows][segs], of ROW_WHOLE rows
   Decision* decision;            // workspace: [n_seqs]
   Tile* tiles;                   // workspace: [n_seqs][segs][TILES]
   SegPlan seg;
@@ -243,68 +246,94 @@ __device__ __forceinline__ uint64_t grid_units(double sum) {                    
   return (uint64_t)__double_as_longlong(sum) & ((1ull << 52) - 1);
 }
 
-// Key of the largest value of every row that is summed here; clears the histograms of those with one.
-// Bound by HBM: 898 rows of 128256 bf16 (230 MB) in 30 us, 7.6 TB/s with what is still in L2.
+// Base-2 exponent of a raw difference.
+__device__ __forceinline__ float exponent_of(float t) { return __fdiv_rn(1.44269504f, t); }
+
+// Key of the largest value of every row that is summed here, and for ROW_WHOLE rows the segment's sum of
+// exponentials in fp32; clears the histograms of the others. Bound by HBM: 898 rows of 128256 bf16 (230
+// MB) in TODO us.
 template <typename T>
 __global__ void __launch_bounds__(VT, SEG_CTAS) max_kernel(VerifyArgs a) {
   __shared__ uint32_t top[VNW];
+  __shared__ ExpSum scratch[VNW];
   grid_release();
   const int64_t row = blockIdx.x;
-  int32_t kind = a.one_kind;
-  if (kind < 0) {
+  if (a.one_kind < 0) {
     grid_wait();
-    kind = a.meta[row].kind;
+    const int32_t kind = a.meta[row].kind;
     if (kind != ROW_WHOLE && !(kind == ROW_MASS && a.hist)) return;
   }
   const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
   const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
   uint4 q[SEG_V];
   load_segment(rv, v0, v1, q);
-  uint32_t k = __reduce_max_sync(0xFFFFFFFFu, key_of(vecs_max_nan<T, SEG_V>(q)));
+  grid_wait();  // expand_kernel has set the keys to 0
+  const RowMeta meta = a.meta[row];
+  float largest;
+  if (meta.kind == ROW_WHOLE && a.sums) {
+    const float c = exponent_of(meta.t);
+    const ExpSum sum = block_expsum<VNW>(sum_segment<T>(q, v1 - v0, c, &largest).total(), c, scratch);
+    if (threadIdx.x == 0) a.sums[row * a.seg.segs + blockIdx.y] = sum;
+  } else {
+    largest = vecs_max_nan<T, SEG_V>(q);
+    if (a.hist && blockIdx.y == 0)
+      for (int i = threadIdx.x; i < STEPS; i += VT) a.hist[row * STEPS + i] = 0;
+  }
+  uint32_t k = __reduce_max_sync(0xFFFFFFFFu, key_of(largest));
   if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = k;
   __syncthreads();
-  grid_wait();  // expand_kernel has set the keys to 0
-  if (kind == ROW_MASS && blockIdx.y == 0)
-    for (int i = threadIdx.x; i < STEPS; i += VT) a.hist[row * STEPS + i] = 0;
   if (threadIdx.x < 32) {
     k = __reduce_max_sync(0xFFFFFFFFu, threadIdx.x < VNW ? top[threadIdx.x] : 0u);
     if (threadIdx.x == 0) atomicMax(&a.meta[row].max_key, k);
   }
 }
 
-// Mass of every whole row: the sum of its weights. CTAs take the rows and segments in max_kernel's order
-// backwards, since what that read last is still in L2. Bound by issue and the FMA pipe, not by memory: 18
-// instructions a 32 elements (the exponential's polynomial in pairs, the exact sums), 898 rows of 128256
-// bf16 in 88 us (2.6 TB/s). Scalar arithmetic took 15% longer; one pass that keeps a running maximum is no
-// choice, since a weight is rounded after its distance from the final maximum.
+// What is known of a ROW_WHOLE row's mass Z (in 2^-40, as the sampler rounds it) from its segments' sums:
+// lo <= Z <= hi. With u = 2^-24 and M the largest key, Z differs from the sum S of e^((x - max) / T) by
+//   a weight's key, its distance and its exponential:  S u (2 |M| + 58)
+//   its floor, or its absence beyond 27.73:            2^-40 an element
+// and the fp32 sums from S, elements below 2^-40 of the largest left aside, by at most u S times
+//   132 for an element (its exponent, 40 at most: 64 and 40 for the two roundings, 80 for the factor c, all by
+//   ln 2; 4 for ex2), 33 for a thread's additions, 5 for a warp's and 5 for a block's, 2 for each segment,
+//   and 116 for each change of the largest value: two in a thread, one in the warp, one in the block, one here
+// which is below 1000 u S + 2 segs u S. A sum that is not finite, or a temperature near the ends of the
+// range, tells nothing: hi is infinite.
+struct Mass {
+  double lo, hi;
+};
+__device__ __forceinline__ Mass mass_near(const VerifyArgs& a, int64_t row, float t, float raw_max, float m) {
+  const float c = exponent_of(t);
+  float s = 0.0f;
+  for (int32_t i = 0; i < a.seg.segs; ++i) {
+    const float2 p = __ldcg(reinterpret_cast<const float2*>(a.sums + row * a.seg.segs + i));
+    s += p.y * ex2((p.x - raw_max) * c);
+  }
+  const double off = 0x1p-24 * (1000.0 + 2.1 * (double)fabsf(m) + 2.0 * a.seg.segs), sum = (double)s * 0x1p40;
+  if (!(s < INFINITY) || !(off < 0.25) || !(t >= 0x1p-20f && t <= 0x1p20f)) return Mass{0.0, INFINITY};
+  const double few = 1.1 * (double)a.V;
+  return Mass{sum * (1.0 - off) - few, sum * (1.0 + off) + few};
+}
+
+// The mass of the rows that sequences draw a residual from: the sum of the row's weights, a CTA per segment.
+// Bound by issue and the FMA pipe, not by memory: 18 instructions a 32 elements (the exponential's polynomial
+// in pairs, the exact sums), TODO. (Scalar arithmetic took 15% longer. Summed for every row, before
+// the decisions, instead of the near sums: 898 rows of 128256 bf16 in 88 us.)
 template <typename T>
 __global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
   __shared__ uint64_t part[VNW];
   grid_release();
-  const int64_t row = a.n_rows - 1 - blockIdx.x;
-  const RowView<T> rv(static_cast<const T*>(a.x) + row * a.row_stride, a.V);
-  const int32_t v0 = (int32_t)(gridDim.y - 1 - blockIdx.y) * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
-  uint4 q[SEG_V];
-  if (a.one_kind == ROW_WHOLE) load_segment(rv, v0, v1, q);
-  grid_wait();  // the rows' largest values
-  const RowMeta meta = a.meta[row];
+  grid_wait();  // the decisions
+  const Decision d = a.decision[blockIdx.x];
+  if (!d.draws || d.kind != EV_REJECT) return;
+  const RowMeta meta = a.meta[d.row];
   if (meta.kind != ROW_WHOLE) return;
-  if (a.one_kind != ROW_WHOLE) load_segment(rv, v0, v1, q);
-  const float raw = value_of(meta.max_key), m = Scale(meta.t)(raw);
-  const uint32_t sk = key_of(m);
-  const bool ok = meta.max_key != 0xFFFFFFFFu && sk < KEY_POS_INF && sk > KEY_NEG_INF;
-  if (blockIdx.y == 0 && threadIdx.x == 0) {
-    pb_row_info* o = a.info + row;
-    o->thr_key = 0;  // every key is above it
-    o->n_tie_kept = 0;
-    o->kept_count = a.V;
-    o->status = ok ? PB_ROW_OK : PB_ROW_NONFINITE;
-    o->max_key = m;
-    o->flags = PB_PATH_LARGE;
-  }
-  if (!ok) return;
-  const Weigher weigh(meta.t, m, raw);
+  const RowView<T> rv(static_cast<const T*>(a.x) + d.row * a.row_stride, a.V);
+  const int32_t v0 = (int32_t)blockIdx.y * a.seg.per, v1 = min(rv.nvec, v0 + a.seg.per);
+  uint4 q[SEG_V];
+  load_segment(rv, v0, v1, q);
+  const float raw = value_of(meta.max_key);
+  const Weigher weigh(meta.t, Scale(meta.t)(raw), raw);
   double s0 = GRID, s1 = GRID;  // (at most SEG_V * EPV weights of 1 in both)
 #pragma unroll
   for (int i = 0; i < SEG_V; ++i) {
@@ -323,10 +352,29 @@ __global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
   if (threadIdx.x < 32) {
     z = warp_sum(threadIdx.x < VNW ? part[threadIdx.x] : 0ull);
     if (threadIdx.x == 0) {  // (whole numbers: the order of the segments does not matter)
-      atomicAdd(reinterpret_cast<unsigned long long*>(&a.info[row].z_q), (unsigned long long)z);
-      atomicAdd(reinterpret_cast<unsigned long long*>(&a.info[row].kept_q), (unsigned long long)z);
+      atomicAdd(reinterpret_cast<unsigned long long*>(&a.info[d.row].z_q), (unsigned long long)z);
+      atomicAdd(reinterpret_cast<unsigned long long*>(&a.info[d.row].kept_q), (unsigned long long)z);
     }
   }
+}
+
+// The mass of one row, by one CTA: for the few drafts that mass_near's bounds do not settle.
+template <typename T>
+__device__ __noinline__ uint64_t mass_of(const RowView<T>& rv, float t, float m, float raw, uint64_t* scan) {
+  constexpr int EPV = Elem<T>::EPV;
+  const Weigher weigh(t, m, raw);
+  uint64_t z = 0;
+  for (int32_t v = threadIdx.x; v < rv.nvec; v += VT) {
+    float w[EPV], y[EPV];
+    weigh.template of<T>(load_vec(rv, v), w, y);
+    double s = GRID;
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) s = __dadd_rd(s, (double)w[j]);
+    z += grid_units(s);
+  }
+  uint64_t total;
+  block_excl_scan<uint64_t, VT>(z, scan, &total);
+  return total;
 }
 
 // ---- top-p alone -----------------------------------------------------------------------------
@@ -560,8 +608,6 @@ __global__ void __launch_bounds__(VT) order_kernel(VerifyArgs a) {
 }
 
 // ---- deciding --------------------------------------------------------------------------------
-
-enum : int32_t { EV_REJECT = 0, EV_BAD = 1, EV_TIE = 2, EV_LAST = 3 };
 
 __device__ __forceinline__ float prob_at(const VerifyArgs& a, int64_t d, int64_t i) {
   const int64_t at = d * a.probs_stride + i;
@@ -1015,6 +1061,21 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
     return;
   }
 
+  // a row's record; that of a ROW_WHOLE row, without its mass, from its largest value (every key is above
+  // thr_key)
+  auto record = [&](int64_t r) -> pb_row_info {
+    pb_row_info f = a.info[r];
+    if (row_is == ROW_WHOLE && settled) {
+      const uint32_t raw = a.meta[r].max_key, m = key_of(scaled(value_of(raw)));
+      f.status = raw != 0xFFFFFFFFu && m < KEY_POS_INF && m > KEY_NEG_INF ? PB_ROW_OK : PB_ROW_NONFINITE;
+      f.max_key = value_of(m);
+      f.thr_key = 0;
+      f.n_tie_kept = 0;
+      f.z_q = f.kept_q = 0;  // (mass_kernel adds them)
+    }
+    return f;
+  };
+
   // the first row that is not accepted
   int64_t from = lo, stop = hi - 1;
   int32_t kind = EV_LAST;
@@ -1022,7 +1083,7 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
     if (tid == 0) sh.event = 0x7FFFFFFF;
     __syncthreads();
     for (int64_t r = from + tid; r < hi; r += VT) {
-      const pb_row_info f = a.info[r];
+      const pb_row_info f = record(r);
       const Draft d = r == lo + tid ? first : draft_of(r);
       int32_t ev = -1;
       if (!settled || f.status != PB_ROW_OK) {
@@ -1046,9 +1107,16 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
               else ev = EV_TIE;
             }
             const uint64_t px = (kept || ev == EV_TIE) ? weight_q(y, f.max_key) : 0;
-            const double want = a.probs ? __dmul_rn(d.u, (double)d.prob) : d.u;
-            ok = __dmul_rn(want, __ull2double_rn(f.kept_q)) < __ull2double_rn(px);
-            if (ev == EV_TIE && !ok) ev = EV_REJECT;  // rejected either way
+            const double want = a.probs ? __dmul_rn(d.u, (double)d.prob) : d.u, p = __ull2double_rn(px);
+            if (row_is == ROW_WHOLE) {
+              // (what fp64's own roundings add is far below the bounds' slack)
+              const Mass z = mass_near(a, r, tf, value_of(a.meta[r].max_key), f.max_key);
+              ok = want * z.lo < p;
+              if (ok && !(want * z.hi < p)) ev = EV_TIE;
+            } else {
+              ok = __dmul_rn(want, __ull2double_rn(f.kept_q)) < p;
+              if (ev == EV_TIE && !ok) ev = EV_REJECT;  // rejected either way
+            }
           }
         }
         if (ev < 0 && !ok) ev = EV_REJECT;
@@ -1062,6 +1130,19 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
     kind = e & 3;
     stop = lo + (e >> 2);
     if (kind != EV_TIE) break;
+    if (row_is == ROW_WHOLE) {
+      const float raw = value_of(a.meta[stop].max_key), m = scaled(raw);
+      const RowView<T> row(static_cast<const T*>(a.x) + stop * a.row_stride, a.V);
+      const uint64_t z = mass_of<T>(row, tf, m, raw, near_sh.scan);
+      const Draft d = draft_of(stop);
+      const double want = a.probs ? __dmul_rn(d.u, (double)d.prob) : d.u;
+      if (!(__dmul_rn(want, __ull2double_rn(z)) < __ull2double_rn(weight_q(scaled(d.logit), m)))) {
+        kind = EV_REJECT;
+        break;
+      }
+      from = stop + 1;  // accepted
+      continue;
+    }
     // rank of the draft among the equals of the last kept key, in index order
     const pb_row_info f = a.info[stop];
     const int32_t x = (int32_t)a.drafts[stop];
@@ -1119,9 +1200,11 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
   for (int64_t r = lo + tid; r < stop; r += VT) a.out_tokens[r] = a.drafts[r];
   if (tid == 0) {
     a.out_accepted[seq] = (int32_t)(stop - lo);
+    const pb_row_info f = record(stop);
+    if (row_is == ROW_WHOLE && settled) a.info[stop] = f;
     int32_t st = PB_ROW_OK;
     if (!settled) st = PB_ROW_INTERNAL;
-    else if (kind == EV_BAD) st = a.info[stop].status != PB_ROW_OK ? a.info[stop].status : PB_ROW_BAD_UNIFORM;
+    else if (kind == EV_BAD) st = f.status != PB_ROW_OK ? f.status : PB_ROW_BAD_UNIFORM;
     if (a.out_status) a.out_status[seq] = st;
     if (greedy && kind != EV_BAD) a.out_tokens[stop] = a.tok[stop];
   }
@@ -1416,7 +1499,7 @@ __global__ void __launch_bounds__(VT, 2) draw_kernel(VerifyArgs a) {
 constexpr int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 struct VerifyPlan {
-  int64_t rowp, rowq, info, tok, meta, decision, tiles, hist, list, sampler, bytes;  // offsets in the workspace, its size
+  int64_t rowp, rowq, info, tok, meta, decision, tiles, sums, hist, list, sampler, bytes;  // offsets in the workspace, its size
 };
 VerifyPlan verify_plan(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype, int kinds) {
   const SegPlan seg = seg_plan(vocab, elem_size(dtype), nullptr, 1);  // (rows of any alignment: the most segments)
@@ -1434,6 +1517,7 @@ VerifyPlan verify_plan(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype,
   v.meta = take(n_rows * (int64_t)sizeof(RowMeta));
   v.decision = take(n_seqs * (int64_t)sizeof(Decision));
   v.tiles = take(n_seqs * seg.segs * TILES * (int64_t)sizeof(Tile));
+  v.sums = take(kinds & PB_VERIFY_WHOLE ? n_rows * seg.segs * (int64_t)sizeof(ExpSum) : 0);
   v.hist = take(kinds & PB_VERIFY_TOPP ? n_rows * STEPS * 8 : 0);
   v.list = take(kinds & PB_VERIFY_TOPP ? n_rows * LIST * 8 : 0);
   v.sampler = at;
@@ -1450,6 +1534,7 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
   a.meta = reinterpret_cast<RowMeta*>(ws + plan.meta);
   a.decision = reinterpret_cast<Decision*>(ws + plan.decision);
   a.tiles = reinterpret_cast<Tile*>(ws + plan.tiles);
+  if (kinds & PB_VERIFY_WHOLE) a.sums = reinterpret_cast<ExpSum*>(ws + plan.sums);
   if (kinds & PB_VERIFY_TOPP) {
     a.hist = reinterpret_cast<uint64_t*>(ws + plan.hist);
     a.list = reinterpret_cast<uint64_t*>(ws + plan.list);
@@ -1470,7 +1555,6 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
                        : pb_sample(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr, st);
   }
   if (rc == PB_OK && (kinds & (PB_VERIFY_WHOLE | PB_VERIFY_TOPP))) rc = launch_after(max_kernel<T>, a, rows, VT, st);
-  if (rc == PB_OK && (kinds & PB_VERIFY_WHOLE)) rc = launch_after(mass_kernel<T>, a, rows, VT, st);
   if (rc == PB_OK && (kinds & PB_VERIFY_TOPP)) {
     rc = launch_after(hist_kernel<T>, a, rows, VT, st);
     if (rc == PB_OK) rc = launch_after(cut_kernel, a, each_row, VT, st);
@@ -1484,12 +1568,13 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
   if (rc == PB_OK) rc = launch_after(decide_kernel<T>, a, seqs, VT, st);
   // (a batch whose every sequence draws in decide_kernel needs no more)
   if (rc != PB_OK || (kinds == PB_VERIFY_SMALL && a.groups.keys)) return rc;
+  if (kinds & PB_VERIFY_WHOLE) rc = launch_after(mass_kernel<T>, a, parts, VT, st);
   // few sequences: a segment's tiles shared between more CTAs, as long as all of them run at once (64
   // sequences of 49152 bf16 with draft probabilities: 14.6 us against 18 us unshared, 16 mixed ones of
   // fp16: 6.3 us against 12.9 us)
   a.share = TILES;
   while (a.share > 1 && 2 * a.n_seqs * a.seg.segs * (TILES / a.share) <= WEIGH_CTAS) a.share /= 2;
-  rc = launch_after(weigh_kernel<T>, a, dim3(parts.x, parts.y, TILES / a.share), VT, st);
+  if (rc == PB_OK) rc = launch_after(weigh_kernel<T>, a, dim3(parts.x, parts.y, TILES / a.share), VT, st);
   if (rc == PB_OK) rc = launch_after(draw_kernel<T>, a, seqs, VT, st);
   return rc;
 }

@@ -210,6 +210,33 @@ def test_weights_whose_reduction_is_a_tie(cuda):
         _check(x, [(1.0, 1.0, 0)], [0], np.zeros(1, dtype=np.int64), np.array([u]))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [7, 4099, 50021])
+def test_random_numbers_at_the_edge(cuda, dtype, V):
+    """Random numbers a few roundings around the draft's probability: the exact masses decide."""
+    n = 24
+    params = [((1.0, 0.7, 3.0, 1e-3)[s % 4], 1.0, 0) for s in range(8)]
+    S = len(params)
+    x = workloads.head_boosted(S * (n + 1), V, seed=V, dtype=dtype)
+    x[n + 1 : 2 * (n + 1)] -= x[n + 1 : 2 * (n + 1)].max(1, keepdim=True).values  # largest value 0
+    x[2 * (n + 1) : 3 * (n + 1)] += 500.0
+    d = _drafts(x, [n] * S, 1, favourite=0.5)
+    probs = _probs(x, [n] * S, params, 2).clamp(min=1e-6)
+    u, row = np.zeros(len(x)), 0
+    for s, (T, _, _) in enumerate(params):
+        keys = (x[s * (n + 1) : (s + 1) * (n + 1)].float() / torch.tensor(T)).numpy()
+        for j in range(n):
+            r = s * (n + 1) + j
+            w = oracle.verify.weights(keys[j], float(keys[j].max()))
+            share = float(w[d[r]]) / float(w.sum())
+            # mostly just inside, so that a sequence goes on; the last few wherever they fall
+            off = (-1, -3, -1e-12 * 2**53, -1e-6 * 2**53)[j % 4] if j < n - 4 else (-1, 0, 1, 2)[(s + j) % 4]
+            u[r] = min(max(share / float(probs[row, d[r]]) * (1 + off * 2.0**-53), 0.0), 1 - 2.0**-53)
+            row += 1
+    _check(x, params, [n] * S, d, u, probs)
+    _check(x, params, [n] * S, d, u, probs, marks=False)
+
+
 def test_strides_and_offsets(cuda):
     """Rows that start anywhere, rows apart, and draft distributions with rows apart."""
     S, V = 9, 1003
