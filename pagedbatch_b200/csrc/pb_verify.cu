@@ -250,8 +250,8 @@ __device__ __forceinline__ uint64_t grid_units(double sum) {                    
 __device__ __forceinline__ float exponent_of(float t) { return __fdiv_rn(1.44269504f, t); }
 
 // Key of the largest value of every row that is summed here, and for ROW_WHOLE rows the segment's sum of
-// exponentials in fp32; clears the histograms of the others. Bound by HBM: 898 rows of 128256 bf16 (230
-// MB) in TODO us.
+// exponentials in fp32; clears the histograms of the others. Bound by HBM, the sums by issue nearly as much:
+// 898 rows of 128256 bf16 (230 MB) in 44 us, 5.3 TB/s (30 us without the sums).
 template <typename T>
 __global__ void __launch_bounds__(VT, SEG_CTAS) max_kernel(VerifyArgs a) {
   __shared__ uint32_t top[VNW];
@@ -316,8 +316,8 @@ __device__ __forceinline__ Mass mass_near(const VerifyArgs& a, int64_t row, floa
 
 // The mass of the rows that sequences draw a residual from: the sum of the row's weights, a CTA per segment.
 // Bound by issue and the FMA pipe, not by memory: 18 instructions a 32 elements (the exponential's polynomial
-// in pairs, the exact sums), TODO. (Scalar arithmetic took 15% longer. Summed for every row, before
-// the decisions, instead of the near sums: 898 rows of 128256 bf16 in 88 us.)
+// in pairs, the exact sums), 256 rows of 128256 bf16 in 18 us. (Scalar arithmetic took longer: 233 us a call
+// against 209 us. The masses of all 898 rows, before the decisions and instead of the near sums: 88 us.)
 template <typename T>
 __global__ void __launch_bounds__(VT, 4) mass_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
@@ -405,8 +405,8 @@ __device__ __forceinline__ void add_to_step(uint32_t* lo, uint64_t u) {
 }
 
 // Sums of the weights of every ROW_MASS row, by step: shared-memory atomics for the segment, then one
-// global atomic a step that holds weight (whole numbers: no order shows). Bound by issue: 42 instructions a
-// 32 elements, 256 rows of 49152 bf16 in 28 us. (With the cut found by the sampler's cluster kernel, a
+// global atomic a step that holds weight (whole numbers: no order shows). Bound by issue: about 36
+// instructions a 32 elements, 256 rows of 49152 bf16 in 24 us. (With the cut found by the sampler's cluster kernel, a
 // cluster's repeated sums over its row, the whole call took 238 us instead of 139 us.)
 template <typename T>
 __global__ void __launch_bounds__(VT, 3) hist_kernel(VerifyArgs a) {
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(VT) cut_kernel(VerifyArgs a) {
 }
 
 // The elements of that step, in any order, listed by each CTA for itself and then added to the row's list. A vector is left after one comparison of its largest element;
-// elements surely outside the step by their raw values after two. 256 rows of 49152 bf16 in 16 us, the rows
+// elements surely outside the step by their raw values after two. 256 rows of 49152 bf16 in 14 us, the rows
 // from L2, bound by issue.
 template <typename T>
 __global__ void __launch_bounds__(VT, 4) gather_kernel(VerifyArgs a) {
@@ -1002,7 +1002,7 @@ __device__ __noinline__ int32_t draw_near(const DrawRow<T>& row, const GroupKeys
 }
 
 // A CTA per sequence: the first row that is not accepted, its accepted tokens, and for sequences whose
-// rows' group keys are known the draw. Latency: 8 us for 256 sequences without draws here, 15 us for 64
+// rows' group keys are known the draw. Latency: 10 us for 256 sequences without draws here, 15 us for 64
 // that draw from their top-k rows (the groups' list, their values, the weights: each waits for the one
 // before). With the draws left to weigh_kernel and draw_kernel that call took 106 us instead of 65 us.
 template <typename T>
@@ -1227,8 +1227,8 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
 
 // CTA (sequence, segment, share): the sums of a share of the segment's tiles. Every thread leaves its own
 // sum of each tile in shared memory; the warps then take a tile each. 256 rows of 128256 bf16 with their
-// fp32 draft probabilities (197 MB) in 51 us, 3.9 TB/s, bound by issue (the weights, and a product and two
-// sums of fp64 an element).
+// fp32 draft probabilities (197 MB) in 53 us, 3.7 TB/s, bound by issue: 40 instructions a 32 elements (the
+// weights, and a product and four sums of fp64).
 template <typename T>
 __global__ void __launch_bounds__(VT, 3) weigh_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
