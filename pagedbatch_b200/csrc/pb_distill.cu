@@ -16,7 +16,7 @@
 // loss from the row's entries. For the tail bucket the entries are kept out of the sums exactly (a bit
 // per element of the segment in shared memory), so S has no cancellation however sure the student is.
 // Backward: one launch, z in and dz out, on the statistics of the forward. Both passes are bound by
-// HBM: V * es bytes a row forward, twice that backward. [4096, 128256] bf16 with a tail, summed: 567 us,
+// HBM: V * es bytes a row forward, twice that backward. [4096, 128256] bf16 with a tail, summed: 560 us,
 // floor 326 us if the backward pass found the logits on chip, 488 us as they are read twice. (A persistent
 // kernel that takes both passes over a few rows at a time, the second from L2, took 570 us: its halves wait
 // for one another.)
@@ -169,8 +169,8 @@ struct GradRow {
 };
 
 // CTA (row, segment): the sums of the segment's exponentials. [4096, 128256] bf16 with a tail (1.05 GB) in
-// 217 us, 4.8 TB/s: its loads stand still while the entries are marked. (Entries matched by each warp for
-// itself, without the marks, took a quarter longer.)
+// 207 us, 5.1 TB/s: no more loads are issued while the entries are marked. (Entries matched by each warp for
+// itself, without the marks, took a quarter longer; four CTAs to an SM without spilled registers, 5%.)
 template <typename T, bool TAIL>
 __global__ void __launch_bounds__(SEG_T, SEG_CTAS) part_kernel(DistillArgs a) {
   constexpr int EPV = Elem<T>::EPV;
@@ -187,52 +187,38 @@ __global__ void __launch_bounds__(SEG_T, SEG_CTAS) part_kernel(DistillArgs a) {
   grid_release();
 
   // mark the segment's entries, while its vectors are on their way
-  int64_t e = tid < a.K ? entry_index(a, row, tid) : -1;
+  const int32_t first = rv.first(v0), e0 = max(0, first), e1 = min(a.V, rv.first(v1));
+  auto place = [&](int i) -> int32_t {  // of entry i in the segment's vectors, or -1
+    const int64_t e = entry_index(a, row, i);
+    return e >= e0 && e < e1 ? (int32_t)e - first : -1;
+  };
+  int32_t b = tid < a.K ? place(tid) : -1;
 #pragma unroll
   for (int w = tid; w < SEG_T * SEG_V * EPV / 32; w += SEG_T) mask[w] = 0;
   marked[tid] = 0;
   if (tid == 0) any_dup = 0;
   __syncthreads();
-  ExpSum mem = expsum_empty();
-  const int32_t e0 = max(0, rv.first(v0)), e1 = min(a.V, rv.first(v1));
   for (int i = tid; i < a.K; i += SEG_T) {
-    if (i != tid) e = entry_index(a, row, i);
-    if (e < e0 || e >= e1) continue;
-    const uint32_t b = (uint32_t)((int32_t)e - rv.first(v0)), v = b / EPV;
-    if ((atomicOr(&mask[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1u) {
-      any_dup = 1;
-    } else if (TAIL) {
-      // the first to mark an element adds its term, which counts once, however many entries name it
-      // (a NaN or +inf logit makes the sum NaN, as in the stream)
-      atomicOr(&marked[v % SEG_T], 1u << (v / SEG_T));
-      const float z = Elem<T>::ld(rv.row + e), m = fmaxf(LOWEST, z);
-      mem = expsum_join(mem, ExpSum{m, ex2((z - m) * a.c)}, a.c);
-    }
+    if (i != tid) b = place(i);
+    if (b < 0) continue;
+    if ((atomicOr(&mask[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1u) any_dup = 1;
+    else if (TAIL) atomicOr(&marked[b / EPV % SEG_T], 1u << (b / EPV / SEG_T));
   }
   __syncthreads();
-  if (TAIL && any_dup) {
-    // which of an element's entries came first above is a matter of chance, and with it the order of the
-    // sums: the terms anew, each by the first of its entries
-    mem = expsum_empty();
-    for (int i = tid; i < a.K; i += SEG_T) {
-      const int64_t ei = entry_index(a, row, i);
-      if (ei < e0 || ei >= e1) continue;
-      bool again = false;
-      for (int j = 0; j < i && !again; ++j) again = entry_index(a, row, j) == ei;
-      if (again) continue;
-      const float z = Elem<T>::ld(rv.row + ei), m = fmaxf(LOWEST, z);
-      mem = expsum_join(mem, ExpSum{m, ex2((z - m) * a.c)}, a.c);
-    }
-  }
-
+  // the entries' elements, each once however many entries name it, leave the vectors for a sum of their own
+  ExpSum mem = expsum_empty();
   if constexpr (TAIL) {
     uint32_t mk = marked[tid];
-    if (mk) {  // an entry's element counts as -inf here
+    if (mk) {
 #pragma unroll
       for (int i = 0; i < SEG_V; ++i) {
         if (!((mk >> i) & 1u)) continue;
-        const uint32_t b = (uint32_t)(tid + i * SEG_T) * EPV;
-        const uint32_t bits = mask[b >> 5] >> (b & 31);
+        const uint32_t at = (uint32_t)(tid + i * SEG_T) * EPV, bits = mask[at >> 5] >> (at & 31) & ((1u << EPV) - 1u);
+        for (uint32_t left = bits; left; left &= left - 1) {
+          // (a NaN or +inf logit makes the sum NaN, as in the stream)
+          const float z = Elem<T>::elem(q[i], __ffs(left) - 1), m = fmaxf(LOWEST, z);
+          mem = expsum_join(mem, ExpSum{m, ex2((z - m) * a.c)}, a.c);
+        }
         uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
 #pragma unroll
         for (int x = 0; x < EPV; ++x) {
