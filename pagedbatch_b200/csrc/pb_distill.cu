@@ -427,9 +427,8 @@ int check(const DistillArgs& a, int es, int64_t vocab, float temperature) {
   if (!a.z || !a.lp || !a.idx || !a.stats) return PB_E_INVALID;
   if (a.n > (int64_t)(0x7FFFFFFF / 8)) return PB_E_INVALID;
   if (a.z_stride < 0 || a.lp_stride < 0 || a.idx_stride < 0) return PB_E_INVALID;
-  if (reinterpret_cast<uintptr_t>(a.z) % es) return PB_E_INVALID;
-  if (reinterpret_cast<uintptr_t>(a.stats) & 15) return PB_E_INVALID;
-  if ((reinterpret_cast<uintptr_t>(a.idx) % (a.idx64 ? 8 : 4)) || (reinterpret_cast<uintptr_t>(a.lp) & 3))
+  if (!aligned(a.z, es) || !aligned(a.stats, 16) || !aligned(a.idx, a.idx64 ? 8 : 4) || !aligned(a.lp, 4) ||
+      !aligned(a.weight, 4) || !aligned(a.loss, 4) || !aligned(a.grad, 4) || !aligned(a.dz, es))
     return PB_E_INVALID;
   return PB_OK;
 }
@@ -469,7 +468,7 @@ int pb_distill_forward(const void* logits, int dtype, int64_t n_rows, int64_t vo
   a.K = n_entries;
   const int rc = check(a, es, vocab, temperature);
   if (rc != PB_OK || n_rows == 0) return rc;
-  if (!out_loss || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)) return PB_E_INVALID;
+  if (!out_loss || !workspace || !aligned(workspace, 16)) return PB_E_INVALID;
   if (ws_bytes < pb_distill_ws_bytes(n_rows, vocab, dtype)) return PB_E_INVALID;
   a.parts = static_cast<Part*>(workspace);
   a.c = (float)(1.4426950408889634 / (double)temperature);
@@ -505,7 +504,6 @@ int pb_distill_backward(const void* logits, int dtype, int64_t n_rows, int64_t v
   const int rc = check(a, es, vocab, temperature);
   if (rc != PB_OK || n_rows == 0) return rc;
   if (!grad_loss || !out_grad || grad_stride < 0) return PB_E_INVALID;
-  if (reinterpret_cast<uintptr_t>(out_grad) % es) return PB_E_INVALID;
   a.c = (float)(1.4426950408889634 / (double)temperature);
   a.inv_tau = 1.0f / temperature;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -515,7 +513,7 @@ int pb_distill_backward(const void* logits, int dtype, int64_t n_rows, int64_t v
 }
 
 int pb_distill_sum(const float* loss, int64_t n_rows, float* out_sum, void* stream) {
-  if (n_rows < 0 || !out_sum || (n_rows && !loss)) return PB_E_INVALID;
+  if (n_rows < 0 || !out_sum || (n_rows && !loss) || !aligned(loss, 4) || !aligned(out_sum, 4)) return PB_E_INVALID;
   distill_sum_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(loss, n_rows, out_sum);
   return cudaGetLastError() == cudaSuccess ? PB_OK : PB_E_LAUNCH;
 }

@@ -320,6 +320,9 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 
 // ---- host side -------------------------------------------------------------------------------
 
+// Whether an array of elements of `size` bytes can start at p (null: there is none).
+inline bool aligned(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+
 inline int elem_size(int dtype) {
   return (dtype == PB_DTYPE_F32) ? 4 : (dtype == PB_DTYPE_BF16 || dtype == PB_DTYPE_F16) ? 2 : 0;
 }

@@ -419,9 +419,9 @@ int pb_top_logprobs(const void* logits, int dtype, int64_t n_rows, int64_t vocab
   if (n_rows == 0) return PB_OK;
   if (!logits || !out_logprob || !out_index || !out_lse) return PB_E_INVALID;
   if (n_rows > (int64_t)(0x7FFFFFFF / 8)) return PB_E_INVALID;
-  if (reinterpret_cast<uintptr_t>(logits) % es) return PB_E_INVALID;
+  if (!aligned(logits, es) || !aligned(out_logprob, 4) || !aligned(out_index, 4) || !aligned(out_lse, 4)) return PB_E_INVALID;
   const TopPlan plan = top_plan(n_rows, vocab, es, logits, row_stride);
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || ws_bytes < plan.bytes) return PB_E_INVALID;
+  if (!workspace || !aligned(workspace, 256) || ws_bytes < plan.bytes) return PB_E_INVALID;
   TopArgs a;
   a.x = logits;
   a.row_stride = row_stride;

@@ -1601,15 +1601,17 @@ int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int6
   if (!logits || !params || !row_offsets || !drafts || !uniforms || !out_tokens || !out_accepted || !workspace)
     return PB_E_INVALID;
   if (n_rows > (1 << 28) || n_seqs > n_rows) return PB_E_INVALID;
-  if (reinterpret_cast<uintptr_t>(logits) % es) return PB_E_INVALID;
+  if (!aligned(logits, es) || !aligned(params, 8) || !aligned(row_offsets, 4) || !aligned(drafts, 8) ||
+      !aligned(uniforms, 8) || !aligned(out_tokens, 8) || !aligned(out_accepted, 4) || !aligned(out_status, 4))
+    return PB_E_INVALID;
   if (draft_probs) {
     const int ps = elem_size(probs_dtype);
-    if (!ps || probs_stride < vocab || reinterpret_cast<uintptr_t>(draft_probs) % ps) return PB_E_INVALID;
+    if (!ps || probs_stride < vocab || !aligned(draft_probs, ps)) return PB_E_INVALID;
   }
   if (kinds < 0 || kinds > PB_VERIFY_ANY) return PB_E_INVALID;
   const int k = kinds ? kinds : PB_VERIFY_ANY;
   const VerifyPlan plan = verify_plan(n_rows, n_seqs, vocab, dtype, k);
-  if ((reinterpret_cast<uintptr_t>(workspace) & 255) || ws_bytes < plan.bytes) return PB_E_INVALID;
+  if (!aligned(workspace, 256) || ws_bytes < plan.bytes) return PB_E_INVALID;
   VerifyArgs a = {};
   a.x = logits;
   a.row_stride = row_stride;

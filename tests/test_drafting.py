@@ -144,6 +144,34 @@ def test_c_abi_refusals(lib):
     assert lib.pb_distill_stats_bytes(-1) == -1 and lib.pb_distill_stats_bytes(3) == 96
 
 
+def test_misaligned_arrays_are_refused(lib):
+    """Arrays that do not start on their elements' size, as a slice of a byte buffer may."""
+    b = np.zeros(4096, np.uint8)
+    base = (b.ctypes.data + 255) & ~255  # nothing reads it
+    ws = lib.pb_verify_ws_bytes(2, 1, 8, 0, 0)
+    ok = [base, 0, 2, 8, 8, base, 1, base, base, base, None, 0, 1, 8, 0, base, base, None, base, ws, None]
+    for at, off in ((5, 1), (5, 4), (7, 2), (8, 4), (9, 4), (15, 4), (16, 1), (17, 2)):
+        a = list(ok)
+        a[at] = base + off
+        assert lib.pb_verify(*a) == -1, at
+    ok = [base, 0, 2, 8, 8, 2, 1.0, base, base, base, base, 1 << 20, None]
+    for at in (7, 8, 9):
+        a = list(ok)
+        a[at] = base + 2
+        assert lib.pb_top_logprobs(*a) == -1, at
+    ok = [base, 0, 2, 8, 8, base, 2, base, 2, 4, 2, 1.0, 0, None, base, base, base, 1 << 20, None]
+    for at in (5, 7, 13, 14, 15, 16):
+        a = list(ok)
+        a[at] = base + 2
+        assert lib.pb_distill_forward(*a) == -1, at
+    ok = [base, 0, 2, 8, 8, base, 2, base, 2, 4, 2, 1.0, None, base, base, 1, base, None]
+    for at in (5, 7, 12, 13, 14, 16):
+        a = list(ok)
+        a[at] = base + 2
+        assert lib.pb_distill_backward(*a) == -1, at
+    assert lib.pb_distill_sum(base + 2, 2, base, None) == -1 and lib.pb_distill_sum(base, 2, base + 1, None) == -1
+
+
 def test_kinds_of_sequences():
     def kinds(t, p, k):
         return ops.row_kinds(ops.pack_params(t, p, k, [0.0] * len(t)))
