@@ -305,6 +305,15 @@ def test_types_of_the_record(cuda):
         assert torch.equal(a, pb.distill_loss(z.cuda(), lp.to(dtype).float().cuda(), idx.cuda()))
 
 
+def test_differentiates_once(cuda):
+    z = torch.randn(4, 100, device="cuda", requires_grad=True)
+    lp, idx = entries(z.detach().cpu(), 5, 1)
+    loss = pb.distill_loss(z, lp.cuda(), idx.cuda(), reduction="sum")
+    (g,) = torch.autograd.grad(loss, z, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_repeated_entries_give_the_same_bits(cuda, dtype):
     """However the threads meet at an element that several entries name."""
