@@ -107,6 +107,13 @@ __device__ __forceinline__ uint4 pack_vec(const float* x) {
   }
 }
 
+// Element x of a vector, from the word that holds it.
+template <typename T>
+__device__ __forceinline__ float word_elem(uint32_t v, int x) {
+  if constexpr (Elem<T>::EPV == 4) return __uint_as_float(v);
+  else return Elem<T>::elem(make_uint4(v, 0u, 0u, 0u), x & 1);
+}
+
 // A row's gradient: where it goes, and its scale g.
 template <typename T>
 struct GradRow {
@@ -214,17 +221,20 @@ __global__ void __launch_bounds__(SEG_T, SEG_CTAS) part_kernel(DistillArgs a) {
       for (int i = 0; i < SEG_V; ++i) {
         if (!((mk >> i) & 1u)) continue;
         const uint32_t at = (uint32_t)(tid + i * SEG_T) * EPV, bits = mask[at >> 5] >> (at & 31) & ((1u << EPV) - 1u);
-        for (uint32_t left = bits; left; left &= left - 1) {
-          // (a NaN or +inf logit makes the sum NaN, as in the stream)
-          const float z = Elem<T>::elem(q[i], __ffs(left) - 1), m = fmaxf(LOWEST, z);
-          mem = expsum_join(mem, ExpSum{m, ex2((z - m) * a.c)}, a.c);
-        }
         uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-#pragma unroll
-        for (int x = 0; x < EPV; ++x) {
+#pragma unroll 1
+        for (uint32_t left = bits; left; left &= left - 1) {
+          const int x = __ffs(left) - 1, word = (EPV == 4) ? x : x >> 1;
           const uint32_t part = (EPV == 4) ? 0xFFFFFFFFu : 0xFFFFu << (16 * (x & 1));
-          uint32_t& word = w[(EPV == 4) ? x : x >> 1];
-          if ((bits >> x) & 1u) word = (word & ~part) | (Elem<T>::NEG_INF_WORD & part);
+          uint32_t v = w[0];
+#pragma unroll
+          for (int j = 1; j < 4; ++j) v = word == j ? w[j] : v;
+          // (a NaN or +inf logit makes the sum NaN, as in the stream)
+          const float z = word_elem<T>(v, x), m = fmaxf(LOWEST, z);
+          mem = expsum_join(mem, ExpSum{m, ex2((z - m) * a.c)}, a.c);
+          v = (v & ~part) | (Elem<T>::NEG_INF_WORD & part);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = word == j ? v : w[j];
         }
         q[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
