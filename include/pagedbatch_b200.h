@@ -289,16 +289,17 @@ PB_API int pb_stop_check(const int64_t* tokens, int64_t n_rows, const int32_t* r
  *   out_status   optional device int32[n_seqs]: PB_ROW_* of the row where the sequence stopped.
  *
  * Semantics, per row, with P_i = q_i on the kept set of pb_sample's rule, Z = sum P (kept_q), x the
- * draft, u = floor(uniform * 2^53) / 2^53 and D_i the draft distribution (D_x = 1 without one):
+ * draft, u the row's uniform as given and D_i the draft distribution (D_x = 1 without one):
  *   accept x iff (u * D_x) * Z < P_x, in fp64, every conversion and product rounded to nearest
  *   (greedy rows: iff x is the row's first maximum; a draft outside [0, vocab) is never accepted);
  *   at the first row that does not accept, draw from max(0, P_i - floor(D_i * Z)) (fp64 product; 0
  *   for D_i <= 0 or NaN), or without a distribution from P without x; with every draft accepted
  *   draw from P at the last row; where those weights are all 0, from P.
  *   draw: the first index, ascending, whose inclusive prefix of the weights exceeds
- *   floor(u * 2^53 * sum / 2^53), u of the sequence's last row (the sampler draws in the order of falling probability instead).
- * workspace: pb_verify_ws_bytes(n_rows, n_seqs, vocab, dtype, kinds) bytes of device memory, 256-byte aligned, of any
- * content, not used by another call while this one runs.
+ *   floor(floor(u * 2^53) * sum / 2^53), u of the sequence's last row (the sampler draws in the order of
+ *   falling probability instead).
+ * workspace: pb_verify_ws_bytes(n_rows, n_seqs, vocab, dtype, kinds) bytes of device memory, 256-byte
+ * aligned, of any content, not used by another call while this one runs.
  */
 #define PB_VERIFY_SMALL 1 /* greedy, or 0 < top_k <= 128 */
 #define PB_VERIFY_WHOLE 2 /* neither top-k nor top-p */

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(TT, SEG_CTAS) part_kernel(TopArgs a) {
 }
 
 // A CTA per row, as above. Latency (the keys, the bound, the groups, the order, each after the one before),
-// 592 rows at a time: 9 us for 256 rows of k 50, 31 us for 1024 of k 128. (Six CTAs to an SM did not shorten
+// 592 rows at a time: 9 us for 256 rows of k 50, 30 us for 1024 of k 128. (Six CTAs to an SM did not shorten
 // it.)
 template <typename T>
 __global__ void __launch_bounds__(TT, 4) select_kernel(TopArgs a) {
