@@ -909,7 +909,8 @@ __device__ int32_t draw_listed(const DrawRow<T>& row, const GroupKeys& g, int64_
     for (int j = 0; j < PER; ++j) {
       if (p[j]) {
         uint64_t taken = 0;
-        if (row.dist) taken = grid_units(row.taken_by(fminf(d[j], row.d_most)));
+        // (NaN is 0 before the bound, which would take all of the weight in its place)
+        if (row.dist) taken = grid_units(row.taken_by(fminf(fmaxf(d[j], 0.0f), row.d_most)));
         else if (row.residual && sh.sorted[i0 + j] == row.dx) taken = p[j];
         r[j] = p[j] > taken ? p[j] - taken : 0;
       }

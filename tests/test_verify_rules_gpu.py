@@ -1,0 +1,49 @@
+"""Corners of the verification's rule on a B200, against its restatement (oracle/verify.py), token for token."""
+
+import numpy as np
+import pytest
+import torch
+
+from pagedbatch_b200 import workloads
+from test_verify_gpu import _check, _probs
+
+pytestmark = pytest.mark.gpu
+
+
+def _view(x, shift):
+    """The rows on the device, `shift` elements past a 16-byte boundary."""
+    buf = torch.zeros(len(x), (x.shape[1] + 31) // 16 * 16, dtype=x.dtype, device="cuda")
+    view = buf[:, shift : shift + x.shape[1]]
+    view.copy_(x)
+    return view
+
+
+def _rejected(x):
+    """A draft per row that no parameters with a filter keep: the row's smallest value."""
+    return x.float().argmin(1).numpy().astype(np.int64)
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,spread", [(256, 3.0), (4096, 3.0), (4096, 0.0)])
+def test_odd_values_at_some_of_the_kept_tokens(cuda, dtype, V, spread, shift):
+    """NaN and negative draft probabilities take nothing of a token's weight, infinite ones all of it,
+    whichever launch draws: few values near the kept ones, many equal ones (spread 0), rows of any alignment."""
+    S, n = 48, 1
+    g = torch.Generator().manual_seed(V)
+    x = workloads.head_boosted(2 * S, V, seed=V, dtype=dtype)
+    if not spread:
+        x = torch.randint(-1, 2, (2 * S, V), generator=g).to(dtype)
+        x[:, 0] = -3.0
+    params = [((1.0, 0.7)[s % 2], (1.0, 0.95)[s // 2 % 2], (5, 20, 50, 128)[s // 4 % 4]) for s in range(S)]
+    probs = _probs(x, [n] * S, params, 1)
+    top = torch.topk(x[0::2].float(), 40, dim=1).indices
+    for j, odd in enumerate((torch.nan, -torch.inf, -0.5, torch.inf, torch.nan)):
+        at = top[:, torch.randperm(40, generator=g)[:8]]
+        probs.scatter_(1, at, odd)
+    probs[:, 0] = 0.1  # (the draft's own is an ordinary one where it is token 0)
+    drafts = _rejected(x)
+    for seed in range(4):
+        u = np.random.default_rng(seed).random(2 * S)
+        u[0::2] = 1.0 - 2.0**-53
+        _check(x, params, [n] * S, drafts, u, probs, view=_view(x, shift))
