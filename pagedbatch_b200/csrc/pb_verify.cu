@@ -176,7 +176,10 @@ __device__ __forceinline__ float surely_below(uint32_t thr, float tf) {
 // two elements at a time:
 //  * x / T: a product with the exact reciprocal of a power of two, else by Markstein's division
 //    (IBM J. Res. Dev. 34, 1990): with y = RN(1 / T), two corrections q += (x - q T) y, the remainders
-//    exact in one fused operation each, give RN(x / T) while nothing over- or underflows;
+//    exact in one fused operation each, give RN(x / T) while nothing over- or underflows. Values of
+//    |x| < 2^-100 (a remainder may lie below the subnormals) or |x / T| < 2^-126 can miss a last bit. They
+//    are below 2^-40 of the row's largest, so RN(y - max) is -max all the same and no weight sees it; a
+//    comparison with the last kept key does, and rows whose cut is as near to 0 are not `fast` (DrawRow);
 //  * keys further than 40 below the maximum, whose weight is below 2^-40, are taken as 40 below it.
 struct Weigher {
   float t, recip, inv, m;
@@ -650,6 +653,8 @@ struct DrawRow {
     // (a key more than 28 below the largest has no weight, kept or not: masked values among a top-k)
     raw_lo = fmaxf(surely_below(f.thr_key, tf), surely_below(key_of(f.max_key - 28.0f), tf));
     thr = value_of(f.thr_key);
+    // (the quotients that the packed steps may miss are below 2^-60, as T >= 2^-40)
+    if (fabsf(thr) < 0x1p-59f) weigh.fast = false;
     z = __ull2double_rn(f.kept_q) * 0x1p-40;
     d_most = 2048.0f / (float)z;  // (anywhere between 1 / Z and 4095 / Z would do)
   }

@@ -47,3 +47,23 @@ def test_odd_values_at_some_of_the_kept_tokens(cuda, dtype, V, spread, shift):
         u = np.random.default_rng(seed).random(2 * S)
         u[0::2] = 1.0 - 2.0**-53
         _check(x, params, [n] * S, drafts, u, probs, view=_view(x, shift))
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("low,high", [(-149, -126), (-128, -120), (-126, -100), (-60, -20)])
+def test_cuts_next_to_zero(cuda, dtype, low, high, shift):
+    """One ordinary value and the rest next to zero, where top-k or top-p cuts: x / T in one rounding decides
+    which of them are kept, quotients below the normal numbers included."""
+    S, V = 120, 4096
+    g = torch.Generator().manual_seed(-low)
+    e = torch.randint(low, high + 1, (S, V), generator=g).double()
+    x = torch.ldexp(1.0 + torch.rand(S, V, generator=g, dtype=torch.float64), e)
+    x *= torch.where(torch.rand(S, V, generator=g) < 0.5, -1.0, 1.0)
+    x[1::3] = x[1::3, torch.randint(0, 40, (V,), generator=g)]  # rows of few values, many equal
+    x[torch.arange(S), torch.randint(0, V, (S,), generator=g)] = 1.0
+    x = x.to(dtype)
+    for k, p in ((50, 1.0), (128, 0.7), (300, 1.0), (1500, 0.8), (0, 0.4), (0, 0.9)):
+        params = [((0.7, 1.3, 3.0, 1.9999999)[s % 4], p, k) for s in range(S)]
+        u = np.random.default_rng(k).random(S)
+        _check(x, params, [0] * S, np.zeros(S, np.int64), u, view=_view(x, shift))
