@@ -1125,8 +1125,9 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
             if (row_is == ROW_WHOLE) {
               // (what fp64's own roundings add is far below the bounds' slack)
               const Mass z = mass_near(a, r, tf, value_of(a.meta[r].max_key), f.max_key);
-              ok = want * z.lo < p;
-              if (ok && !(want * z.hi < p)) ev = EV_TIE;
+              // (a negative product is below any weight; with no lower bound on the mass it would not show)
+              ok = want < 0.0 || want * z.lo < p;
+              if (ok && !(want < 0.0) && !(want * z.hi < p)) ev = EV_TIE;
             } else {
               ok = __dmul_rn(want, __ull2double_rn(f.kept_q)) < p;
               if (ev == EV_TIE && !ok) ev = EV_REJECT;  // rejected either way

@@ -67,3 +67,15 @@ def test_cuts_next_to_zero(cuda, dtype, low, high, shift):
         params = [((0.7, 1.3, 3.0, 1.9999999)[s % 4], p, k) for s in range(S)]
         u = np.random.default_rng(k).random(S)
         _check(x, params, [0] * S, np.zeros(S, np.int64), u, view=_view(x, shift))
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0**-19, 2.0**-22, 1e-12])
+def test_negative_shares_of_drafts_without_weight(cuda, temperature):
+    """u D Z < P holds for a negative D whatever P is, however little is known of the mass before it is summed."""
+    S, V = 8, 4099
+    x = workloads.head_boosted(2 * S, V, seed=3)
+    probs = torch.full((S, V), 1.0 / V)
+    drafts = _rejected(x)
+    probs[torch.arange(S), torch.from_numpy(drafts[0::2])] = torch.tensor([-0.5, -1e-30, 0.0, 0.5, -torch.inf, torch.nan, -1.0, 1e-30])
+    for u in (0.0, 2.0**-53, 0.5, 1.0 - 2.0**-53):
+        _check(x, [(temperature, 1.0, 0)] * S, [1] * S, drafts, np.full(2 * S, u), probs)
