@@ -108,16 +108,28 @@ def row_kinds(rec: np.ndarray) -> tuple[int, int]:
 def mark_rows(params: torch.Tensor, rec: np.ndarray) -> torch.Tensor:
     """Record on the device params tensor which launch suits its rows (read by the path choice)."""
     params._pb_group_rows = group_rows(rec)
-    params._pb_kinds = row_kinds(rec)
     return params
+
+
+def noted_kinds(params: torch.Tensor) -> tuple[int, int]:
+    """``row_kinds`` of the records a params tensor was uploaded from, (0, 0) where they are not known. Found
+    when a verification first asks: the sampler, which uploads records every step, has no use for them."""
+    kinds = getattr(params, "_pb_kinds", None)
+    if kinds is None:
+        rec = getattr(params, "_pb_records", None)
+        kinds = params._pb_kinds = (0, 0) if rec is None else row_kinds(rec)
+    return kinds
 
 
 def params_tensor(rec: np.ndarray, device, pinned: bool = True) -> torch.Tensor:
     """Upload packed records: one pinned host buffer, one non-blocking H2D copy."""
-    host = torch.from_numpy(rec.view(np.uint8).copy())
+    rec = rec.copy()
+    host = torch.from_numpy(rec.view(np.uint8))
     if pinned:
         host = host.pin_memory()
-    return mark_rows(host.to(device, non_blocking=True), rec)
+    params = mark_rows(host.to(device, non_blocking=True), rec)
+    params._pb_records = rec
+    return params
 
 
 _WS: dict = {}

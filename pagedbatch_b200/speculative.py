@@ -26,12 +26,12 @@ from .sampling import _INVALID_DISTRIBUTION, pack_rows
 __all__ = ["verify", "verify_tokens"]
 
 
-def _kinds(params: torch.Tensor, vocab: int) -> int:
-    bits, kmax = getattr(params, "_pb_kinds", (0, 0))
+def _kinds(noted: tuple[int, int], vocab: int) -> int:
+    bits, kmax = noted
     return bits if kmax < vocab else 0  # a top_k of the vocabulary or more is no filter: any kind
 
 
-def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs):
+def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=None):
     if not logits.is_cuda:
         raise ValueError("pagedbatch_b200.verify needs CUDA logits; move the tensor with .cuda() first")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
@@ -68,7 +68,7 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs):
     with ops.on_device(dev):
         # a buffer of this call's own: the allocator hands it on in stream order, and a captured
         # graph keeps its copy
-        kinds = _kinds(params, V)
+        kinds = _kinds(ops.noted_kinds(params) if noted is None else noted, V)
         n_ws = L.pb_verify_ws_bytes(R, S, V, code, kinds)
         ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
         rc = L.pb_verify(
@@ -166,8 +166,8 @@ def verify_tokens(logits: torch.Tensor, drafts: Sequence[Sequence[int]], params:
     np.concatenate(parts, out=host.numpy())
     dev = host.to(logits.device, non_blocking=True)
     tokens, accepted, status = _launch(
-        logits, ops.mark_rows(dev[: ends[0]], rec), dev[ends[1] : ends[2]].view(torch.int64),
-        dev[ends[2] : ends[3]].view(torch.int32), dev[ends[0] : ends[1]].view(torch.float64), draft_probs)
+        logits, dev[: ends[0]], dev[ends[1] : ends[2]].view(torch.int64), dev[ends[2] : ends[3]].view(torch.int32),
+        dev[ends[0] : ends[1]].view(torch.float64), draft_probs, ops.row_kinds(rec))
     got, n_ok, st = tokens.tolist(), accepted.tolist(), status.tolist()
     for s, code in enumerate(st):
         if code == _lib.ROW_NONFINITE:
