@@ -281,7 +281,9 @@ PB_API int pb_stop_check(const int64_t* tokens, int64_t n_rows, const int32_t* r
  *                rows (row r of sequence s has draft_probs row r - s). Null: a draft is certain (its
  *                distribution is one token), as drafts looked up in the prompt are.
  *   kinds        which kinds of sequences the batch holds (PB_VERIFY_*, 0: any): a launch whose kind
- *                is absent is left out. A sequence of a kind not named reports PB_ROW_INTERNAL.
+ *                is absent is left out. A sequence of a kind not named reports PB_ROW_INTERNAL, or with
+ *                PB_VERIFY_REST added is verified as any other, only slower: for calls whose parameters
+ *                may have changed since they were looked at (a captured one's, before each replay).
  *   out_tokens   device int64[n_rows]: from the sequence's first row on, its accepted drafts and the
  *                token drawn after them, then -1. A sequence whose status is not PB_ROW_OK has no
  *                drawn token (-1 there).
@@ -306,6 +308,7 @@ PB_API int pb_stop_check(const int64_t* tokens, int64_t n_rows, const int32_t* r
 #define PB_VERIFY_OTHER 4 /* any other parameters */
 #define PB_VERIFY_TOPP 8  /* top-p alone */
 #define PB_VERIFY_ANY 15
+#define PB_VERIFY_REST 16 /* beside others: kinds that are not named may occur as well */
 PB_API int64_t pb_verify_ws_bytes(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype, int kinds);
 PB_API int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
                      const pb_row_params* params, int64_t n_seqs, const int32_t* row_offsets, const int64_t* drafts,

@@ -24,7 +24,7 @@ ROW_FALLBACK = 32
 CAND_FALLBACK, CAND_GREEDY, CAND_MAX_CAP = 0x100, 0x200, 2048
 PATH_GREEDY, PATH_SMALL, PATH_LARGE, PATH_STREAM = 1, 2, 4, 8
 FINISH_NONE, FINISH_STOP, FINISH_LENGTH = 0, 1, 2
-VERIFY_SMALL, VERIFY_WHOLE, VERIFY_OTHER, VERIFY_TOPP, VERIFY_ANY = 1, 2, 4, 8, 15
+VERIFY_SMALL, VERIFY_WHOLE, VERIFY_OTHER, VERIFY_TOPP, VERIFY_ANY, VERIFY_REST = 1, 2, 4, 8, 15, 16
 TOP_MAX = 256
 DISTILL_MAX_ENTRIES, DISTILL_MAX_VOCAB = 1024, 1 << 20
 MAX_VOCAB = 1 << 24

@@ -99,6 +99,7 @@ struct VerifyArgs {
   int32_t share;                 // tiles per CTA of weigh_kernel: TILES, or its half, quarter or eighth
   GroupKeys groups;              // of the rows the sampler settled (keys null: none)
   int32_t kinds;                 // PB_VERIFY_* of the batch, as the caller names them
+  int32_t rest;                  // what settles rows of other kinds (ROW_SMALL, ROW_OTHER), or -1
   int32_t one_kind;              // ROW_WHOLE or ROW_MASS where every row is of that kind, else -1
   int64_t* out_tokens;           // [n_rows]
   int32_t* out_accepted;         // [n_seqs]
@@ -111,6 +112,20 @@ __device__ __forceinline__ int32_t row_kind(const pb_row_params& p, int32_t V) {
   if (p.temperature == 0.0) return ROW_SMALL;
   if (p.top_k > 0 && p.top_k < V) return p.top_k <= SMALL_K ? ROW_SMALL : ROW_OTHER;
   return (float)p.top_p < 1.0f ? ROW_MASS : ROW_WHOLE;
+}
+
+// The launches that settle rows of a kind, as the caller names them (the one for other kinds takes top-p's
+// too), and what settles a sequence's rows in this call.
+__device__ __forceinline__ int32_t takes(int32_t kind) {
+  return kind == ROW_SMALL  ? PB_VERIFY_SMALL
+         : kind == ROW_WHOLE ? PB_VERIFY_WHOLE
+         : kind == ROW_MASS  ? PB_VERIFY_TOPP | PB_VERIFY_OTHER
+                             : PB_VERIFY_OTHER;
+}
+template <bool REST>
+__device__ __forceinline__ int32_t settled_as(const VerifyArgs& a, const pb_row_params& p) {
+  const int32_t kind = row_kind(p, a.V);
+  return REST && !(a.kinds & takes(kind)) ? a.rest : kind;
 }
 
 // Each row's parameters, from its sequence's (a binary search over the offsets, which are brought into shared
@@ -136,14 +151,15 @@ __global__ void __launch_bounds__(256) expand_kernel(VerifyArgs a) {
   pb_row_params p = a.params[lo];
   p.uniform = 0.0;  // the sampler's own draw is not used
   p.rng = 0;
-  const int32_t kind = row_kind(p, a.V);
+  const int32_t kind = a.rest >= 0 ? settled_as<true>(a, p) : settled_as<false>(a, p);
   a.meta[r] = RowMeta{(float)p.temperature, kind, 0u, 0u, 0ull, 0ull, 0, (float)p.top_p};
   a.rowq[r] = p;
   // rows of other kinds pass through pb_sample_ws as greedy ones, its cheapest
   if (kind != ROW_SMALL) p.temperature = 0.0, p.top_p = 1.0, p.top_k = 0;
   a.rowp[r] = p;
   pb_row_info* o = a.info + r;
-  o->status = PB_ROW_INTERNAL;  // until a launch settles the row
+  // until a launch settles the row: the sampler's cluster kernel, or (a kind that no launch is for) none
+  o->status = kind == ROW_OTHER && a.rest == ROW_OTHER ? PB_ROW_FALLBACK : PB_ROW_INTERNAL;
   o->z_q = o->kept_q = 0;
   a.tok[r] = -1;
   a.out_tokens[r] = -1;
@@ -1018,8 +1034,9 @@ __device__ __noinline__ int32_t draw_near(const DrawRow<T>& row, const GroupKeys
 // A CTA per sequence: the first row that is not accepted, its accepted tokens, and for sequences whose
 // rows' group keys are known the draw. Latency: 10 us for 256 sequences without draws here, 15 us for 64
 // that draw from their top-k rows (the groups' list, their values, the weights: each waits for the one
-// before). With the draws left to weigh_kernel and draw_kernel that call took 106 us instead of 65 us.
-template <typename T>
+// before). With the draws left to weigh_kernel and draw_kernel that call took 106 us instead of 65 us. REST: rows
+// of kinds that are not named may occur. (One kernel for both took 1.4 us more.)
+template <typename T, bool REST>
 __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
   constexpr int EPV = Elem<T>::EPV;
   __shared__ struct {
@@ -1059,11 +1076,9 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
     return d;
   };
   const Draft first = draft_of(lo + tid);
-  // whether a launch settles rows of this kind (the one for other kinds takes top-p's too)
-  const int32_t row_is = row_kind(p, a.V);
-  const int32_t takes = row_is == ROW_SMALL ? PB_VERIFY_SMALL : row_is == ROW_WHOLE ? PB_VERIFY_WHOLE
-                        : row_is == ROW_MASS ? PB_VERIFY_TOPP | PB_VERIFY_OTHER : PB_VERIFY_OTHER;
-  const bool settled = (a.kinds & takes) != 0;
+  // whether a launch settles rows of this kind
+  const int32_t row_is = settled_as<REST>(a, p);
+  const bool settled = REST || (a.kinds & takes(row_is)) != 0;
   const double u_draw = lo < hi ? a.uniforms[hi - 1] : 0.0;
   grid_wait();  // the rows' records
   if (lo >= hi) {  // a sequence without rows
@@ -1541,7 +1556,8 @@ VerifyPlan verify_plan(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype,
 }
 
 template <typename T>
-int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan& plan, cudaStream_t st) {
+int verify_run(VerifyArgs a, int dtype, int named, uint8_t* ws, const VerifyPlan& plan, cudaStream_t st) {
+  const int kinds = named & PB_VERIFY_ANY;
   a.rowp = reinterpret_cast<pb_row_params*>(ws + plan.rowp);
   a.rowq = reinterpret_cast<pb_row_params*>(ws + plan.rowq);
   a.info = reinterpret_cast<pb_row_info*>(ws + plan.info);
@@ -1556,9 +1572,14 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
   }
   a.seg = seg_plan(a.V, sizeof(T), a.x, a.row_stride);
   a.kinds = kinds;
+  // rows of kinds that are not named: by the cluster kernel where it is launched, else by the sampler's launches
+  // (which settle any row) where they are
+  const bool general = (kinds & (PB_VERIFY_TOPP | PB_VERIFY_OTHER)) != 0;
+  a.rest = !(named & PB_VERIFY_REST) ? -1 : !general && (kinds & PB_VERIFY_SMALL) ? ROW_SMALL : ROW_OTHER;
   a.one_kind = kinds == PB_VERIFY_WHOLE ? ROW_WHOLE : kinds == PB_VERIFY_TOPP ? ROW_MASS : -1;
   const dim3 rows((unsigned)a.n_rows, (unsigned)a.seg.segs), each_row((unsigned)a.n_rows);
   const dim3 seqs((unsigned)a.n_seqs), parts((unsigned)a.n_seqs, (unsigned)a.seg.segs);
+  auto fallback = [&] { return sample_fallback_rows(a.x, dtype, a.n_rows, a.V, a.row_stride, a.rowq, a.tok, a.info, st); };
   expand_kernel<<<(unsigned)((a.n_rows + 255) / 256), 256, 0, st>>>(a);
   int rc = cudaGetLastError() == cudaSuccess ? PB_OK : PB_E_LAUNCH;
   if (rc == PB_OK && (kinds & PB_VERIFY_SMALL)) {
@@ -1569,18 +1590,19 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
                                       ws + plan.sampler, plan.bytes - plan.sampler, st)
                        : pb_sample(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr, st);
   }
+  // (before the pass over whole rows, which the launches after it overlap with)
+  if (rc == PB_OK && a.rest == ROW_OTHER && !general) rc = fallback();
   if (rc == PB_OK && (kinds & (PB_VERIFY_WHOLE | PB_VERIFY_TOPP))) rc = launch_after(max_kernel<T>, a, rows, VT, st);
   if (rc == PB_OK && (kinds & PB_VERIFY_TOPP)) {
     rc = launch_after(hist_kernel<T>, a, rows, VT, st);
     if (rc == PB_OK) rc = launch_after(cut_kernel, a, each_row, VT, st);
     if (rc == PB_OK) rc = launch_after(gather_kernel<T>, a, rows, VT, st);
   }
-  if (rc == PB_OK && (kinds & (PB_VERIFY_TOPP | PB_VERIFY_OTHER))) {
+  if (rc == PB_OK && general) {
     rc = launch_after(order_kernel, a, each_row, VT, st);
-    if (rc == PB_OK)
-      rc = sample_fallback_rows(a.x, dtype, a.n_rows, a.V, a.row_stride, a.rowq, a.tok, a.info, st);
+    if (rc == PB_OK) rc = fallback();
   }
-  if (rc == PB_OK) rc = launch_after(decide_kernel<T>, a, seqs, VT, st);
+  if (rc == PB_OK) rc = launch_after(a.rest >= 0 ? decide_kernel<T, true> : decide_kernel<T, false>, a, seqs, VT, st);
   // (a batch whose every sequence draws in decide_kernel needs no more)
   if (rc != PB_OK || (kinds == PB_VERIFY_SMALL && a.groups.keys)) return rc;
   if (kinds & PB_VERIFY_WHOLE) rc = launch_after(mass_kernel<T>, a, parts, VT, st);
@@ -1594,12 +1616,15 @@ int verify_run(VerifyArgs a, int dtype, int kinds, uint8_t* ws, const VerifyPlan
   return rc;
 }
 
+// 0, or some kinds with or without PB_VERIFY_REST.
+bool kinds_ok(int kinds) { return kinds == 0 || (kinds > 0 && kinds <= (PB_VERIFY_ANY | PB_VERIFY_REST) && (kinds & PB_VERIFY_ANY)); }
+
 }  // namespace
 
 extern "C" {
 
 int64_t pb_verify_ws_bytes(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype, int kinds) {
-  if (n_rows < 0 || n_seqs < 0 || vocab <= 0 || !elem_size(dtype) || kinds < 0 || kinds > PB_VERIFY_ANY) return PB_E_INVALID;
+  if (n_rows < 0 || n_seqs < 0 || vocab <= 0 || !elem_size(dtype) || !kinds_ok(kinds)) return PB_E_INVALID;
   return verify_plan(n_rows, n_seqs, vocab, dtype, kinds ? kinds : PB_VERIFY_ANY).bytes;
 }
 
@@ -1623,7 +1648,7 @@ int pb_verify(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int6
     const int ps = elem_size(probs_dtype);
     if (!ps || probs_stride < vocab || !aligned(draft_probs, ps)) return PB_E_INVALID;
   }
-  if (kinds < 0 || kinds > PB_VERIFY_ANY) return PB_E_INVALID;
+  if (!kinds_ok(kinds)) return PB_E_INVALID;
   const int k = kinds ? kinds : PB_VERIFY_ANY;
   const VerifyPlan plan = verify_plan(n_rows, n_seqs, vocab, dtype, k);
   if (!aligned(workspace, 256) || ws_bytes < plan.bytes) return PB_E_INVALID;

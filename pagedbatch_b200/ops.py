@@ -111,6 +111,12 @@ def mark_rows(params: torch.Tensor, rec: np.ndarray) -> torch.Tensor:
     return params
 
 
+def unchanged(params: torch.Tensor) -> bool:
+    """Whether a params tensor's records are surely those it was uploaded with: not where something was written to
+    it since, nor for inference tensors, which do not count their writes."""
+    return not params.is_inference() and params._version == getattr(params, "_pb_version", None)
+
+
 def noted_kinds(params: torch.Tensor) -> tuple[int, int]:
     """``row_kinds`` of the records a params tensor was uploaded from, (0, 0) where they are not known. Found
     when a verification first asks: the sampler, which uploads records every step, has no use for them."""
@@ -124,11 +130,12 @@ def noted_kinds(params: torch.Tensor) -> tuple[int, int]:
 def params_tensor(rec: np.ndarray, device, pinned: bool = True) -> torch.Tensor:
     """Upload packed records: one pinned host buffer, one non-blocking H2D copy."""
     rec = rec.copy()
-    host = torch.from_numpy(rec.view(np.uint8))
-    if pinned:
-        host = host.pin_memory()
-    params = mark_rows(host.to(device, non_blocking=True), rec)
-    params._pb_records = rec
+    with torch.inference_mode(False):  # (a tensor that counts its writes)
+        host = torch.from_numpy(rec.view(np.uint8))
+        if pinned:
+            host = host.pin_memory()
+        params = mark_rows(host.to(device, non_blocking=True), rec)
+    params._pb_records, params._pb_version = rec, params._version
     return params
 
 

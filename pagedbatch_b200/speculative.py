@@ -26,9 +26,16 @@ from .sampling import _INVALID_DISTRIBUTION, pack_rows
 __all__ = ["verify", "verify_tokens"]
 
 
-def _kinds(noted: tuple[int, int], vocab: int) -> int:
-    bits, kmax = noted
-    return bits if kmax < vocab else 0  # a top_k of the vocabulary or more is no filter: any kind
+def _kinds(params: torch.Tensor, noted: tuple[int, int] | None, vocab: int) -> int:
+    """The kinds of sequences to launch for: those of the records (`noted`, or as the params tensor was uploaded,
+    and then any other as well where it was written to since or may be before a replay of this call)."""
+    known = noted is not None
+    bits, kmax = noted if known else ops.noted_kinds(params)
+    if not bits or kmax >= vocab:
+        return 0  # (a top_k of the vocabulary or more is no filter: any kind)
+    if known or (ops.unchanged(params) and not torch.cuda.is_current_stream_capturing()):
+        return bits
+    return bits | _lib.VERIFY_REST
 
 
 def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=None):
@@ -68,7 +75,7 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=No
     with ops.on_device(dev):
         # a buffer of this call's own: the allocator hands it on in stream order, and a captured
         # graph keeps its copy
-        kinds = _kinds(ops.noted_kinds(params) if noted is None else noted, V)
+        kinds = _kinds(params, noted, V)
         n_ws = L.pb_verify_ws_bytes(R, S, V, code, kinds)
         ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
         rc = L.pb_verify(
@@ -103,7 +110,10 @@ def verify(logits: torch.Tensor, params: torch.Tensor, drafts: torch.Tensor, row
 
     * ``logits [R, V]``: CUDA, float32 / bfloat16 / float16, last dim contiguous;
     * ``params``: one packed ``pb_row_params`` record per sequence (``ops.params_tensor``), which may be
-      kept from step to step (their ``uniform`` is not used);
+      kept from step to step and written to in place, before the replay of a captured call as well (their
+      ``uniform`` is not used). The launches are those for the kinds of sequences it was uploaded with;
+      sequences of other kinds take the sampler's general kernel and are slower. Writes that torch does not
+      count (through ``.data``, or a kernel of one's own) need a clone, which has no note of kinds;
     * ``drafts int64[R]``: the draft each row judges (ignored at a sequence's last row);
     * ``row_offsets int32[S + 1]``: sequence ``s`` owns rows ``row_offsets[s]`` to ``row_offsets[s + 1] - 1``;
       it starts at 0, ends at R and gives every sequence at least one row (not checked on the host);

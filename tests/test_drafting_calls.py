@@ -1,9 +1,16 @@
 """What the calls of drafted decoding do on the host (CPU only)."""
 
 import numpy as np
+import pytest
 import torch
 
-from pagedbatch_b200 import _lib, ops
+from pagedbatch_b200 import _lib, build, ops
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return _lib.load()
 
 
 def _records():
@@ -25,3 +32,22 @@ def test_the_sampler_does_not_look_for_kinds_of_sequences(monkeypatch):
         assert ops.noted_kinds(params) == (_lib.VERIFY_SMALL | _lib.VERIFY_WHOLE, 50)
     assert len(asked) == 1
     assert ops.noted_kinds(params.clone()) == (0, 0)
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_records_written_to_are_known_as_such(inference):
+    with torch.inference_mode(inference):
+        params = ops.params_tensor(_records(), "cpu", pinned=False)
+        assert ops.unchanged(params)
+        assert not ops.unchanged(params.clone())
+        params[32:64].zero_()
+        assert not ops.unchanged(params)
+    assert not ops.unchanged(params)
+
+
+def test_kinds_beside_others(lib):
+    """PB_VERIFY_REST goes with some kind, and needs no more memory than the kinds do."""
+    for kinds in range(1, 16):
+        assert lib.pb_verify_ws_bytes(7, 3, 1000, 1, kinds | _lib.VERIFY_REST) == lib.pb_verify_ws_bytes(7, 3, 1000, 1, kinds)
+    for kinds in (_lib.VERIFY_REST, 32, 32 | 1, -16):
+        assert lib.pb_verify_ws_bytes(7, 3, 1000, 1, kinds) == -1
