@@ -38,13 +38,25 @@ def _kinds(params: torch.Tensor, noted: tuple[int, int] | None, vocab: int) -> i
     return bits | _lib.VERIFY_REST
 
 
+def _check_dtype(name: str, t: torch.Tensor) -> None:
+    if t.dtype not in ops._DTYPE_CODE:
+        raise ValueError(f"unsupported {name} dtype {t.dtype}")
+
+
+def _check_probs(draft_probs: torch.Tensor | None, n: int, vocab: int) -> None:
+    if draft_probs is None:
+        return
+    if draft_probs.dim() != 2 or draft_probs.shape != (n, vocab) or (draft_probs.stride(1) != 1 and vocab > 1):
+        raise ValueError(f"draft_probs must be [{n}, {vocab}] with a contiguous last dimension: a row per draft")
+    _check_dtype("draft_probs", draft_probs)
+
+
 def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=None):
     if not logits.is_cuda:
         raise ValueError("pagedbatch_b200.verify needs CUDA logits; move the tensor with .cuda() first")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("logits must be a [rows, vocab] tensor with a contiguous last dimension")
-    if logits.dtype not in ops._DTYPE_CODE:
-        raise ValueError(f"unsupported logits dtype {logits.dtype}")
+    _check_dtype("logits", logits)
     if params.dtype != torch.uint8 or params.numel() % _lib.ROW_PARAMS.itemsize or not params.is_contiguous():
         raise ValueError("params must be packed pb_row_params records (uint8), one per sequence")
     dev = logits.device
@@ -58,11 +70,7 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=No
         raise ValueError(f"params and draft_probs must be on the logits' device {dev}")
     if S > R:
         raise ValueError(f"{S} sequences for {R} rows: every sequence has at least one row")
-    if draft_probs is not None:
-        if draft_probs.dim() != 2 or draft_probs.shape != (R - S, V) or (draft_probs.stride(1) != 1 and V > 1):
-            raise ValueError(f"draft_probs must be [{R - S}, {V}] with a contiguous last dimension: a row per draft")
-        if draft_probs.dtype not in ops._DTYPE_CODE:
-            raise ValueError(f"unsupported draft_probs dtype {draft_probs.dtype}")
+    _check_probs(draft_probs, R - S, V)
     tokens = torch.empty(R, dtype=torch.int64, device=dev)
     accepted = torch.empty(S, dtype=torch.int32, device=dev)
     status = torch.empty(S, dtype=torch.int32, device=dev)
@@ -136,8 +144,9 @@ def verify_tokens(logits: torch.Tensor, drafts: Sequence[Sequence[int]], params:
 
     ``drafts[s]`` are sequence ``s``'s drafted token ids, ``params[s]`` its ``SamplingParams``;
     ``logits [R, V]`` holds ``len(drafts[s]) + 1`` rows for each sequence, one after another. A sequence that is
-    not greedy takes ``len(drafts[s]) + 1`` float64 draws from its generator. CPU logits are copied to
-    the current CUDA device first, as in ``sample_tokens``."""
+    not greedy takes ``len(drafts[s]) + 1`` float64 draws from its generator; a call that is refused takes none.
+    CPU logits are copied to the current CUDA device first, as in ``sample_tokens``, and CPU ``draft_probs`` with
+    them."""
     S = len(drafts)
     if len(params) != S or len(generators) != S:
         raise ValueError(f"{len(params)} params and {len(generators)} generators for {S} sequences")
@@ -158,15 +167,24 @@ def verify_tokens(logits: torch.Tensor, drafts: Sequence[Sequence[int]], params:
     rec = pack_rows(params, np.zeros(S))
     if S == 0:
         return []
+    _check_dtype("logits", logits)
+    _check_probs(draft_probs, R - S, V)
+    if logits.is_cuda:
+        dev = logits.device
+    elif torch.cuda.is_available():
+        dev = torch.device("cuda", torch.cuda.current_device())
+    else:
+        raise RuntimeError("pagedbatch_b200 verifies on a CUDA device and none is available")
+    if draft_probs is not None and draft_probs.device != dev:
+        if logits.is_cuda or draft_probs.is_cuda:
+            raise ValueError(f"draft_probs must be on the logits' device {dev}")
+        draft_probs = draft_probs.to(dev, non_blocking=draft_probs.is_pinned())
+    logits = logits.to(dev, non_blocking=not logits.is_cuda and logits.is_pinned())
     uniforms = np.zeros(R)
     for s, (p, g) in enumerate(zip(params, generators, strict=True)):
         if p.temperature != 0:
             n = int(lens[s]) + 1
             uniforms[offsets[s] : offsets[s] + n] = torch.rand(n, dtype=torch.float64, generator=g).numpy()
-    if not logits.is_cuda:
-        if not torch.cuda.is_available():
-            raise RuntimeError("pagedbatch_b200 verifies on a CUDA device and none is available")
-        logits = logits.to(torch.cuda.current_device(), non_blocking=logits.is_pinned())
     if logits.stride(1) != 1:
         logits = logits.contiguous()
     # parameters, random numbers, drafts and offsets in one pinned buffer and one copy
@@ -174,10 +192,10 @@ def verify_tokens(logits: torch.Tensor, drafts: Sequence[Sequence[int]], params:
     ends = np.cumsum([p.size for p in parts])
     host = torch.empty(int(ends[-1]), dtype=torch.uint8, pin_memory=True)
     np.concatenate(parts, out=host.numpy())
-    dev = host.to(logits.device, non_blocking=True)
+    buf = host.to(dev, non_blocking=True)
     tokens, accepted, status = _launch(
-        logits, dev[: ends[0]], dev[ends[1] : ends[2]].view(torch.int64), dev[ends[2] : ends[3]].view(torch.int32),
-        dev[ends[0] : ends[1]].view(torch.float64), draft_probs, ops.row_kinds(rec))
+        logits, buf[: ends[0]], buf[ends[1] : ends[2]].view(torch.int64), buf[ends[2] : ends[3]].view(torch.int32),
+        buf[ends[0] : ends[1]].view(torch.float64), draft_probs, ops.row_kinds(rec))
     got, n_ok, st = tokens.tolist(), accepted.tolist(), status.tolist()
     for s, code in enumerate(st):
         if code == _lib.ROW_NONFINITE:

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from pagedbatch_b200 import _lib, build, ops
+import pagedbatch_b200 as pb
+from pagedbatch_b200 import SamplingParams, _lib, build, ops
 
 
 @pytest.fixture(scope="module")
@@ -51,3 +52,18 @@ def test_kinds_beside_others(lib):
         assert lib.pb_verify_ws_bytes(7, 3, 1000, 1, kinds | _lib.VERIFY_REST) == lib.pb_verify_ws_bytes(7, 3, 1000, 1, kinds)
     for kinds in (_lib.VERIFY_REST, 32, 32 | 1, -16):
         assert lib.pb_verify_ws_bytes(7, 3, 1000, 1, kinds) == -1
+
+
+def test_refused_calls_leave_the_generators(monkeypatch):
+    """verify_tokens draws random numbers when every check is behind it, the device's among them."""
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    g = [torch.Generator().manual_seed(s) for s in range(2)]
+    before = [x.get_state() for x in g]
+    params, drafts, z = [SamplingParams()] * 2, [[1], [2, 3]], torch.zeros(5, 8)
+    ok = torch.zeros(3, 8)
+    for logits, probs, error in ((z, ok[:2], ValueError), (z, ok[:, :7], ValueError), (z, ok.double(), ValueError),
+                                 (z, torch.zeros(8, 3).T, ValueError), (z, ok[0], ValueError), (z.double(), None, ValueError),
+                                 (z, ok, RuntimeError), (z, None, RuntimeError)):
+        with pytest.raises(error):
+            pb.verify_tokens(logits, drafts, params, g, draft_probs=probs)
+        assert all(torch.equal(a, b.get_state()) for a, b in zip(before, g, strict=True))

@@ -89,3 +89,26 @@ def test_overwritten_where_equal_values_are_cut(cuda, noted):
         g.replay()
         torch.cuda.synchronize()
         _same(out, oracle.verify.verify(x, params, [n] * S, d, u))
+
+
+def test_draft_distributions_on_the_host(cuda):
+    """verify_tokens copies CPU draft_probs with CPU logits; those that are not with the logits are refused, and the
+    generators keep their state."""
+    lens = [2, 0, 3]
+    x = workloads.head_boosted(sum(lens) + 3, 4099, seed=1)
+    params = [KINDS["topk"](1), KINDS["whole"](1), KINDS["topp"](1)]
+    probs = _probs(x, lens, params, 2)
+    at = np.concatenate([[0], np.cumsum(np.array(lens) + 1)])
+    drafts = [x[at[s] : at[s] + n].argmax(1).tolist() for s, n in enumerate(lens)]
+    sp = [pb.SamplingParams(temperature=t, top_p=p, top_k=k) for t, p, k in params]
+
+    def call(z, p, gens=None):
+        return pb.verify_tokens(z, drafts, sp, gens or [torch.Generator().manual_seed(s) for s in range(3)], draft_probs=p)
+
+    want = call(x.cuda(), probs.cuda())
+    assert want == call(x, probs) == call(x.pin_memory(), probs.pin_memory()) == call(x, probs.cuda())
+    gens = [torch.Generator().manual_seed(s) for s in range(3)]
+    for bad in (probs, probs.cuda()[:, :-1], probs.cuda()[1:], probs.cuda().double()):
+        with pytest.raises(ValueError):
+            call(x.cuda(), bad, gens)
+    assert call(x.cuda(), probs.cuda(), gens) == want
