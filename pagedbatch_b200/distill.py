@@ -19,6 +19,42 @@ __all__ = ["distill_loss"]
 STATS = 32  # bytes of a row's statistics (pb_distill_stats_bytes)
 
 
+def _prepare(z, lp, idx, row_weight, temperature):
+    """Refuses what the kernels do not take; the teacher's entries, the weights and the temperature as they take them."""
+    if not z.is_cuda:
+        raise ValueError("pagedbatch_b200.distill_loss needs CUDA logits; move the tensor with .cuda() first")
+    if z.dim() != 2 or (z.stride(1) != 1 and z.shape[1] > 1):
+        raise ValueError("student_logits must be a [rows, vocab] tensor with a contiguous last dimension")
+    if z.dtype not in ops._DTYPE_CODE:
+        raise ValueError(f"unsupported student_logits dtype {z.dtype}")
+    n, V = z.shape
+    if not 1 <= V <= _lib.DISTILL_MAX_VOCAB:
+        raise ValueError(f"the vocabulary must hold 1 to {_lib.DISTILL_MAX_VOCAB} tokens, got {V}")
+    if lp.dim() != 2 or lp.shape[0] != n or not 1 <= lp.shape[1] <= _lib.DISTILL_MAX_ENTRIES:
+        raise ValueError(f"teacher_logprobs must be [{n}, K] with K in [1, {_lib.DISTILL_MAX_ENTRIES}]")
+    if lp.dtype not in ops._DTYPE_CODE:
+        raise ValueError(f"unsupported teacher_logprobs dtype {lp.dtype}")
+    if idx.shape != lp.shape or idx.dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_indices must be int32 or int64, of teacher_logprobs' shape")
+    if lp.requires_grad or (row_weight is not None and row_weight.requires_grad):
+        raise ValueError("the teacher's entries and the row weights take no gradient: detach them")
+    if row_weight is not None and (row_weight.dtype != torch.float32 or row_weight.shape != (n,)):
+        raise ValueError(f"row_weight must be a float32 tensor of {n} values")
+    dev = z.device
+    if lp.device != dev or idx.device != dev or (row_weight is not None and row_weight.device != dev):
+        raise ValueError(f"the teacher's entries and the row weights must be on the logits' device {dev}")
+    t = check_temperature(temperature)
+    if lp.dtype != torch.float32:
+        lp = lp.float()
+    if lp.stride(1) != 1:
+        lp = lp.contiguous()
+    if idx.stride(1) != 1:
+        idx = idx.contiguous()
+    if row_weight is not None:
+        row_weight = row_weight.contiguous()
+    return lp, idx, row_weight, t
+
+
 def _arguments(z, lp, idx, temperature):
     """What the forward and the backward call have in common."""
     n, V = z.shape
@@ -56,6 +92,61 @@ def _backward(z, lp, idx, weight, stats, temperature, grad_loss):
     return dz
 
 
+@torch.library.custom_op("pagedbatch_b200::distill_loss", mutates_args=())
+def distill_op(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_indices: torch.Tensor,
+               row_weight: torch.Tensor | None, temperature: float, tail: bool, total: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows' losses (or their sum) and their statistics."""
+    prepared = _prepare(student_logits, teacher_logprobs, teacher_indices, row_weight, temperature)
+    loss, buf = _forward(student_logits, *prepared, tail, total)
+    return loss, buf[: student_logits.shape[0] * STATS].clone()
+
+
+@distill_op.register_fake
+def _(student_logits, teacher_logprobs, teacher_indices, row_weight, temperature, tail, total):
+    _prepare(student_logits, teacher_logprobs, teacher_indices, row_weight, temperature)
+    n = student_logits.shape[0]
+    return (student_logits.new_empty(() if total else (n,), dtype=torch.float32),
+            student_logits.new_empty((n * STATS,), dtype=torch.uint8))
+
+
+def _check_backward(z, stats, grad_loss):
+    n = z.shape[0]
+    if stats.dtype != torch.uint8 or stats.shape != (n * STATS,) or not stats.is_contiguous() or stats.device != z.device:
+        raise ValueError("stats must be those of the forward call on the same rows")
+    if grad_loss.dtype != torch.float32 or grad_loss.shape not in ((), (n,)) or grad_loss.device != z.device:
+        raise ValueError(f"grad_loss must be one float32 value or {n} of them")
+
+
+@torch.library.custom_op("pagedbatch_b200::distill_loss_backward", mutates_args=())
+def distill_backward_op(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_indices: torch.Tensor,
+                        row_weight: torch.Tensor | None, stats: torch.Tensor, temperature: float,
+                        grad_loss: torch.Tensor) -> torch.Tensor:
+    """The gradient in the student's logits."""
+    lp, idx, weight, t = _prepare(student_logits, teacher_logprobs, teacher_indices, row_weight, temperature)
+    _check_backward(student_logits, stats, grad_loss)
+    return _backward(student_logits, lp, idx, weight, stats, t, grad_loss)
+
+
+@distill_backward_op.register_fake
+def _(student_logits, teacher_logprobs, teacher_indices, row_weight, stats, temperature, grad_loss):
+    _prepare(student_logits, teacher_logprobs, teacher_indices, row_weight, temperature)
+    _check_backward(student_logits, stats, grad_loss)
+    return student_logits.new_empty(student_logits.shape)
+
+
+def _save(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:4], output[1])
+    ctx.temperature = inputs[4]
+
+
+def _backward_traced(ctx, grad_loss, _):
+    dz = distill_backward_op(*ctx.saved_tensors, ctx.temperature, grad_loss)
+    return dz, None, None, None, None, None, None
+
+
+distill_op.register_autograd(_backward_traced, setup_context=_save)
+
+
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, lp, idx, weight, temperature, tail, total):
@@ -88,41 +179,13 @@ def distill_loss(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, t
       are all padding, have loss and gradient 0 whatever their logits hold.
 
     An index outside [-1, V) makes its row's loss NaN."""
-    z, lp, idx = student_logits, teacher_logprobs, teacher_indices
-    if not z.is_cuda:
-        raise ValueError("pagedbatch_b200.distill_loss needs CUDA logits; move the tensor with .cuda() first")
-    if z.dim() != 2 or (z.stride(1) != 1 and z.shape[1] > 1):
-        raise ValueError("student_logits must be a [rows, vocab] tensor with a contiguous last dimension")
-    if z.dtype not in ops._DTYPE_CODE:
-        raise ValueError(f"unsupported student_logits dtype {z.dtype}")
-    n, V = z.shape
-    if not 1 <= V <= _lib.DISTILL_MAX_VOCAB:
-        raise ValueError(f"the vocabulary must hold 1 to {_lib.DISTILL_MAX_VOCAB} tokens, got {V}")
-    if lp.dim() != 2 or lp.shape[0] != n or not 1 <= lp.shape[1] <= _lib.DISTILL_MAX_ENTRIES:
-        raise ValueError(f"teacher_logprobs must be [{n}, K] with K in [1, {_lib.DISTILL_MAX_ENTRIES}]")
-    if lp.dtype not in ops._DTYPE_CODE:
-        raise ValueError(f"unsupported teacher_logprobs dtype {lp.dtype}")
-    if idx.shape != lp.shape or idx.dtype not in (torch.int32, torch.int64):
-        raise ValueError("teacher_indices must be int32 or int64, of teacher_logprobs' shape")
-    if lp.requires_grad or (row_weight is not None and row_weight.requires_grad):
-        raise ValueError("the teacher's entries and the row weights take no gradient: detach them")
-    if row_weight is not None and (row_weight.dtype != torch.float32 or row_weight.shape != (n,)):
-        raise ValueError(f"row_weight must be a float32 tensor of {n} values")
-    dev = z.device
-    if lp.device != dev or idx.device != dev or (row_weight is not None and row_weight.device != dev):
-        raise ValueError(f"the teacher's entries and the row weights must be on the logits' device {dev}")
     if reduction not in ("none", "sum"):
         raise ValueError(f"reduction must be 'none' or 'sum', got {reduction!r}")
-    t = check_temperature(temperature)
-    if lp.dtype != torch.float32:
-        lp = lp.float()
-    if lp.stride(1) != 1:
-        lp = lp.contiguous()
-    if idx.stride(1) != 1:
-        idx = idx.contiguous()
-    if row_weight is not None:
-        row_weight = row_weight.contiguous()
+    z = student_logits
+    lp, idx, row_weight, t = _prepare(z, teacher_logprobs, teacher_indices, row_weight, temperature)
     total = reduction == "sum"
+    if ops.traced(z):
+        return distill_op(z, lp, idx, row_weight, t, bool(tail), total)[0]
     if not (z.requires_grad and torch.is_grad_enabled()):
         return _forward(z, lp, idx, row_weight, t, bool(tail), total)[0]
     return _Distill.apply(z, lp, idx, row_weight, t, bool(tail), total)

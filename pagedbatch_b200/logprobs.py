@@ -31,7 +31,7 @@ def check_temperature(temperature: float) -> float:
     return t
 
 
-def _launch(logits: torch.Tensor, k: int, temperature: float):
+def _check(logits: torch.Tensor, k: int, temperature: float) -> float:
     if not logits.is_cuda:
         raise ValueError("pagedbatch_b200.top_logprobs needs CUDA logits; move the tensor with .cuda() first")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
@@ -41,7 +41,12 @@ def _launch(logits: torch.Tensor, k: int, temperature: float):
     n, V = logits.shape
     if not 1 <= k <= min(_lib.TOP_MAX, V):
         raise ValueError(f"k must be in [1, {min(_lib.TOP_MAX, V)}], got {k}")
-    t = check_temperature(temperature)
+    return check_temperature(temperature)
+
+
+def _launch(logits: torch.Tensor, k: int, temperature: float):
+    t = _check(logits, k, temperature)
+    n, V = logits.shape
     dev = logits.device
     lp = torch.empty((n, k), dtype=torch.float32, device=dev)
     idx = torch.empty((n, k), dtype=torch.int32, device=dev)
@@ -65,6 +70,7 @@ def top_logprobs_op(logits: torch.Tensor, k: int, temperature: float) -> tuple[t
 
 @top_logprobs_op.register_fake
 def _(logits, k, temperature):
+    _check(logits, k, temperature)
     n = logits.shape[0]
     return (logits.new_empty((n, k), dtype=torch.float32), logits.new_empty((n, k), dtype=torch.int32),
             logits.new_empty((n,), dtype=torch.float32))
@@ -74,4 +80,5 @@ def top_logprobs(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopL
     """The ``k`` (at most 256) largest log-probabilities of ``softmax(logits / temperature)`` of every
     row of ``logits [n, V]`` (CUDA, float32 / bfloat16 / float16), on the current stream.
     Rows with NaN or +inf logits, or only -inf, have NaN log-probabilities. No gradient flows back."""
-    return TopLogprobs(*_launch(logits.detach(), int(k), temperature))
+    launch = top_logprobs_op if ops.traced(logits) else _launch
+    return TopLogprobs(*launch(logits.detach(), int(k), float(temperature)))

@@ -51,7 +51,8 @@ def _check_probs(draft_probs: torch.Tensor | None, n: int, vocab: int) -> None:
     _check_dtype("draft_probs", draft_probs)
 
 
-def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=None):
+def _check(logits, params, drafts, row_offsets, uniforms, draft_probs) -> int:
+    """Refuses what the kernels do not take; the number of sequences."""
     if not logits.is_cuda:
         raise ValueError("pagedbatch_b200.verify needs CUDA logits; move the tensor with .cuda() first")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
@@ -71,12 +72,19 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=No
     if S > R:
         raise ValueError(f"{S} sequences for {R} rows: every sequence has at least one row")
     _check_probs(draft_probs, R - S, V)
+    if S == 0 and R:
+        raise ValueError(f"{R} rows for no sequence")
+    return S
+
+
+def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=None):
+    S = _check(logits, params, drafts, row_offsets, uniforms, draft_probs)
+    R, V = logits.shape
+    dev = logits.device
     tokens = torch.empty(R, dtype=torch.int64, device=dev)
     accepted = torch.empty(S, dtype=torch.int32, device=dev)
     status = torch.empty(S, dtype=torch.int32, device=dev)
     if S == 0:
-        if R:
-            raise ValueError(f"{R} rows for no sequence")
         return tokens, accepted, status
     L = _lib.load()
     code = ops._DTYPE_CODE[logits.dtype]
@@ -105,10 +113,25 @@ def verify_op(logits: torch.Tensor, params: torch.Tensor, drafts: torch.Tensor, 
     return tokens, accepted
 
 
+@torch.library.custom_op("pagedbatch_b200::verify_with_status", mutates_args=())
+def verify_with_status_op(
+        logits: torch.Tensor, params: torch.Tensor, drafts: torch.Tensor, row_offsets: torch.Tensor, uniforms: torch.Tensor,
+        draft_probs: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Tokens, accepted counts and status codes."""
+    return _launch(logits, params, drafts, row_offsets, uniforms, draft_probs)
+
+
 @verify_op.register_fake
 def _(logits, params, drafts, row_offsets, uniforms, draft_probs=None):
-    s = params.numel() // _lib.ROW_PARAMS.itemsize
+    s = _check(logits, params, drafts, row_offsets, uniforms, draft_probs)
     return logits.new_empty((logits.shape[0],), dtype=torch.int64), logits.new_empty((s,), dtype=torch.int32)
+
+
+@verify_with_status_op.register_fake
+def _(logits, params, drafts, row_offsets, uniforms, draft_probs=None):
+    s = _check(logits, params, drafts, row_offsets, uniforms, draft_probs)
+    return (logits.new_empty((logits.shape[0],), dtype=torch.int64), logits.new_empty((s,), dtype=torch.int32),
+            logits.new_empty((s,), dtype=torch.int32))
 
 
 def verify(logits: torch.Tensor, params: torch.Tensor, drafts: torch.Tensor, row_offsets: torch.Tensor,
@@ -134,6 +157,9 @@ def verify(logits: torch.Tensor, params: torch.Tensor, drafts: torch.Tensor, row
     ``tokens`` holds, from each sequence's first row on, its accepted drafts and the token drawn after
     them, then -1. ``with_status`` adds ``int32[S]`` status codes (``PB_ROW_*``; where it is not 0 the
     drawn token is -1). Runs on the current stream of the logits' device and can be captured."""
+    if ops.traced(logits):
+        op = verify_with_status_op if with_status else verify_op
+        return tuple(op(logits, params, drafts, row_offsets, uniforms, draft_probs))
     out = _launch(logits, params, drafts, row_offsets, uniforms, draft_probs)
     return out if with_status else out[:2]
 

@@ -3,6 +3,7 @@
 import numpy as np
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 import pagedbatch_b200 as pb
 from pagedbatch_b200 import SamplingParams, _lib, build, ops
@@ -67,3 +68,50 @@ def test_refused_calls_leave_the_generators(monkeypatch):
         with pytest.raises(error):
             pb.verify_tokens(logits, drafts, params, g, draft_probs=probs)
         assert all(torch.equal(a, b.get_state()) for a, b in zip(before, g, strict=True))
+
+
+def test_fake_tensors():
+    """Shapes and types of the results without data, and the same refusals."""
+    with FakeTensorMode():
+        z = torch.empty(5, 100, device="cuda", dtype=torch.bfloat16)
+        lp, idx, lse = pb.top_logprobs(z, 7, temperature=0.5)
+        assert lp.shape == idx.shape == (5, 7) and lse.shape == (5,)
+        assert (lp.dtype, idx.dtype, lse.dtype) == (torch.float32, torch.int32, torch.float32) and lp.is_cuda
+        with pytest.raises(ValueError, match="k must be"):
+            pb.top_logprobs(z, 101)
+        params = torch.empty(64, dtype=torch.uint8, device="cuda")
+        d, u = torch.empty(5, dtype=torch.int64, device="cuda"), torch.empty(5, dtype=torch.float64, device="cuda")
+        off = torch.empty(3, dtype=torch.int32, device="cuda")
+        for probs in (None, torch.empty(3, 100, device="cuda")):
+            tok, acc, st = pb.verify(z, params, d, off, u, draft_probs=probs, with_status=True)
+            assert tok.shape == (5,) and acc.shape == st.shape == (2,)
+            assert (tok.dtype, acc.dtype, st.dtype) == (torch.int64, torch.int32, torch.int32)
+            assert len(pb.verify(z, params, d, off, u, draft_probs=probs)) == 2
+        with pytest.raises(ValueError, match="draft_probs"):
+            pb.verify(z, params, d, off, u, draft_probs=torch.empty(2, 100, device="cuda"))
+        z.requires_grad_()
+        for reduction, shape in (("none", (5,)), ("sum", ())):
+            loss = pb.distill_loss(z, lp, idx, reduction=reduction, row_weight=torch.empty(5, device="cuda"))
+            assert loss.shape == shape and loss.dtype == torch.float32
+            assert loss.requires_grad
+
+
+def test_ops_refuse_what_the_calls_refuse():
+    """The registered ops check their arguments themselves."""
+    op, back = torch.ops.pagedbatch_b200.distill_loss, torch.ops.pagedbatch_b200.distill_loss_backward
+    with FakeTensorMode():
+        z, lp, w = (torch.empty(s, device="cuda") for s in ((3, 50), (3, 4), (3,)))
+        idx = torch.empty(3, 4, dtype=torch.int32, device="cuda")
+        stats, g = torch.empty(96, dtype=torch.uint8, device="cuda"), torch.empty(3, device="cuda")
+        ok = dict(z=z, lp=lp, idx=idx, w=w, t=1.0)
+        for bad in (dict(lp=lp[:2]), dict(idx=idx[:, :2]), dict(idx=idx.short()), dict(w=w[:1]), dict(t=0.0), dict(z=z.double()),
+                    dict(z=torch.empty(50, 3, device="cuda").T), dict(lp=torch.empty(3, 4))):
+            a = list((ok | bad).values())
+            with pytest.raises(ValueError):
+                op(*a, False, False)
+            with pytest.raises(ValueError):
+                back(*a[:4], stats, a[4], g)
+        for st, gr in ((stats[:64], g), (stats.float(), g), (stats, g[:1]), (stats, g.double()), (stats, g[None])):
+            with pytest.raises(ValueError):
+                back(z, lp, idx, w, st, 1.0, gr)
+        assert back(z, lp, idx, None, stats, 1.0, g[0]).shape == z.shape
