@@ -1,9 +1,10 @@
-"""The operators of drafted decoding in recorded calls (make_fx, torch.compile) and on fake tensors: a
-recorded call computes what the call does, on other inputs as well."""
+"""The operators of drafted decoding in recorded calls (make_fx, torch.compile), on fake tensors and under forward
+mode: a recorded call computes what the call does, on other inputs as well, and what has no derivative says so."""
 
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
@@ -94,6 +95,18 @@ def test_fake_gradient(cuda):
         lp, idx, _ = pb.top_logprobs(z, 7)
         (grad,) = torch.autograd.grad(pb.distill_loss(z, lp, idx, reduction="sum"), z)
         assert grad.shape == z.shape and grad.dtype == z.dtype
+
+
+def test_forward_mode_is_refused(cuda):
+    """No tangent is lost without a word, in the logits or in the teacher's record."""
+    args = _distill_inputs(1)
+    with fwAD.dual_level():
+        for at in (0, 1, 3):
+            a = list(args)
+            a[at] = fwAD.make_dual(a[at], torch.ones_like(a[at]))
+            with pytest.raises(NotImplementedError):
+                _loss(*a)
+        assert fwAD.unpack_dual(_loss(*args)).tangent is None
 
 
 def test_the_op_differentiates_once(cuda):
