@@ -9,7 +9,7 @@ ids. Formulas and edge cases are stated at ``pb_distill_forward`` in ``include/p
 from __future__ import annotations
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
@@ -187,7 +187,8 @@ def distill_loss(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, t
     total = reduction == "sum"
     if ops.traced(z):
         return distill_op(z, lp, idx, row_weight, t, bool(tail), total)[0]
-    if any(a is not None and unpack_dual(a).tangent is not None for a in (z, lp, row_weight)):
+    if forward_ad._current_level >= 0 and any(  # (inside a level of dual tensors)
+            a is not None and forward_ad.unpack_dual(a).tangent is not None for a in (z, lp, row_weight)):
         raise NotImplementedError("distill_loss has no forward-mode derivative")
     if not (z.requires_grad and torch.is_grad_enabled()):
         return _forward(z, lp, idx, row_weight, t, bool(tail), total)[0]

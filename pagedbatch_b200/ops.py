@@ -71,11 +71,13 @@ class on_device:
             torch.cuda.set_device(self.prev)
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
 def traced(t: torch.Tensor) -> bool:
     """Whether a call on ``t`` is to be recorded, or ``t`` holds no data (torch.compile, make_fx, fake tensors, other
     dispatch modes and tensor classes). Such calls go through the registered ops; others past their dispatch."""
-    return (torch.compiler.is_compiling() or type(t) not in (torch.Tensor, torch.nn.Parameter)
-            or torch._C._len_torch_dispatch_stack() > 0)
+    return torch.compiler.is_compiling() or type(t) not in _PLAIN or torch._C._len_torch_dispatch_stack() > 0
 
 
 GROUP_KMAX = 128  # largest top_k the two-pass launch of pb_sample_ws settles

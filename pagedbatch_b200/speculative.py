@@ -33,7 +33,7 @@ def _kinds(params: torch.Tensor, noted: tuple[int, int] | None, vocab: int) -> i
     bits, kmax = noted if known else ops.noted_kinds(params)
     if not bits or kmax >= vocab:
         return 0  # (a top_k of the vocabulary or more is no filter: any kind)
-    if known or (ops.unchanged(params) and not torch.cuda.is_current_stream_capturing()):
+    if known or (ops.unchanged(params) and not torch._C._cuda_isCurrentStreamCapturing()):
         return bits
     return bits | _lib.VERIFY_REST
 
