@@ -56,7 +56,7 @@ struct RowMeta {
 constexpr int WEIGH_CTAS = 3 * 148;    // CTAs of weigh_kernel that are on the device at once
 constexpr int STEPS = 512;             // histogram steps of a row's key
 constexpr float STEP_SCALE = STEPS / 28.0f;  // keys further than 27.73 below the maximum have no weight
-constexpr int LIST = 2048;             // elements order_kernel takes from one step
+constexpr int LIST = 2048;             // elements order_kernel takes from one step (a row has its vocabulary's at most)
 
 // Sums of one tile of the row a sequence draws from, in units of 2^-40. Where top-p cut among the
 // equals of the last kept key, `w` leaves those equals out, `tie_w` is theirs and `ties` counts them.
@@ -88,7 +88,8 @@ struct VerifyArgs {
   pb_row_params* rowp;           // workspace: [n_rows], what pb_sample_ws sees
   pb_row_params* rowq;           // workspace: [n_rows], the rows' own
   uint64_t* hist;                // workspace: [n_rows][STEPS] (a batch with ROW_MASS rows)
-  uint64_t* list;                // ... [n_rows][LIST]
+  uint64_t* list;                // ... [n_rows][list_len]
+  int32_t list_len;              // LIST, or the vocabulary where it is smaller
   pb_row_info* info;             // workspace: [n_rows]
   int64_t* tok;                  // workspace: [n_rows], the sampler's tokens (greedy rows' maxima)
   RowMeta* meta;                 // workspace: [n_rows]
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(VT, 4) gather_kernel(VerifyArgs a) {
   const uint32_t n = found;
   if (threadIdx.x == 0 && n) base = atomicAdd(&a.meta[row].listed, n);
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n && base + i < (uint32_t)LIST; i += VT) a.list[row * LIST + base + i] = list[i];
+  for (uint32_t i = threadIdx.x; i < n && base + i < (uint32_t)a.list_len; i += VT) a.list[row * a.list_len + base + i] = list[i];
 }
 
 // The last kept element among them, in the order (key descending, index ascending): what the row's
@@ -583,7 +584,7 @@ __global__ void __launch_bounds__(VT) order_kernel(VerifyArgs a) {
   const int tid = threadIdx.x;
   const RowMeta meta = a.meta[row];
   pb_row_info* o = a.info + row;
-  if (meta.kind == ROW_OTHER || (meta.kind == ROW_MASS && o->status != PB_ROW_NONFINITE && (meta.listed == 0 || meta.listed > (uint32_t)LIST))) {
+  if (meta.kind == ROW_OTHER || (meta.kind == ROW_MASS && o->status != PB_ROW_NONFINITE && (meta.listed == 0 || meta.listed > (uint32_t)a.list_len))) {
     if (tid == 0) o->status = PB_ROW_FALLBACK;
     return;
   }
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__(VT) order_kernel(VerifyArgs a) {
   const int32_t n = (int32_t)meta.listed;
   uint32_t size = 2;
   while (size < (uint32_t)n) size <<= 1;
-  for (uint32_t i = tid; i < size; i += VT) list[i] = i < (uint32_t)n ? __ldcg(a.list + row * LIST + i) : 0ull;
+  for (uint32_t i = tid; i < size; i += VT) list[i] = i < (uint32_t)n ? __ldcg(a.list + row * a.list_len + i) : 0ull;
   if (tid == 0) kept = 0, kept_q = 0;
   __syncthreads();
   for (uint32_t k = 2; k <= size; k <<= 1)
@@ -1528,6 +1529,8 @@ __global__ void __launch_bounds__(VT, 2) draw_kernel(VerifyArgs a) {
 
 constexpr int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
+constexpr int64_t list_len(int64_t vocab) { return vocab < LIST ? vocab : LIST; }
+
 struct VerifyPlan {
   int64_t rowp, rowq, info, tok, meta, decision, tiles, sums, hist, list, sampler, bytes;  // offsets in the workspace, its size
 };
@@ -1549,7 +1552,7 @@ VerifyPlan verify_plan(int64_t n_rows, int64_t n_seqs, int64_t vocab, int dtype,
   v.tiles = take(n_seqs * seg.segs * TILES * (int64_t)sizeof(Tile));
   v.sums = take(kinds & PB_VERIFY_WHOLE ? n_rows * seg.segs * (int64_t)sizeof(ExpSum) : 0);
   v.hist = take(kinds & PB_VERIFY_TOPP ? n_rows * STEPS * 8 : 0);
-  v.list = take(kinds & PB_VERIFY_TOPP ? n_rows * LIST * 8 : 0);
+  v.list = take(kinds & PB_VERIFY_TOPP ? n_rows * list_len(vocab) * 8 : 0);
   v.sampler = at;
   v.bytes = at + (kinds & PB_VERIFY_SMALL ? pb_sample_ws_bytes(n_rows, vocab, dtype) : 0);
   return v;
@@ -1569,6 +1572,7 @@ int verify_run(VerifyArgs a, int dtype, int named, uint8_t* ws, const VerifyPlan
   if (kinds & PB_VERIFY_TOPP) {
     a.hist = reinterpret_cast<uint64_t*>(ws + plan.hist);
     a.list = reinterpret_cast<uint64_t*>(ws + plan.list);
+    a.list_len = (int32_t)list_len(a.V);
   }
   a.seg = seg_plan(a.V, sizeof(T), a.x, a.row_stride);
   a.kinds = kinds;

@@ -115,3 +115,10 @@ def test_ops_refuse_what_the_calls_refuse():
             with pytest.raises(ValueError):
                 back(z, lp, idx, w, st, 1.0, gr)
         assert back(z, lp, idx, None, stats, 1.0, g[0]).shape == z.shape
+
+
+def test_workspace_of_small_vocabularies(lib):
+    """What top-p sequences need of a row's step is no more than the row."""
+    for V in (1, 48, 1000, 5000):
+        more = lib.pb_verify_ws_bytes(4096, 64, V, 0, _lib.VERIFY_TOPP) - lib.pb_verify_ws_bytes(4096, 64, V, 0, _lib.VERIFY_OTHER)
+        assert more == 4096 * 8 * (512 + min(V, 2048))
