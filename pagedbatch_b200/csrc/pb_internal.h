@@ -20,6 +20,12 @@ struct GroupKeys {
 GroupKeys sample_ws_keys(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
                          const void* workspace, int64_t ws_bytes);
 
+// pb_sample_ws's launches for a batch whose group keys sample_ws_keys names, each waiting for the whole of the one
+// before. (pb_sample_ws lets them overlap, and where no row is greedy or small top-k none of them waits: the
+// last one may end before the keys are written.)
+int sample_ws_in_turn(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                      const pb_row_params* params, int64_t* out_token, pb_row_info* info, void* workspace, void* stream);
+
 // The cluster kernel over the rows whose status in `info` is PB_ROW_FALLBACK (vocab < 2^24, valid
 // arguments): their tokens and records are written, the other rows' are left as they are.
 int sample_fallback_rows(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,

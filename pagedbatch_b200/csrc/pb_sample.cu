@@ -2497,9 +2497,9 @@ int64_t group_grid(int64_t ntasks) {
   return std::max<int64_t>(1, std::min<int64_t>(full, (ntasks + GM_WARPS - 1) / GM_WARPS));
 }
 
-// pass 1 -> pass 2 (programmatic dependency) -> cluster kernel over the rows pass 2 left
+// pass 1 -> pass 2 (programmatic dependency unless `in_turn`) -> cluster kernel over the rows pass 2 left
 template <typename T>
-int run_groups(const Args& a, uint8_t* workspace, int es, cudaStream_t st) {
+int run_groups(const Args& a, uint8_t* workspace, int es, cudaStream_t st, bool in_turn) {
   const GroupPlan gp = group_plan(a.n_rows, a.vocab, es);
   GroupArgs g;
   g.logits = a.logits;
@@ -2520,7 +2520,7 @@ int run_groups(const Args& a, uint8_t* workspace, int es, cudaStream_t st) {
   g.vocab_offset = a.vocab_offset;
   group_max_kernel<T><<<(unsigned)group_grid<T>(gp.ntasks), GM_THREADS, 0, st>>>(g);
   if (cudaGetLastError() != cudaSuccess) return PB_E_LAUNCH;
-  const bool pdl = getenv("PB_NO_PDL") == nullptr;
+  const bool pdl = !in_turn && getenv("PB_NO_PDL") == nullptr;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.n_rows, 1, 1);
   cfg.blockDim = dim3(GS_THREADS, 1, 1);
@@ -2540,15 +2540,15 @@ int run_groups(const Args& a, uint8_t* workspace, int es, cudaStream_t st) {
   return launch<T>(c, cluster_size_for(a.n_rows, a.vocab, es), st, pdl);
 }
 
-int run_groups_args(const Args& a, int dtype, int es, uint8_t* workspace, cudaStream_t st) {
-  if (dtype == PB_DTYPE_F32) return run_groups<float>(a, workspace, es, st);
-  if (dtype == PB_DTYPE_BF16) return run_groups<__nv_bfloat16>(a, workspace, es, st);
-  return run_groups<__half>(a, workspace, es, st);
+int run_groups_args(const Args& a, int dtype, int es, uint8_t* workspace, cudaStream_t st, bool in_turn = false) {
+  if (dtype == PB_DTYPE_F32) return run_groups<float>(a, workspace, es, st, in_turn);
+  if (dtype == PB_DTYPE_BF16) return run_groups<__nv_bfloat16>(a, workspace, es, st, in_turn);
+  return run_groups<__half>(a, workspace, es, st, in_turn);
 }
 
 int run_groups_dtype(const void* logits, int dtype, int es, int64_t n_rows, int64_t vocab, int64_t row_stride,
                      const int32_t* row_index, const pb_row_params* params, int64_t* out_token,
-                     pb_row_info* out_info, uint8_t* workspace, cudaStream_t st) {
+                     pb_row_info* out_info, uint8_t* workspace, cudaStream_t st, bool in_turn = false) {
   Args a;
   a.logits = static_cast<const char*>(logits);
   a.n_rows = n_rows;
@@ -2564,7 +2564,7 @@ int run_groups_dtype(const void* logits, int dtype, int es, int64_t n_rows, int6
   a.cand_out = nullptr;
   a.cand_cap = 0;
   a.vocab_offset = 0;
-  return run_groups_args(a, dtype, es, workspace, st);
+  return run_groups_args(a, dtype, es, workspace, st, in_turn);
 }
 
 // ---- allocation-free entry point -------------------------------------------------------------
@@ -2665,6 +2665,12 @@ GroupKeys sample_ws_keys(const void* logits, int dtype, int64_t n_rows, int64_t 
   g.groups = (int32_t)p.ngr;
   g.elems = GM_GB / es;
   return g;
+}
+
+int sample_ws_in_turn(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                      const pb_row_params* params, int64_t* out_token, pb_row_info* info, void* workspace, void* stream) {
+  return run_groups_dtype(logits, dtype, dtype == PB_DTYPE_F32 ? 4 : 2, n_rows, vocab, row_stride, nullptr, params, out_token,
+                          info, static_cast<uint8_t*>(workspace), static_cast<cudaStream_t>(stream), true);
 }
 
 int sample_fallback_rows(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,

@@ -1590,9 +1590,13 @@ int verify_run(VerifyArgs a, int dtype, int named, uint8_t* ws, const VerifyPlan
     // the two-pass launch where the rows suit it, else pb_sample's own launches (the workspace's other
     // launch cuts rows into pieces for large batches: 72 rows of 50021 fp16 take it 31 us, these 27 us)
     a.groups = sample_ws_keys(a.x, dtype, a.n_rows, a.V, a.row_stride, ws + plan.sampler, plan.bytes - plan.sampler);
-    rc = a.groups.keys ? pb_sample_ws(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr,
-                                      ws + plan.sampler, plan.bytes - plan.sampler, st)
-                       : pb_sample(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr, st);
+    if (!a.groups.keys)
+      rc = pb_sample(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr, st);
+    else if (a.rest == ROW_SMALL)  // (rows of any kind, perhaps none that pb_sample_ws's launches wait for)
+      rc = sample_ws_in_turn(a.x, dtype, a.n_rows, a.V, a.row_stride, a.rowp, a.tok, a.info, ws + plan.sampler, st);
+    else
+      rc = pb_sample_ws(a.x, dtype, a.n_rows, a.V, a.row_stride, nullptr, a.rowp, a.tok, a.info, nullptr, ws + plan.sampler,
+                        plan.bytes - plan.sampler, st);
   }
   // (before the pass over whole rows, which the launches after it overlap with)
   if (rc == PB_OK && a.rest == ROW_OTHER && !general) rc = fallback();
