@@ -266,7 +266,7 @@ PB_API int pb_stop_check(const int64_t* tokens, int64_t n_rows, const int32_t* r
  * Verification of drafted tokens (speculative decoding): no counterpart in the reference, which
  * decodes one token a step. A sequence with d drafts owns d + 1 consecutive logits rows, the target's
  * distributions at each draft's position and after the last; rows of sequence s are
- * row_offsets[s] .. row_offsets[s + 1) - 1, row_offsets[0] = 0, at least one row a sequence.
+ * row_offsets[s] .. row_offsets[s + 1] - 1, row_offsets[0] = 0, at least one row a sequence.
  *
  *   logits       device [n_rows, vocab] as pb_sample's.
  *   params       device pb_row_params[n_seqs]: the sequence's sampling parameters (`uniform` and

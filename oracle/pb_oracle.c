@@ -72,13 +72,13 @@ static uint64_t weight_q(float key, float m) {
   return (uint64_t)(w * 0x1p40f);
 }
 
-/* floor(p * z) for an fp32 p in [0, 1) and z < 2^64, exact */
 /* Weights of n scaled keys against their largest m (the rule of pb_sample, used row by row by the
  * verification oracle). */
 void pbo_weights(const float* keys, int64_t n, float m, uint64_t* q) {
   for (int64_t i = 0; i < n; ++i) q[i] = weight_q(keys[i], m);
 }
 
+/* floor(p * z) for an fp32 p in [0, 1) and z < 2^64, exact */
 static uint64_t mul_floor(float p, uint64_t z) {
   uint32_t b = f2u(p);
   uint32_t e8 = (b >> 23) & 0xFF;

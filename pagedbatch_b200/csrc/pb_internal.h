@@ -8,11 +8,10 @@
 namespace pb {
 
 // Group keys that pb_sample_ws leaves in its workspace: for every row, the key of the largest value of
-// each `elems` consecutive elements (128 bytes), `groups` of them, rows `stride` keys apart (a multiple
-// of 4).
+// each 128 bytes (8 vectors of 16), `groups` of them, rows `stride` keys apart (a multiple of 4).
 struct GroupKeys {
   const uint32_t* keys;
-  int32_t stride, groups, elems;
+  int32_t stride, groups;
 };
 
 // The group keys of a pb_sample_ws call with these arguments, or keys = nullptr where it takes its

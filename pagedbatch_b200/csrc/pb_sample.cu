@@ -2656,14 +2656,13 @@ namespace pb {
 
 GroupKeys sample_ws_keys(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
                          const void* workspace, int64_t ws_bytes) {
-  GroupKeys g = {nullptr, 0, 0, 0};
+  GroupKeys g = {nullptr, 0, 0};
   const int es = (dtype == PB_DTYPE_F32) ? 4 : 2;
   const GroupPlan p = group_plan(n_rows, vocab, es);
   if (!groups_eligible(logits, row_stride, es, n_rows, vocab) || ws_bytes < p.bytes) return g;
   g.keys = static_cast<const uint32_t*>(workspace);
   g.stride = (int32_t)p.ngs;
   g.groups = (int32_t)p.ngr;
-  g.elems = GM_GB / es;
   return g;
 }
 

@@ -53,7 +53,7 @@ struct RowMeta {
   float top_p;
 };
 
-constexpr int WEIGH_CTAS = 3 * 148;    // CTAs of weigh_kernel that are on the device at once
+constexpr int WEIGH_CTAS = 3 * 148;    // CTAs of weigh_kernel that are on a B200 at once (3 on each SM)
 constexpr int STEPS = 512;             // histogram steps of a row's key
 constexpr float STEP_SCALE = STEPS / 28.0f;  // keys further than 27.73 below the maximum have no weight
 constexpr int LIST = 2048;             // elements order_kernel takes from one step (a row has its vocabulary's at most)
@@ -1363,12 +1363,11 @@ __global__ void __launch_bounds__(VT, 3) weigh_kernel(VerifyArgs a) {
 struct DrawShared {
   uint64_t scan[VNW + 1];
   uint32_t tscan[VNW + 1];
-  uint64_t total, left;
+  uint64_t left;     // the draw's number within its tile
   int32_t tile;      // the draw's tile
   uint32_t before;   // equals of the last kept key before it
   int32_t cut;       // the tile in which the kept equals end
   uint32_t cut_before;
-  int32_t found;
 };
 
 // The draw: one CTA per sequence. Tiles are in index order, so are a tile's vectors over the threads. Only
@@ -1415,15 +1414,10 @@ __global__ void __launch_bounds__(VT, 2) draw_kernel(VerifyArgs a) {
     for (int q = 0; q < EPV; ++q) s += r[q];
     return units(s);
   };
-  // sum of tile k with the equals before it known: from its record, or where the kept equals end
-  // inside it, from sh.total (computed once below)
-  if (tid == 0) {
-    sh.tile = sh.cut = -1;
-    sh.found = -1;
-    sh.total = 0;
-  }
+  if (tid == 0) sh.tile = sh.cut = -1;
   __syncthreads();
-  uint64_t cut_w = 0;  // weight of the tile in which the kept equals end
+  // a tile's weight comes from its record, but for the one in which the kept equals end: that is weighed again
+  uint64_t cut_w = 0;
   if (row.cut_ties) {
     uint32_t base = 0;
     for (int32_t k0 = 0; k0 < nt; k0 += VT) {
