@@ -16,7 +16,8 @@
 // loss from the row's entries. For the tail bucket the entries are kept out of the sums exactly (a bit
 // per element of the segment in shared memory), so S has no cancellation however sure the student is.
 // Backward: one launch, z in and dz out, on the statistics of the forward. Both passes are bound by
-// HBM: V * es bytes a row forward, twice that backward. [4096, 128256] bf16 with a tail, summed: 560 us,
+// HBM: V * es bytes a row forward, twice that backward. [4096, 128256] bf16 with a tail, summed: 557 us of launches
+// back to back (a captured step; one call by itself 606 us, as the host starts each half),
 // floor 326 us if the backward pass found the logits on chip, 488 us as they are read twice. (A persistent
 // kernel that takes both passes over a few rows at a time, the second from L2, took 570 us: its halves wait
 // for one another.)
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(SEG_T, SEG_CTAS) part_kernel(DistillArgs a) {
 }
 
 // One warp per row: joins the row's segments, takes the loss from its entries, and leaves what the
-// backward pass needs. Its loads of entries go ahead of the wait for the segments. 6.5 us for 4096 rows.
+// backward pass needs. Its loads of entries go ahead of the wait for the segments. 10 us for 4096 rows.
 template <typename T, bool TAIL>
 __global__ void __launch_bounds__(256) finish_kernel(DistillArgs a) {
   const int lane = threadIdx.x & 31;

@@ -21,7 +21,8 @@
 //      with top-p alone: max_kernel, then hist_kernel sums the weights in 512 steps of the key,
 //      cut_kernel finds the step in which the mass passes top-p, gather_kernel lists its elements and
 //      order_kernel finds the last kept one among them. Every other row (large top-k, a step of too
-//      many elements, rejected parameters): the sampler's cluster kernel.
+//      many elements, rejected parameters): the sampler's cluster kernel. Rows of kinds that the caller does not
+//      name but allows (PB_VERIFY_REST): pb_sample_ws's or the cluster kernel, whichever is launched.
 //   3. decide_kernel: a CTA per sequence finds the first rejected row.
 //   4. mass_kernel: that row's mass, where it has no filters.
 //   5. weigh_kernel: that row's weights, summed per tile (256 vectors), a CTA per segment.
