@@ -1139,12 +1139,14 @@ __global__ void __launch_bounds__(VT, 2) decide_kernel(VerifyArgs a) {
             }
             const uint64_t px = (kept || ev == EV_TIE) ? weight_q(y, f.max_key) : 0;
             const double want = a.probs ? __dmul_rn(d.u, (double)d.prob) : d.u, p = __ull2double_rn(px);
-            if (row_is == ROW_WHOLE) {
+            if (want < 0.0) {  // below any weight, be it 0
+              ok = true;
+              ev = -1;
+            } else if (row_is == ROW_WHOLE) {
               // (what fp64's own roundings add is far below the bounds' slack)
               const Mass z = mass_near(a, r, tf, value_of(a.meta[r].max_key), f.max_key);
-              // (a negative product is below any weight; with no lower bound on the mass it would not show)
-              ok = want < 0.0 || want * z.lo < p;
-              if (ok && !(want < 0.0) && !(want * z.hi < p)) ev = EV_TIE;
+              ok = want * z.lo < p;
+              if (ok && !(want * z.hi < p)) ev = EV_TIE;
             } else {
               ok = __dmul_rn(want, __ull2double_rn(f.kept_q)) < p;
               if (ev == EV_TIE && !ok) ev = EV_REJECT;  // rejected either way

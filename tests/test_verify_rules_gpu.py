@@ -79,3 +79,18 @@ def test_negative_shares_of_drafts_without_weight(cuda, temperature):
     probs[torch.arange(S), torch.from_numpy(drafts[0::2])] = torch.tensor([-0.5, -1e-30, 0.0, 0.5, -torch.inf, torch.nan, -1.0, 1e-30])
     for u in (0.0, 2.0**-53, 0.5, 1.0 - 2.0**-53):
         _check(x, [(temperature, 1.0, 0)] * S, [1] * S, drafts, np.full(2 * S, u), probs)
+
+
+@pytest.mark.parametrize("V", [24, 704, 5003])
+def test_negative_shares_of_drafts_cut_among_equals(cuda, V):
+    """... a draft among the equals of the last kept value, where top-p cuts them, being one without weight."""
+    S = 12
+    x = torch.zeros(2 * S, V)
+    x[:, ::3] = 1.0
+    params = [(1.0, (0.3, 0.6)[s % 2], (0, 50, V - 1)[s % 3]) for s in range(S)]
+    drafts = np.repeat(np.arange(S) * 3 % V, 2).astype(np.int64)
+    drafts[0::4] = (V - 1) // 3 * 3  # the last of the equals
+    probs = torch.full((S, V), 1.0 / V)
+    probs[:, :] = torch.tensor([-1.0, -1e-30, 1e-30])[torch.arange(S) // 4, None]
+    for u in (0.0, 0.25, 1.0 - 2.0**-53):
+        _check(x, params, [1] * S, drafts, np.full(2 * S, u), probs)
