@@ -14,7 +14,7 @@ The rule, its arithmetic and the order of the draws are stated at ``pb_verify`` 
 
 from __future__ import annotations
 
-import ctypes
+import functools
 from collections.abc import Sequence
 
 import numpy as np
@@ -51,8 +51,8 @@ def _check_probs(draft_probs: torch.Tensor | None, n: int, vocab: int) -> None:
     _check_dtype("draft_probs", draft_probs)
 
 
-def _check(logits, params, drafts, row_offsets, uniforms, draft_probs) -> int:
-    """Refuses what the kernels do not take; the number of sequences."""
+def _check(logits, params, drafts, row_offsets, uniforms, draft_probs):
+    """Refuses what the kernels do not take; rows, vocabulary, sequences and the device."""
     if not logits.is_cuda:
         raise ValueError("pagedbatch_b200.verify needs CUDA logits; move the tensor with .cuda() first")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
@@ -74,13 +74,16 @@ def _check(logits, params, drafts, row_offsets, uniforms, draft_probs) -> int:
     _check_probs(draft_probs, R - S, V)
     if S == 0 and R:
         raise ValueError(f"{R} rows for no sequence")
-    return S
+    return R, V, S, dev
+
+
+@functools.lru_cache(maxsize=256)
+def _ws_bytes(rows: int, seqs: int, vocab: int, dtype: int, kinds: int) -> int:
+    return _lib.load().pb_verify_ws_bytes(rows, seqs, vocab, dtype, kinds)
 
 
 def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=None):
-    S = _check(logits, params, drafts, row_offsets, uniforms, draft_probs)
-    R, V = logits.shape
-    dev = logits.device
+    R, V, S, dev = _check(logits, params, drafts, row_offsets, uniforms, draft_probs)
     tokens = torch.empty(R, dtype=torch.int64, device=dev)
     accepted = torch.empty(S, dtype=torch.int32, device=dev)
     status = torch.empty(S, dtype=torch.int32, device=dev)
@@ -92,7 +95,7 @@ def _launch(logits, params, drafts, row_offsets, uniforms, draft_probs, noted=No
         # a buffer of this call's own: the allocator hands it on in stream order, and a captured
         # graph keeps its copy
         kinds = _kinds(params, noted, V)
-        n_ws = L.pb_verify_ws_bytes(R, S, V, code, kinds)
+        n_ws = _ws_bytes(R, S, V, code, kinds)
         ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
         rc = L.pb_verify(
             logits.data_ptr(), code, R, V, logits.stride(0) if R > 1 else V, params.data_ptr(), S,
@@ -123,13 +126,13 @@ def verify_with_status_op(
 
 @verify_op.register_fake
 def _(logits, params, drafts, row_offsets, uniforms, draft_probs=None):
-    s = _check(logits, params, drafts, row_offsets, uniforms, draft_probs)
+    _, _, s, _ = _check(logits, params, drafts, row_offsets, uniforms, draft_probs)
     return logits.new_empty((logits.shape[0],), dtype=torch.int64), logits.new_empty((s,), dtype=torch.int32)
 
 
 @verify_with_status_op.register_fake
 def _(logits, params, drafts, row_offsets, uniforms, draft_probs=None):
-    s = _check(logits, params, drafts, row_offsets, uniforms, draft_probs)
+    _, _, s, _ = _check(logits, params, drafts, row_offsets, uniforms, draft_probs)
     return (logits.new_empty((logits.shape[0],), dtype=torch.int64), logits.new_empty((s,), dtype=torch.int32),
             logits.new_empty((s,), dtype=torch.int32))
 
