@@ -16,7 +16,8 @@
 // (from L2); their values at or above it are the candidates, a little more than k, put in order by
 // counting for each the candidates before it, or where they are many by a bitonic network. A row with more
 // candidates than the list holds, nearly all of them equal as a mask makes them, has those above that
-// value listed and the first of its equals added; any other is selected by bisection over (value, index).
+// value listed and the first of its equals added; any other is selected by bisection over (value, index), as are
+// rows of fewer groups than k and more elements than the list (k 223, 587 rows of 13394 bf16: 457 us).
 // HBM-bound: V * es bytes a row, and 1/32 of that written as keys. [1024, 128256] bf16, k 128: 77 us, the
 // read's floor 41 us; one CTA or cluster a row, which selects while others read, took 187 us.
 #include "pb_rows.cuh"
