@@ -95,7 +95,8 @@ def _backward(z, lp, idx, weight, stats, temperature, grad_loss):
 
 @torch.library.custom_op("pagedbatch_b200::distill_loss", mutates_args=())
 def distill_op(student_logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_indices: torch.Tensor,
-               row_weight: torch.Tensor | None, temperature: float, tail: bool, total: bool) -> tuple[torch.Tensor, torch.Tensor]:
+               row_weight: torch.Tensor | None, temperature: float, tail: bool,
+               total: bool) -> tuple[torch.Tensor, torch.Tensor]:
     """The rows' losses (or their sum) and their statistics."""
     prepared = _prepare(student_logits, teacher_logprobs, teacher_indices, row_weight, temperature)
     loss, buf = _forward(student_logits, *prepared, tail, total)
